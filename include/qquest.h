@@ -272,6 +272,126 @@ int qq_moe_experts(const qq_moe_plan* plan, const void* x, int64_t x_stride, int
                    const void* const* w_gate, const void* const* w_up, const void* const* w_down, void* h_buf,
                    void* y_buf, void* out, int64_t out_stride, uint32_t* err, void* stream);
 
+/* ---- block tables and slots, made on the device ------------------------ */
+/* Request r holds held[r] blocks of block_size tokens (16, 32, 64 or 128):
+ * position p lives in block block_table[r][p / block_size] at offset
+ * p % block_size, its slot is block * block_size + offset.  Free blocks wait in
+ * a ring: taken at free_blocks[ring[0] % capacity], given back at
+ * free_blocks[ring[1] % capacity], both counts only growing.  claim is
+ * zero-filled once and zero again after every call.  Calls on one set of
+ * tables are ordered on one stream.  No reference counterpart: the reference
+ * hands out single rows on the host (ReqToTokenPool and
+ * TokenToKVPoolAllocator, memory.py:28-76). */
+typedef struct qq_block_tables {
+  int32_t* block_table; /* device [max_reqs][table_stride], max_blocks entries used per row */
+  int64_t table_stride;
+  int32_t* held;        /* device [max_reqs] */
+  int32_t* claim;       /* device [max_reqs], 0 between calls */
+  int32_t* free_blocks; /* device [capacity] */
+  int64_t* ring;        /* device [2]: blocks taken, blocks given (all time) */
+  int32_t capacity;
+  int32_t max_reqs;
+  int32_t max_blocks;
+  int32_t block_size;
+} qq_block_tables;
+
+/* The blocks and slots of a step: entry i's request grows from prefix_lens[i] to
+ * seq_lens[i] tokens, taking the blocks it does not hold yet from the ring in
+ * batch order.  token_offsets ([bs + 1]) receives the exclusive sums of the
+ * new tokens, slots[token_offsets[i] + t] the slot of position prefix + t, and
+ * slots behind the last new token -1 (num_slots is what the caller made room
+ * for; more new tokens than that are QQ_DEV_ERR_BOUNDS).  req_to_token (null:
+ * none; int32 [map_rows][map_stride]) gets the same slots by request and
+ * position, the table the page selection translates through.  An entry of
+ * seq_lens 0 is padding.  A request past the ring's free blocks (the sum in
+ * batch order) gets none, slots of -1 and QQ_DEV_ERR_CAPACITY; a bad length, a
+ * request out of range or named a second time likewise with
+ * QQ_DEV_ERR_BOUNDS.  bs <= QQ_MAX_BS. */
+int qq_block_plan(const qq_block_tables* tables, const int64_t* req_pool_indices, const int64_t* seq_lens,
+                  const int64_t* prefix_lens, int bs, int64_t* slots, int64_t num_slots, int64_t* token_offsets,
+                  int32_t* req_to_token, int64_t map_stride, int64_t map_rows, uint32_t* err, void* stream);
+
+/* Entry i's request keeps the blocks of its first keep_lens[i] tokens (null:
+ * none, the request is finished); the others go back to the ring in batch
+ * order, their table entries become -1.  A request of -1 is padding; errors as above. */
+int qq_block_trim(const qq_block_tables* tables, const int64_t* req_pool_indices, const int64_t* keep_lens, int bs,
+                  uint32_t* err, void* stream);
+
+/* ---- KV cache in 8 bits ------------------------------------------------ */
+/* One layer: e4m3 codes [num_blocks][kv_heads][block_size][head_dim] and fp32
+ * scales [num_blocks][kv_heads]; a value is its code times the scale of its
+ * block and head.  block_size 16, 32, 64 or 128, head_dim a multiple of 8 up
+ * to 256, codes 16-byte aligned, num_blocks * kv_heads * block_size < 2^31.
+ * state (device [2 + num_blocks], zero-filled once) is needed by
+ * qq_kv8_append alone.  No reference counterpart: the reference keeps K and V
+ * in the model's dtype (MHATokenToKVPool, memory.py:79-120). */
+typedef struct qq_kv8_cache {
+  uint8_t* k;
+  uint8_t* v;
+  float* k_scale;
+  float* v_scale;
+  uint32_t* state;
+  int32_t num_blocks;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t block_size;
+} qq_kv8_cache;
+
+/* Quantises token t's keys and values (row t of k / v, [kv_heads][head_dim],
+ * k_stride / v_stride elements between tokens, rows and pointers 16-byte
+ * aligned) into slot slots[t]; -1 skips a token.  Per block and head the scale
+ * is the smallest power of two s with amax <= 448 s over the finite values
+ * written, or the block's scale before where that is larger; the codes the
+ * block holds are requantised when it grows.  A token at offset 0 starts its
+ * block anew.  Infinities are stored as +-448 s, NaN as NaN.  The tokens of a
+ * block stand next to each other in ascending slots: a block met twice in one
+ * call, like a slot out of range, is QQ_DEV_ERR_BOUNDS and one of the two
+ * stretches is not written.  Calls on one layer are ordered on one stream. */
+int qq_kv8_append(const qq_kv8_cache* cache, const void* k, const void* v, int dtype, int64_t k_stride,
+                  int64_t v_stride, const int64_t* slots, int64_t num_tokens, uint32_t* err, void* stream);
+
+/* k_out / v_out [num_tokens][kv_heads][head_dim] (contiguous, 16-byte aligned) <- the
+ * values of the slots; -1 gives zeros, a slot out of range zeros and QQ_DEV_ERR_BOUNDS. */
+int qq_kv8_gather(const qq_kv8_cache* cache, const int64_t* slots, int64_t num_tokens, void* k_out, void* v_out,
+                  int dtype, uint32_t* err, void* stream);
+
+/* Bytes of device scratch (16-byte aligned, any content) the attention calls
+ * below need: max_keys is table_stride * block_size, or top_k; num_tokens the
+ * query rows.  Each call's scratch is its own while it runs. */
+size_t qq_kv8_workspace_bytes(const qq_kv8_cache* cache, int q_heads, int dtype, int bs, int64_t num_tokens,
+                              int64_t max_keys, int extend);
+
+/* out[i] ([q_heads][head_dim], the query dtype) = attention of q[i] over the
+ * seq_lens[i] cached tokens of request req_pool_indices[i]; query head h reads
+ * KV head h / (q_heads / kv_heads); fp32 scores, softmax and sums.  seq_lens 0
+ * gives zeros (padding); a length past the table or a request out of range
+ * gives zeros and QQ_DEV_ERR_BOUNDS; a block out of range takes no part and
+ * is reported too.  bf16 with head_dim 128 and up to 16 query heads per KV
+ * head runs on the tensor cores, anything else on the fp32 units. */
+int qq_kv8_decode_attention(const qq_kv8_cache* cache, const qq_batch* batch, const int32_t* block_table,
+                            int64_t table_stride, int64_t table_rows, const void* q, int dtype, int q_heads,
+                            int64_t q_stride, float scaling, void* out, int64_t out_stride, uint32_t* err,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
+/* The same over the slots rows[i][0 .. lens[i]) (duplicates counted; a
+ * negative row takes no part), as qq_quest_retrieve_topk and a req_to_token
+ * made by qq_block_plan give them. */
+int qq_kv8_sparse_attention(const qq_kv8_cache* cache, int bs, const int32_t* rows, int64_t rows_stride, int top_k,
+                            const int32_t* lens, const void* q, int dtype, int q_heads, int64_t q_stride,
+                            float scaling, void* out, int64_t out_stride, uint32_t* err, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* Causal attention of an extend batch: row token_offsets[i] + t of q (t <
+ * seq_lens[i] - prefix_lens[i]) attends to positions 0 .. prefix_lens[i] + t
+ * of its request, read through block_table (the new tokens are in the cache
+ * already).  out_cache_loc and max_seq_len are not read.  Rows behind the
+ * last sequence are left as they were, like those of an entry whose lengths,
+ * offset or request do not fit (QQ_DEV_ERR_BOUNDS). */
+int qq_kv8_extend_attention(const qq_kv8_cache* cache, const qq_extend_batch* batch, const int32_t* block_table,
+                            int64_t table_stride, int64_t table_rows, const void* q, int dtype, int q_heads,
+                            int64_t q_stride, float scaling, void* out, int64_t out_stride, uint32_t* err,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- [Q3] per-step bounds fold + finalize ----------------------------- */
 #define QQ_STEP_FOLD 1     /* running min/max <- key of the previous token */
 #define QQ_STEP_FINALIZE 2 /* finalize pages whose 64th token arrived, advance counters */

@@ -10,7 +10,9 @@ plus :class:`~qwenquest_b200.quest.QuestAlgorithm` and
 APIs, and :class:`~qwenquest_b200.graphs.DecodeStepGraph` (a decode step
 captured in a CUDA graph); :class:`~qwenquest_b200.moe.B200SparseMoeBlock` and
 :func:`~qwenquest_b200.moe.install_moe` (the model's MoE blocks on the tensor
-cores).  All decode work runs in hand-written CUDA kernels in ``libqquest.so``
+cores); :class:`~qwenquest_b200.kv8.KV8Cache` and
+:class:`~qwenquest_b200.kv8.BlockTables` (a KV cache in 8 bits with its block
+tables and attention).  All decode work runs in hand-written CUDA kernels in ``libqquest.so``
 (C ABI: ``include/qquest.h``); nothing falls back to the CPU.  Importing this
 package does not load the library; the first backend / algorithm object does.
 """
@@ -21,8 +23,10 @@ __all__ = [
     "B200QuestHiSparseBackend",
     "B200QuestOnlyBackend",
     "B200SparseMoeBlock",
+    "BlockTables",
     "DecodeStepGraph",
     "HiSparseCoordinator",
+    "KV8Cache",
     "QuestAlgorithm",
     "QuestTrace",
     "install_moe",
@@ -38,6 +42,10 @@ def __getattr__(name):
         from qwenquest_b200 import moe
 
         return getattr(moe, name)
+    if name in ("BlockTables", "KV8Cache"):
+        from qwenquest_b200 import kv8
+
+        return getattr(kv8, name)
     if name == "DecodeStepGraph":
         from qwenquest_b200.graphs import DecodeStepGraph
 

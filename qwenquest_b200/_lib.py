@@ -114,6 +114,35 @@ class QQMoePlan(ctypes.Structure):
     ]
 
 
+class QQKv8Cache(ctypes.Structure):
+    _fields_ = [
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("k_scale", c_void_p),
+        ("v_scale", c_void_p),
+        ("state", c_void_p),
+        ("num_blocks", c_int32),
+        ("kv_heads", c_int32),
+        ("head_dim", c_int32),
+        ("block_size", c_int32),
+    ]
+
+
+class QQBlockTables(ctypes.Structure):
+    _fields_ = [
+        ("block_table", c_void_p),
+        ("table_stride", c_int64),
+        ("held", c_void_p),
+        ("claim", c_void_p),
+        ("free_blocks", c_void_p),
+        ("ring", c_void_p),
+        ("capacity", c_int32),
+        ("max_reqs", c_int32),
+        ("max_blocks", c_int32),
+        ("block_size", c_int32),
+    ]
+
+
 class QQHostRing(ctypes.Structure):
     _fields_ = [("rows", c_void_p), ("state", c_void_p), ("capacity", c_int64)]
 
@@ -140,6 +169,8 @@ _H = POINTER(QQHiSparseState)
 _E = POINTER(QQExtendBatch)
 _HB = POINTER(QQHotBuffer)
 _PP = POINTER(c_void_p)
+_C8 = POINTER(QQKv8Cache)
+_BT = POINTER(QQBlockTables)
 
 #: every exported symbol with its (restype, argtypes); tests check the list
 #: against include/qquest.h
@@ -164,6 +195,23 @@ SIGNATURES: dict[str, tuple] = {
     "qq_moe_experts": (
         c_int, [POINTER(QQMoePlan), c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                 c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
+    "qq_block_plan": (
+        c_int, [_BT, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64,
+                c_void_p, c_void_p]),
+    "qq_block_trim": (c_int, [_BT, c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
+    "qq_kv8_append": (
+        c_int, [_C8, c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p]),
+    "qq_kv8_gather": (c_int, [_C8, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
+    "qq_kv8_workspace_bytes": (c_size_t, [_C8, c_int, c_int, c_int, c_int64, c_int64, c_int]),
+    "qq_kv8_decode_attention": (
+        c_int, [_C8, _B, c_void_p, c_int64, c_int64, c_void_p, c_int, c_int, c_int64, c_float, c_void_p, c_int64,
+                c_void_p, c_void_p, c_size_t, c_void_p]),
+    "qq_kv8_sparse_attention": (
+        c_int, [_C8, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int, c_int, c_int64, c_float, c_void_p,
+                c_int64, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "qq_kv8_extend_attention": (
+        c_int, [_C8, _E, c_void_p, c_int64, c_int64, c_void_p, c_int, c_int, c_int64, c_float, c_void_p, c_int64,
+                c_void_p, c_void_p, c_size_t, c_void_p]),
     "qq_quest_decode_step": (
         c_int, [_S, c_int, c_int, c_int, _PP, c_int, c_int64, _B, c_void_p, c_void_p, _T, c_int64,
                 c_void_p, c_size_t, c_void_p]),
@@ -260,9 +308,11 @@ def ptr_array(ptrs: list[int]):
 
 __all__ = [
     "QQBatch",
+    "QQBlockTables",
     "QQError",
     "QQExtendBatch",
     "QQHiSparseState",
+    "QQKv8Cache",
     "QQMoePlan",
     "QQHotBuffer",
     "QQNewToken",

@@ -1,0 +1,627 @@
+// The 8-bit block KV cache: its tables and slots, made on the GPU from request
+// lengths, and the quantising write with its read-back.
+//
+// Tables.  Request r holds held[r] blocks, block_table[r][0 .. held[r]); free
+// blocks wait in a ring (taken at its head, given back at its tail), so which
+// block a request gets depends on the order of calls alone.  A step's batch
+// grows requests (qq_block_plan) or shrinks them (qq_block_trim) without a
+// host round trip, so both can be captured in a graph.
+//
+// Quantisation.  Per block and KV head a power of two s = 2^k, k the smallest
+// with amax <= 448 * 2^k over the finite values written; a value is stored as
+// e4m3(x / s), to nearest even.  A power of two costs no accuracy in a
+// floating-point code (the significand is kept; values below 2^-6 s lose bits,
+// at most one binade earlier than with amax / 448) and makes growth exact:
+// when a later token needs a larger scale, the codes the block holds are
+// multiplied by s_old / s_new, which changes their exponents only and rounds
+// none but those that fall below 2^-6 of the new scale.
+
+#include <climits>
+
+#include <cuda_fp16.h>
+
+#include "kv8.cuh"
+
+namespace qq {
+namespace {
+
+using namespace kv8;
+
+// ------------------------------------------------------------------ tables
+
+struct TableArgs {
+  int32_t* table;
+  int64_t stride;
+  int32_t* held;
+  int32_t* claim;
+  int32_t* free_blocks;
+  int64_t* ring;
+  int capacity, max_reqs, max_blocks, shift;
+  const int64_t* reqs;
+  const int64_t* seq;     // plan: lengths with the new tokens; trim: tokens to keep (null: none)
+  const int64_t* prefix;  // plan: lengths before them
+  int bs;
+  int64_t* slots;
+  int64_t num_slots;
+  int64_t* offsets;
+  int32_t* map;
+  int64_t map_stride, map_rows;
+  uint32_t* err;
+};
+
+constexpr int kTableThreads = 1024;
+constexpr int kTablePer = QQ_MAX_BS / kTableThreads;  // batch entries per thread at most
+
+// Shared arrays of bs entries each (plus one for the two prefix sums).
+struct TableSmem {
+  int64_t* off;   // [bs + 1] new tokens before entry i
+  int32_t* sum;   // [bs + 1] blocks moved before entry i
+  int32_t* req;   // -1: nothing to do for this entry
+  int32_t* held;
+  int64_t* pre;
+};
+__host__ __device__ inline size_t table_smem_bytes(int bs) { return (size_t)(bs + 1) * 12 + (size_t)bs * 16 + 16; }
+__device__ inline TableSmem table_smem(void* p, int bs) {
+  TableSmem s;
+  s.off = static_cast<int64_t*>(p);
+  s.pre = s.off + bs + 1;
+  s.sum = reinterpret_cast<int32_t*>(s.pre + bs);
+  s.req = s.sum + bs + 1;
+  s.held = s.req + bs;
+  return s;
+}
+
+// Exclusive sums over the block of one (int64, int32) pair per thread; totals to all threads.
+__device__ void block_scan(int64_t& a, int32_t& b, int64_t& a_total, int32_t& b_total) {
+  __shared__ int64_t sa[32];
+  __shared__ int32_t sb[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t ia = a;
+  int32_t ib = b;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t ua = __shfl_up_sync(0xffffffffu, ia, o);
+    const int32_t ub = __shfl_up_sync(0xffffffffu, ib, o);
+    if (lane >= o) ia += ua, ib += ub;
+  }
+  if (lane == 31) sa[warp] = ia, sb[warp] = ib;
+  __syncthreads();
+  if (warp == 0) {
+    int64_t wa = sa[lane];
+    int32_t wb = sb[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t ua = __shfl_up_sync(0xffffffffu, wa, o);
+      const int32_t ub = __shfl_up_sync(0xffffffffu, wb, o);
+      if (lane >= o) wa += ua, wb += ub;
+    }
+    sa[lane] = wa, sb[lane] = wb;
+  }
+  __syncthreads();
+  a_total = sa[31], b_total = sb[31];
+  a = ia - a + (warp ? sa[warp - 1] : 0);
+  b = ib - b + (warp ? sb[warp - 1] : 0);
+}
+
+// The last i in [0, n) with sums[i] <= x (sums ascending, sums[0] <= x).
+template <typename V>
+__device__ __forceinline__ int last_at_most(const V* sums, int n, V x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (sums[mid] <= x) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// A request that the batch names twice is served for its first entry only: the
+// claim word of a request takes the largest bs - i (0 between launches).
+__device__ __forceinline__ void claim_requests(const TableArgs& a) {
+  for (int i = threadIdx.x; i < a.bs; i += kTableThreads) {
+    const int64_t r = a.reqs[i];
+    if (r >= 0 && r < a.max_reqs) atomicMax(a.claim + r, a.bs - i);
+  }
+  __syncthreads();
+}
+__device__ __forceinline__ void release_claims(const TableArgs& a) {
+  for (int i = threadIdx.x; i < a.bs; i += kTableThreads) {
+    const int64_t r = a.reqs[i];
+    if (r >= 0 && r < a.max_reqs) a.claim[r] = 0;
+  }
+}
+
+// Latency-bound: a step's batch is a few thousand integers.  kState: this CTA
+// updates the tables (one CTA); kSlots: the grid writes the slots.  Every CTA
+// reads the lengths and sums them itself, so the slots need no second pass
+// over the tables: a page the request does not hold yet is found in the ring.
+template <bool kState, bool kSlots>
+__global__ void __launch_bounds__(kTableThreads) block_plan_kernel(TableArgs a) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  __shared__ int s_taken;
+  const TableSmem s = table_smem(smem_raw, a.bs);
+  const int tid = threadIdx.x;
+  const int block = 1 << a.shift;
+  if (tid == 0) s_taken = 0;
+  claim_requests(a);
+  const int64_t head = a.ring[0], free_count = a.ring[1] - head;
+
+  // ---- this thread's entries: new tokens and blocks to take
+  int64_t toks[kTablePer], my_toks = 0;
+  int32_t need[kTablePer], my_need = 0;
+  const int per = (a.bs + kTableThreads - 1) / kTableThreads;
+#pragma unroll
+  for (int j = 0; j < kTablePer; ++j) {
+    const int i = tid * per + j;
+    toks[j] = 0, need[j] = 0;
+    if (j >= per || i >= a.bs) continue;
+    const int64_t r = a.reqs[i], seq = a.seq[i], pre = a.prefix[i];
+    int32_t req = -1, held = 0;
+    if (seq != 0) {  // 0: a padding entry
+      bool good = pre >= 0 && seq >= pre;
+      if (good) toks[j] = seq - pre;
+      good = good && r >= 0 && r < a.max_reqs && seq <= ((int64_t)a.max_blocks << a.shift);
+      if (good) good = ld_volatile_s32(a.claim + r) == a.bs - i;
+      if (good) {
+        req = (int32_t)r;
+        held = a.held[r];
+        good = held >= 0 && held <= a.max_blocks;
+      }
+      if (good) need[j] = max(0, (int32_t)((seq + block - 1) >> a.shift) - held);
+      else req = -1;
+      if (!good) raise_error(a.err, QQ_DEV_ERR_BOUNDS);
+    }
+    s.req[i] = req;
+    s.held[i] = held;
+    s.pre[i] = pre;
+    my_toks += toks[j];
+    my_need += need[j];
+  }
+  int64_t tok_at = my_toks, tok_total;
+  int32_t need_at = my_need, need_total;
+  block_scan(tok_at, need_at, tok_total, need_total);
+#pragma unroll
+  for (int j = 0; j < kTablePer; ++j) {
+    const int i = tid * per + j;
+    if (j >= per || i >= a.bs) continue;
+    s.off[i] = tok_at;
+    s.sum[i] = need_at;
+    tok_at += toks[j];
+    need_at += need[j];
+    if (need[j] > 0) {
+      if (need_at <= free_count) {
+        atomicMax(&s_taken, need_at);
+      } else {  // the ring runs out: this request stays as it was
+        s.req[i] = -1;
+        raise_error(a.err, QQ_DEV_ERR_CAPACITY);
+      }
+    }
+  }
+  if (tid == 0) {
+    s.off[a.bs] = tok_total;
+    s.sum[a.bs] = need_total;
+    if (tok_total > a.num_slots) raise_error(a.err, QQ_DEV_ERR_BOUNDS);
+  }
+  __syncthreads();
+
+  if (kSlots) {
+    if (blockIdx.x == 0)
+      for (int i = tid; i <= a.bs; i += kTableThreads) a.offsets[i] = s.off[i];
+    for (int64_t t = (int64_t)blockIdx.x * kTableThreads + tid; t < a.num_slots; t += (int64_t)gridDim.x * kTableThreads) {
+      int64_t slot = -1;
+      if (t < tok_total) {
+        const int e = last_at_most(s.off, a.bs, t);
+        const int32_t req = s.req[e];
+        if (req >= 0) {
+          const int64_t pos = s.pre[e] + t - s.off[e];
+          const int32_t page = (int32_t)(pos >> a.shift);
+          const int32_t b = page < s.held[e]
+                                ? a.table[req * a.stride + page]
+                                : a.free_blocks[(head + s.sum[e] + page - s.held[e]) % a.capacity];
+          if (b >= 0) {
+            slot = ((int64_t)b << a.shift) | (pos & (block - 1));
+            if (a.map != nullptr) {
+              if (req < a.map_rows && pos < a.map_stride && slot <= INT_MAX) a.map[req * a.map_stride + pos] = (int32_t)slot;
+              else raise_error(a.err, QQ_DEV_ERR_BOUNDS);
+            }
+          } else {
+            raise_error(a.err, QQ_DEV_ERR_BOUNDS);
+          }
+        }
+      }
+      a.slots[t] = slot;
+    }
+  }
+  if (kState) {
+    __syncthreads();  // the slots above read the tables as they were
+    for (int o = tid; o < s_taken; o += kTableThreads) {
+      const int e = last_at_most(s.sum, a.bs, o);
+      a.table[s.req[e] * a.stride + s.held[e] + o - s.sum[e]] = a.free_blocks[(head + o) % a.capacity];
+    }
+    for (int i = tid; i < a.bs; i += kTableThreads) {
+      if (s.req[i] >= 0) a.held[s.req[i]] = s.held[i] + s.sum[i + 1] - s.sum[i];
+    }
+    release_claims(a);
+    if (tid == 0) a.ring[0] = head + s_taken;
+  }
+}
+
+__global__ void __launch_bounds__(kTableThreads) block_trim_kernel(TableArgs a) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  const TableSmem s = table_smem(smem_raw, a.bs);
+  const int tid = threadIdx.x;
+  const int block = 1 << a.shift;
+  claim_requests(a);
+  const int64_t tail = a.ring[1], room = a.capacity - (tail - a.ring[0]);
+  int32_t back[kTablePer], my_back = 0;
+  const int per = (a.bs + kTableThreads - 1) / kTableThreads;
+#pragma unroll
+  for (int j = 0; j < kTablePer; ++j) {
+    const int i = tid * per + j;
+    back[j] = 0;
+    if (j >= per || i >= a.bs) continue;
+    const int64_t r = a.reqs[i], keep = a.seq == nullptr ? 0 : a.seq[i];
+    int32_t req = -1, held = 0;
+    if (r != -1) {  // -1: a padding entry
+      bool good = r >= 0 && r < a.max_reqs && keep >= 0;
+      if (good) good = ld_volatile_s32(a.claim + r) == a.bs - i;
+      if (good) {
+        req = (int32_t)r;
+        held = a.held[r];
+        good = held >= 0 && held <= a.max_blocks;
+      }
+      if (good && keep < ((int64_t)held << a.shift)) back[j] = held - (int32_t)((keep + block - 1) >> a.shift);
+      if (!good) req = -1, raise_error(a.err, QQ_DEV_ERR_BOUNDS);
+    }
+    s.req[i] = req;
+    s.held[i] = held;
+    my_back += back[j];
+  }
+  int64_t none = 0, none_total;
+  int32_t at = my_back, total;
+  block_scan(none, at, none_total, total);
+#pragma unroll
+  for (int j = 0; j < kTablePer; ++j) {
+    const int i = tid * per + j;
+    if (j >= per || i >= a.bs) continue;
+    s.sum[i] = at;
+    at += back[j];
+  }
+  if (tid == 0) s.sum[a.bs] = total;
+  __syncthreads();
+  if (total > room) {  // more blocks than the ring was made for: a table that names blocks it does not own
+    if (tid == 0) raise_error(a.err, QQ_DEV_ERR_BOUNDS);
+  } else {
+    for (int o = tid; o < total; o += kTableThreads) {
+      const int e = last_at_most(s.sum, a.bs, o);
+      // entry e gives back pages [held - back, held), ascending
+      const int32_t page = s.held[e] - (s.sum[e + 1] - s.sum[e]) + o - s.sum[e];
+      int32_t* p = a.table + s.req[e] * a.stride + page;
+      a.free_blocks[(tail + o) % a.capacity] = *p;
+      *p = -1;
+    }
+    for (int i = tid; i < a.bs; i += kTableThreads)
+      if (s.req[i] >= 0) a.held[s.req[i]] = s.held[i] - (s.sum[i + 1] - s.sum[i]);
+    if (tid == 0) a.ring[1] = tail + total;
+  }
+  release_claims(a);
+}
+
+// ------------------------------------------------------------------ append
+
+struct AppendArgs {
+  Cache c;
+  const void* k;
+  const void* v;
+  int64_t k_stride, v_stride;  // elements between tokens
+  const int64_t* slots;
+  int64_t n;
+  int window;  // tokens whose runs a CTA takes
+  uint32_t* err;
+};
+
+constexpr int kAppendWarps = 8;
+constexpr int kMaxWindow = 64;
+
+// A run is a stretch of tokens whose slots ascend by one inside a block; its
+// first token's CTA quantises it, a warp per (K or V, head): one pass over
+// the run's values for the maximum, one (from L2) that stores the codes.
+// Bound by the values' bytes for a prefill and by the chain slots -> values ->
+// maximum -> codes for a decode step.
+// Two runs of one call that meet in a block would race: a run claims its block
+// with the call's epoch, and the one that finds the epoch there is skipped and
+// reported.  The epoch lives in state[0] and the last CTA to leave advances
+// it, so a captured call gets a new one with every replay.
+template <typename T>
+__global__ void __launch_bounds__(kAppendWarps * 32) kv8_append_kernel(AppendArgs a) {
+  __shared__ int64_t s_slots[kMaxWindow + kMaxBlock + 1];
+  __shared__ int s_conflict;
+  const Cache& c = a.c;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t w0 = (int64_t)blockIdx.x * a.window;
+  const int64_t total = (int64_t)c.num_blocks << c.shift;
+  // s_slots[i] is the slot of token w0 - 1 + i (-1 outside the batch)
+  for (int i = tid; i < a.window + c.block + 1; i += kAppendWarps * 32) {
+    const int64_t t = w0 - 1 + i;
+    s_slots[i] = t >= 0 && t < a.n ? a.slots[t] : -1;
+  }
+  const uint32_t epoch = ld_volatile_u32(c.state) + 1;
+  __syncthreads();
+  const int chunks = c.dim >> 3;  // 8-element pieces of a row
+  const int last = (int)min((int64_t)a.window, a.n - w0);
+  for (int u = 0; u < last; ++u) {
+    const int64_t slot = s_slots[u + 1], prev = s_slots[u];
+    if (slot < 0) continue;  // a padding token
+    if (slot >= total) {
+      if (tid == 0) raise_error(a.err, QQ_DEV_ERR_BOUNDS);
+      continue;
+    }
+    const int off = (int)(slot & (c.block - 1));
+    if (off != 0 && prev == slot - 1) continue;  // inside a run
+    const int32_t b = (int32_t)(slot >> c.shift);
+    int n = 0;  // the run's tokens
+    for (int base = 0; base < c.block; base += 32) {
+      const int i = base + lane;
+      const bool in = off + i < c.block && s_slots[u + 1 + i] == slot + i;
+      const uint32_t m = __ballot_sync(0xffffffffu, in);
+      if (m != 0xffffffffu) {
+        n = base + __ffs(~m) - 1;
+        break;
+      }
+      n = base + 32;
+    }
+    __syncthreads();  // s_conflict of the run before has been read
+    if (tid == 0) s_conflict = atomicExch(c.state + 2 + b, epoch) == epoch;
+    __syncthreads();
+    if (s_conflict) {
+      if (tid == 0) raise_error(a.err, QQ_DEV_ERR_BOUNDS);
+      continue;
+    }
+    const int64_t t0 = w0 + u;
+    for (int p = warp; p < 2 * c.kv_heads; p += kAppendWarps) {
+      const bool is_v = p >= c.kv_heads;
+      const int h = is_v ? p - c.kv_heads : p;
+      const int64_t stride = is_v ? a.v_stride : a.k_stride;
+      const T* src = static_cast<const T*>(is_v ? a.v : a.k) + t0 * stride + (int64_t)h * c.dim;
+      const int64_t bh = (int64_t)b * c.kv_heads + h;
+      uint8_t* codes = (is_v ? c.v : c.k) + bh * c.block * c.dim;
+      float* scale = (is_v ? c.v_scale : c.k_scale) + bh;
+      const float old = off == 0 ? 0.f : *scale;
+      const int items = n * chunks;
+      float most = 0.f;
+#pragma unroll 4
+      for (int i = lane; i < items; i += 32) {
+        const int r = i / chunks;
+        float x[8];
+        load8(src + r * stride + (i - r * chunks) * 8, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float m = fabsf(x[e]);
+          if (m <= 3.402823466e38f) most = fmaxf(most, m);  // infinities and NaN set no scale
+        }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      // most = 1.m * 2^E <= 1.75 * 2^8 * 2^k
+      const uint32_t bits = __float_as_uint(most);
+      const int e2 = max((int)(bits >> 23) - 127 - ((bits & 0x7FFFFFu) <= 0x600000u ? 8 : 7), -126);
+      const float now = fmaxf(old, __uint_as_float((uint32_t)(e2 + 127) << 23));
+      if (off != 0 && now != old) {  // the codes already here, in steps of the larger scale
+        const float ratio = __fdiv_rn(old, now);
+        for (int i = lane; i < c.block * chunks; i += 32) {
+          const int r = i / chunks;
+          if (r >= off && r < off + n) continue;
+          uint2* p8 = reinterpret_cast<uint2*>(codes + (int64_t)i * 8);
+          float x[8];
+          from_e4m3x8(*p8, x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] *= ratio;
+          *p8 = make_uint2(e4m3x2(x[0], x[1]) | (e4m3x2(x[2], x[3]) << 16),
+                           e4m3x2(x[4], x[5]) | (e4m3x2(x[6], x[7]) << 16));
+        }
+      }
+      if (lane == 0) *scale = now;
+      // dividing by a power of two is multiplying by its inverse; a scale the caller brought may be any number
+      const uint32_t nb = __float_as_uint(now);
+      const bool pow2 = (nb & 0x7FFFFFu) == 0 && nb != 0;
+      const float inv = __fdiv_rn(1.f, now);
+      uint8_t* dst = codes + (int64_t)off * c.dim;
+#pragma unroll 4
+      for (int i = lane; i < items; i += 32) {
+        const int r = i / chunks;
+        float x[8];
+        load8(src + r * stride + (i - r * chunks) * 8, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = pow2 ? x[e] * inv : __fdiv_rn(x[e], now);
+        *reinterpret_cast<uint2*>(dst + (int64_t)i * 8) = make_uint2(
+            e4m3x2(x[0], x[1]) | (e4m3x2(x[2], x[3]) << 16), e4m3x2(x[4], x[5]) | (e4m3x2(x[6], x[7]) << 16));
+      }
+    }
+  }
+  // the epoch advances once every CTA has read it
+  if (tid == 0) {
+    __threadfence();
+    if (atomicAdd(c.state + 1, 1u) == gridDim.x - 1) {
+      c.state[1] = 0;
+      c.state[0] = epoch == 0xFFFFFFFFu ? 0u : epoch;  // 0 is never an epoch: the claims start at 0
+    }
+  }
+}
+
+// ------------------------------------------------------------------ gather
+
+// out[i] = the values of slot slots[i] (code times scale): 8 elements per
+// thread and step, bound by the bytes.  A slot of -1 gives zeros.
+template <typename T>
+__global__ void __launch_bounds__(256) kv8_gather_kernel(Cache c, const int64_t* slots, int64_t n, T* k_out, T* v_out,
+                                                         uint32_t* err) {
+  const int chunks = c.dim >> 3, row = c.kv_heads * chunks;
+  const int64_t total = (int64_t)c.num_blocks << c.shift;
+  const int64_t items = n * row;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < items; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t t = i / row;
+    const int w = (int)(i - t * row);
+    const int h = w / chunks, ch = w - h * chunks;
+    const int64_t slot = slots[t];
+    float kx[8] = {}, vx[8] = {};
+    if (slot >= 0 && slot < total) {
+      const int64_t bh = (slot >> c.shift) * c.kv_heads + h;
+      const int64_t at = (bh * c.block + (slot & (c.block - 1))) * c.dim + ch * 8;
+      const float ks = c.k_scale[bh], vs = c.v_scale[bh];
+      from_e4m3x8(*reinterpret_cast<const uint2*>(c.k + at), kx);
+      from_e4m3x8(*reinterpret_cast<const uint2*>(c.v + at), vx);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) kx[e] *= ks, vx[e] *= vs;
+    } else if (slot != -1) {
+      raise_error(err, QQ_DEV_ERR_BOUNDS);
+    }
+    store8(k_out + i * 8, kx);
+    store8(v_out + i * 8, vx);
+  }
+}
+
+int check_tables(const qq_block_tables* t, int bs, const int64_t* reqs) {
+  if (t == nullptr || t->block_table == nullptr || t->held == nullptr || t->claim == nullptr ||
+      t->free_blocks == nullptr || t->ring == nullptr || t->capacity <= 0 || t->max_reqs <= 0 || t->max_blocks <= 0 ||
+      t->table_stride < t->max_blocks || bs < 0 || (bs > 0 && reqs == nullptr))
+    return QQ_ERR_INVALID;
+  if (bs > QQ_MAX_BS ||
+      (t->block_size != 16 && t->block_size != 32 && t->block_size != 64 && t->block_size != 128))
+    return QQ_ERR_UNSUPPORTED;
+  return QQ_OK;
+}
+
+TableArgs table_args(const qq_block_tables& t, const int64_t* reqs, int bs, uint32_t* err) {
+  TableArgs a{};
+  a.table = t.block_table;
+  a.stride = t.table_stride;
+  a.held = t.held;
+  a.claim = t.claim;
+  a.free_blocks = t.free_blocks;
+  a.ring = t.ring;
+  a.capacity = t.capacity;
+  a.max_reqs = t.max_reqs;
+  a.max_blocks = t.max_blocks;
+  while ((1 << a.shift) < t.block_size) ++a.shift;
+  a.reqs = reqs;
+  a.bs = bs;
+  a.err = err;
+  return a;
+}
+
+// Up to this many slots one CTA makes the whole plan; past it the slots take a grid of their own.
+constexpr int64_t kOneCtaSlots = 4096;
+
+}  // namespace
+}  // namespace qq
+
+extern "C" int qq_block_plan(const qq_block_tables* tables, const int64_t* req_pool_indices, const int64_t* seq_lens,
+                             const int64_t* prefix_lens, int bs, int64_t* slots, int64_t num_slots,
+                             int64_t* token_offsets, int32_t* req_to_token, int64_t map_stride, int64_t map_rows,
+                             uint32_t* err, void* stream) {
+  using namespace qq;
+  int rc = check_tables(tables, bs, req_pool_indices);
+  if (rc != QQ_OK) return rc;
+  if (token_offsets == nullptr || num_slots < 0 || (num_slots > 0 && slots == nullptr) ||
+      (bs > 0 && (seq_lens == nullptr || prefix_lens == nullptr)) ||
+      (req_to_token != nullptr && (map_stride <= 0 || map_rows <= 0)))
+    return QQ_ERR_INVALID;
+  TableArgs a = table_args(*tables, req_pool_indices, bs, err);
+  a.seq = seq_lens;
+  a.prefix = prefix_lens;
+  a.slots = slots;
+  a.num_slots = num_slots;
+  a.offsets = token_offsets;
+  a.map = req_to_token;
+  a.map_stride = map_stride;
+  a.map_rows = map_rows;
+  static SmemLimit one, wide, state;
+  const size_t smem = table_smem_bytes(bs);
+  cudaStream_t s = as_stream(stream);
+  if (num_slots <= kOneCtaSlots) {
+    if ((rc = one.ensure((const void*)block_plan_kernel<true, true>, smem)) != QQ_OK) return rc;
+    block_plan_kernel<true, true><<<1, kTableThreads, smem, s>>>(a);
+    return launch_status();
+  }
+  if ((rc = wide.ensure((const void*)block_plan_kernel<false, true>, smem)) != QQ_OK) return rc;
+  if ((rc = state.ensure((const void*)block_plan_kernel<true, false>, smem)) != QQ_OK) return rc;
+  const int64_t ctas = (num_slots + kTableThreads - 1) / kTableThreads;
+  const int most = device_sm_count();
+  block_plan_kernel<false, true><<<(unsigned)(ctas < most ? ctas : most), kTableThreads, smem, s>>>(a);
+  if ((rc = launch_status()) != QQ_OK) return rc;
+  a.err = nullptr;  // what is wrong has been reported
+  block_plan_kernel<true, false><<<1, kTableThreads, smem, s>>>(a);
+  return launch_status();
+}
+
+extern "C" int qq_block_trim(const qq_block_tables* tables, const int64_t* req_pool_indices, const int64_t* keep_lens,
+                             int bs, uint32_t* err, void* stream) {
+  using namespace qq;
+  int rc = check_tables(tables, bs, req_pool_indices);
+  if (rc != QQ_OK || bs == 0) return rc;
+  TableArgs a = table_args(*tables, req_pool_indices, bs, err);
+  a.seq = keep_lens;
+  static SmemLimit limit;
+  const size_t smem = table_smem_bytes(bs);
+  if ((rc = limit.ensure((const void*)block_trim_kernel, smem)) != QQ_OK) return rc;
+  block_trim_kernel<<<1, kTableThreads, smem, as_stream(stream)>>>(a);
+  return launch_status();
+}
+
+extern "C" int qq_kv8_append(const qq_kv8_cache* cache, const void* k, const void* v, int dtype, int64_t k_stride,
+                             int64_t v_stride, const int64_t* slots, int64_t num_tokens, uint32_t* err, void* stream) {
+  using namespace qq;
+  int rc = kv8::check(cache);
+  if (rc != QQ_OK) return rc;
+  if (num_tokens < 0 || cache->state == nullptr || (dtype != QQ_BF16 && dtype != QQ_F32)) return QQ_ERR_INVALID;
+  if (num_tokens == 0) return QQ_OK;
+  const int64_t row = (int64_t)cache->kv_heads * cache->head_dim;
+  if (k == nullptr || v == nullptr || slots == nullptr || k_stride < row || v_stride < row) return QQ_ERR_INVALID;
+  const int size = dtype == QQ_BF16 ? 2 : 4;
+  if ((k_stride * size) % 16 != 0 || (v_stride * size) % 16 != 0 || reinterpret_cast<uintptr_t>(k) % 16 != 0 ||
+      reinterpret_cast<uintptr_t>(v) % 16 != 0)
+    return QQ_ERR_UNSUPPORTED;
+  AppendArgs a{};
+  a.c = kv8::view(*cache);
+  a.k = k;
+  a.v = v;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.slots = slots;
+  a.n = num_tokens;
+  a.err = err;
+  // A CTA per token while there are few (each may be its own run); windows of
+  // more tokens for a prefill, whose runs are whole blocks.
+  a.window = 1;
+  while (a.window < kMaxWindow && num_tokens > 512 * (int64_t)a.window) a.window *= 2;
+  const int64_t ctas = (num_tokens + a.window - 1) / a.window;
+  if (ctas > INT32_MAX) return QQ_ERR_UNSUPPORTED;
+  cudaStream_t s = as_stream(stream);
+  if (dtype == QQ_BF16) kv8_append_kernel<__nv_bfloat16><<<(unsigned)ctas, kAppendWarps * 32, 0, s>>>(a);
+  else kv8_append_kernel<float><<<(unsigned)ctas, kAppendWarps * 32, 0, s>>>(a);
+  return launch_status();
+}
+
+extern "C" int qq_kv8_gather(const qq_kv8_cache* cache, const int64_t* slots, int64_t num_tokens, void* k_out,
+                             void* v_out, int dtype, uint32_t* err, void* stream) {
+  using namespace qq;
+  const int rc = kv8::check(cache);
+  if (rc != QQ_OK) return rc;
+  if (num_tokens < 0 || (dtype != QQ_BF16 && dtype != QQ_F32)) return QQ_ERR_INVALID;
+  if (num_tokens == 0) return QQ_OK;
+  if (slots == nullptr || k_out == nullptr || v_out == nullptr) return QQ_ERR_INVALID;
+  if (reinterpret_cast<uintptr_t>(k_out) % 16 != 0 || reinterpret_cast<uintptr_t>(v_out) % 16 != 0)
+    return QQ_ERR_UNSUPPORTED;
+  const kv8::Cache c = kv8::view(*cache);
+  const int64_t items = num_tokens * c.kv_heads * (c.dim >> 3);
+  const int64_t most = (int64_t)device_sm_count() * 32;
+  const int64_t ctas = (items + 255) / 256 < most ? (items + 255) / 256 : most;
+  cudaStream_t s = as_stream(stream);
+  if (dtype == QQ_BF16)
+    kv8_gather_kernel<<<(unsigned)ctas, 256, 0, s>>>(c, slots, num_tokens, static_cast<__nv_bfloat16*>(k_out),
+                                                     static_cast<__nv_bfloat16*>(v_out), err);
+  else
+    kv8_gather_kernel<<<(unsigned)ctas, 256, 0, s>>>(c, slots, num_tokens, static_cast<float*>(k_out),
+                                                     static_cast<float*>(v_out), err);
+  return launch_status();
+}

@@ -1,0 +1,129 @@
+// What the attention kernels over the 8-bit block cache share: their
+// arguments, and how a key's place and a row's output are found.
+#pragma once
+
+#include "kv8.cuh"
+
+namespace qq {
+namespace kv8 {
+
+// Which keys a batch entry attends to.
+enum Keys : int {
+  kTable = 0,   // one query token per entry, positions [0, seq) through the block table
+  kRows = 1,    // one query token per entry, the listed rows
+  kExtend = 2,  // an entry's new tokens, causal, through the block table
+};
+
+struct AttnArgs {
+  Cache c;
+  int bs;
+  const int64_t* reqs;     // kTable, kExtend
+  const int64_t* seq;      // kTable, kExtend: keys of the entry
+  const int64_t* prefix;   // kExtend: keys before the new tokens
+  const int64_t* offsets;  // kExtend: first query row of each entry
+  const int32_t* table;    // [table_rows][table_stride]
+  int64_t table_stride, table_rows;
+  const int32_t* rows;     // kRows: [bs][rows_stride]
+  int64_t rows_stride;
+  const int32_t* lens;     // kRows
+  int top;                 // kRows: listed rows per entry at most
+  int64_t tokens;          // query rows
+  const void* q;
+  int64_t q_stride;        // elements between query rows
+  void* out;
+  int64_t out_stride;
+  int heads, group;
+  float scale_log2;        // scaling * log2(e)
+  float* part;             // split partials
+  uint32_t* err;
+};
+
+// The keys of one-token entry `e`; 0 when there is nothing to attend to (a
+// bad entry is reported by the caller that passes err and attends to nothing).
+template <int KEYS>
+__device__ __forceinline__ int64_t entry_keys(const AttnArgs& a, int e, uint32_t* err) {
+  if (KEYS == kRows) {
+    const int32_t n = a.lens[e];
+    if (n >= 0 && n <= a.top) return n;
+    raise_error(err, QQ_DEV_ERR_BOUNDS);
+    return 0;
+  }
+  const int64_t n = a.seq[e];
+  if (n == 0) return 0;  // a padding entry
+  const int64_t r = a.reqs[e];
+  if (n > 0 && n <= a.table_stride << a.c.shift && r >= 0 && r < a.table_rows) return n;
+  raise_error(err, QQ_DEV_ERR_BOUNDS);
+  return 0;
+}
+
+// An extend entry's query tile: `n` new tokens at rows `row0`, keys before them `prefix`.
+struct ExtendEntry {
+  int entry;      // -1: no such tile
+  int64_t tile;   // which tile of the entry
+  int64_t row0, n, prefix;
+};
+
+// Tile `x` of the batch's tiles of `rows` new tokens each; called by one whole warp, the same in every lane.
+// A bad entry has no tiles and is reported.
+__device__ __forceinline__ ExtendEntry extend_tile(const AttnArgs& a, int64_t x, int rows, uint32_t* err) {
+  ExtendEntry r{-1, 0, 0, 0, 0};
+  const int lane = threadIdx.x & 31;
+  int64_t before = 0;
+  for (int e0 = 0; e0 < a.bs; e0 += 32) {
+    const int e = e0 + lane;
+    int64_t n = 0, row0 = 0, pre = 0;
+    if (e < a.bs) {
+      const int64_t seq = a.seq[e];
+      row0 = a.offsets[e];
+      pre = a.prefix[e];
+      if (seq != 0) {  // 0: a padding entry
+        const int64_t req = a.reqs[e];
+        n = seq - pre;
+        const bool good = pre >= 0 && n >= 0 && row0 >= 0 && row0 <= a.tokens && n <= a.tokens - row0 &&
+                          seq <= a.table_stride << a.c.shift && req >= 0 && req < a.table_rows;
+        if (!good) {
+          raise_error(err, QQ_DEV_ERR_BOUNDS);
+          n = 0;
+        }
+      }
+    }
+    const int64_t tiles = (n + rows - 1) / rows;
+    int64_t incl = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t u = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += u;
+    }
+    const int64_t excl = before + incl - tiles;
+    const uint32_t m = __ballot_sync(0xffffffffu, x >= excl && x < excl + tiles);
+    if (m != 0) {
+      const int src = __ffs(m) - 1;
+      r.entry = e0 + src;
+      r.tile = x - __shfl_sync(0xffffffffu, excl, src);
+      r.row0 = __shfl_sync(0xffffffffu, row0, src);
+      r.n = __shfl_sync(0xffffffffu, n, src);
+      r.prefix = __shfl_sync(0xffffffffu, pre, src);
+      return r;
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return r;
+}
+
+// The slot of key `j` of entry `e`, -1 when it takes no part (a bad block or row is reported).
+template <int KEYS>
+__device__ __forceinline__ int64_t key_slot(const AttnArgs& a, int e, int64_t req, int64_t j, uint32_t* err) {
+  if (KEYS == kRows) {
+    const int32_t r = a.rows[(int64_t)e * a.rows_stride + j];
+    if (r < 0) return -1;  // a padding row
+    if (r < (int64_t)a.c.num_blocks << a.c.shift) return r;
+  } else {
+    const int32_t b = a.table[req * a.table_stride + (j >> a.c.shift)];
+    if (b >= 0 && b < a.c.num_blocks) return ((int64_t)b << a.c.shift) | (j & (a.c.block - 1));
+  }
+  raise_error(err, QQ_DEV_ERR_BOUNDS);
+  return -1;
+}
+
+}  // namespace kv8
+}  // namespace qq

@@ -28,8 +28,10 @@ from dataclasses import dataclass
 import torch
 
 from qwenquest_b200 import _lib
+from qwenquest_b200._device import DeviceError as _DeviceError
+from qwenquest_b200._device import dtype_code, host_device_pointer, stream_of
 from qwenquest_b200._lib import QQ_STEP_FINALIZE, QQ_STEP_FOLD, check
-from qwenquest_b200.quest import QuestAlgorithm, dtype_code, stream_of
+from qwenquest_b200.quest import QuestAlgorithm
 
 __all__ = ["DeviceHostRows", "HiSparseCoordinator", "SwapInStats"]
 
@@ -59,15 +61,6 @@ class SwapInStats:
 
     def __repr__(self) -> str:
         return f"SwapInStats(hits={self.hits}, misses={self.misses}, fast_path_calls={self.fast_path_calls})"
-
-
-def host_device_pointer(t: torch.Tensor) -> int:
-    """Device address of a pinned host tensor (``cudaHostGetDevicePointer``)."""
-    if not t.is_pinned():
-        raise ValueError("the host tier must be pinned memory")
-    out = ctypes.c_void_p()
-    check(_lib.load().qq_host_device_pointer(t.data_ptr(), ctypes.byref(out)), "host_device_pointer")
-    return int(out.value)
 
 
 _DeviceErrorLike = "_DeviceError"
@@ -118,23 +111,6 @@ class DeviceHostRows:
         pos = (tail + torch.arange(n, device=self.device)) % self.size
         self.rows[pos] = idx
         self.state[1] = tail + n
-
-
-@dataclass
-class _DeviceError:
-    word: torch.Tensor  # pinned host int32 [1]; kernels OR error bits into it
-    dev_ptr: int = 0
-
-    def ptr(self) -> int:
-        if not self.dev_ptr:
-            self.dev_ptr = host_device_pointer(self.word)
-        return self.dev_ptr
-
-    def take(self) -> int:
-        bits = int(self.word[0])
-        if bits:
-            self.word.zero_()
-        return bits
 
 
 @dataclass

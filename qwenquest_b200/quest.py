@@ -27,24 +27,13 @@ import torch
 from qwenquest.quest import QuestSelection, QuestTrace  # the reference's own records
 
 from qwenquest_b200 import _lib
+from qwenquest_b200._device import dtype_code, stream_of
 from qwenquest_b200._lib import QQ_BF16, QQ_F32, QQ_STEP_FINALIZE, QQ_STEP_FOLD, check
 
 __all__ = ["QuestAlgorithm", "QuestSelection", "QuestTrace", "StepLayout"]
 
 _BF16_POS_INF = torch.finfo(torch.bfloat16).max
 _BF16_NEG_INF = torch.finfo(torch.bfloat16).min
-
-
-def dtype_code(dtype: torch.dtype) -> int:
-    if dtype == torch.bfloat16:
-        return QQ_BF16
-    if dtype == torch.float32:
-        return QQ_F32
-    raise ValueError(f"unsupported dtype {dtype}: the kernels take bfloat16 or float32")
-
-
-def stream_of(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
 
 
 class StepLayout:
