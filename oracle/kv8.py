@@ -77,17 +77,20 @@ def rows(codes: np.ndarray, scales: np.ndarray, slots: np.ndarray) -> np.ndarray
     return out
 
 
-def attend(q: np.ndarray, k: np.ndarray, v: np.ndarray, scaling: float):
-    """One query ``q`` [heads, dim] over ``k``, ``v`` [n, kv, dim]: ``(out, weight, spread)``, all float64.
+def attend(q: np.ndarray, k: np.ndarray, v: np.ndarray, scaling: float, v_scale: np.ndarray | None = None):
+    """One query ``q`` [heads, dim] over ``k``, ``v`` [n, kv, dim]: ``(out, weight, spread, small)``, all float64.
 
-    ``out`` [heads, dim]; ``weight`` [heads, dim] = sum_j w_j |v_j| (what errors of the weights are measured
-    by); ``spread`` [heads] = max_j scaling * sum_d |q_d k_jd| (what errors of the scores are).
+    ``out`` [heads, dim]; ``weight`` [heads, dim] = sum_j w_j |v_j| (what relative errors of the weights are
+    measured by); ``spread`` [heads] = max_j scaling * sum_d |q_d k_jd| (what errors of the scores are);
+    ``small`` [heads, dim] = max_j (w_j s_j) sum_j |v_j| / s_j with the scales s_j = ``v_scale`` [n, kv] (what
+    errors of the weights relative to the row's largest scaled weight are).
     """
     heads, dim = q.shape
     n, kv, _ = k.shape
     out, weight, spread = np.zeros((heads, dim)), np.zeros((heads, dim)), np.zeros(heads)
+    small = np.zeros((heads, dim))
     if n == 0:
-        return out, weight, spread
+        return out, weight, spread, small
     for h in range(heads):
         kh, vh = k[:, h // (heads // kv)], v[:, h // (heads // kv)]
         s = kh @ q[h].astype(np.float64) * scaling
@@ -96,7 +99,10 @@ def attend(q: np.ndarray, k: np.ndarray, v: np.ndarray, scaling: float):
         out[h] = w @ vh
         weight[h] = w @ np.abs(vh)
         spread[h] = (np.abs(kh) @ np.abs(q[h].astype(np.float64))).max() * scaling
-    return out, weight, spread
+        if v_scale is not None:
+            s_h = v_scale[:, h // (heads // kv)].astype(np.float64)
+            small[h] = (w * s_h).max() * (np.abs(vh) / s_h[:, None]).sum(0)
+    return out, weight, spread, small
 
 
 class Tables:

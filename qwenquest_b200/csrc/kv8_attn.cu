@@ -275,7 +275,8 @@ int launch_any(AnyArgs g, int64_t tiles, cudaStream_t s) {
   return launch_status();
 }
 
-int run_any(const AttnArgs& a, int keys, int dtype, int64_t max_keys, size_t ws_bytes, cudaStream_t s) {
+int run(const AttnArgs& a, int keys, int dtype, int64_t max_keys, size_t ws_bytes, cudaStream_t s) {
+  if (keys != kExtend && decode_tc_fits(a, dtype)) return run_decode_tc(a, keys, max_keys, ws_bytes, s);
   AnyArgs g = any_shape(a, keys);
   const int64_t tiles = any_tiles(g, keys, a.bs, a.tokens);
   if (tiles > INT32_MAX || (int64_t)a.c.kv_heads * g.chunks > 65535) return QQ_ERR_UNSUPPORTED;
@@ -331,8 +332,15 @@ extern "C" size_t qq_kv8_workspace_bytes(const qq_kv8_cache* cache, int q_heads,
   AnyArgs g = any_shape(a, keys);
   const int64_t tiles = any_tiles(g, keys, bs, num_tokens);
   g.splits = any_splits(g, tiles, a.c.kv_heads, max_keys);
-  if (g.splits <= 1) return 0;
-  return sizeof(float) * (size_t)(tiles * a.c.kv_heads * g.chunks * g.splits * any_record(a.c.dim));
+  size_t need = 0;
+  if (g.splits > 1)
+    need = sizeof(float) * (size_t)(tiles * a.c.kv_heads * g.chunks * g.splits * any_record(a.c.dim));
+  // enough for either kernel: which one runs depends on the pointers' alignment too
+  if (keys != kExtend && decode_tc_fits(a, dtype)) {
+    const size_t tc = decode_tc_workspace(bs, a.c.kv_heads, a.group, max_keys);
+    if (tc > need) need = tc;
+  }
+  return need;
 }
 
 extern "C" int qq_kv8_decode_attention(const qq_kv8_cache* cache, const qq_batch* batch, const int32_t* block_table,
@@ -356,7 +364,7 @@ extern "C" int qq_kv8_decode_attention(const qq_kv8_cache* cache, const qq_batch
   a.table_stride = table_stride;
   a.table_rows = table_rows;
   a.tokens = a.bs;
-  return run_any(a, kTable, dtype, table_stride << a.c.shift, workspace_bytes, as_stream(stream));
+  return run(a, kTable, dtype, table_stride << a.c.shift, workspace_bytes, as_stream(stream));
 }
 
 extern "C" int qq_kv8_sparse_attention(const qq_kv8_cache* cache, int bs, const int32_t* rows, int64_t rows_stride,
@@ -377,7 +385,7 @@ extern "C" int qq_kv8_sparse_attention(const qq_kv8_cache* cache, int bs, const 
   a.lens = lens;
   a.top = top_k;
   a.tokens = bs;
-  return run_any(a, kRows, dtype, top_k, workspace_bytes, as_stream(stream));
+  return run(a, kRows, dtype, top_k, workspace_bytes, as_stream(stream));
 }
 
 extern "C" int qq_kv8_extend_attention(const qq_kv8_cache* cache, const qq_extend_batch* batch,
@@ -404,5 +412,5 @@ extern "C" int qq_kv8_extend_attention(const qq_kv8_cache* cache, const qq_exten
   a.table_stride = table_stride;
   a.table_rows = table_rows;
   a.tokens = batch->num_tokens;
-  return run_any(a, kExtend, dtype, table_stride << a.c.shift, workspace_bytes, as_stream(stream));
+  return run(a, kExtend, dtype, table_stride << a.c.shift, workspace_bytes, as_stream(stream));
 }

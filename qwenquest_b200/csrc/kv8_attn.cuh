@@ -125,5 +125,11 @@ __device__ __forceinline__ int64_t key_slot(const AttnArgs& a, int e, int64_t re
   return -1;
 }
 
+// The tensor-core kernel for one query token per entry (kTable, kRows): whether
+// it takes these arguments, the scratch it needs, and its launch.
+bool decode_tc_fits(const AttnArgs& a, int dtype);
+size_t decode_tc_workspace(int bs, int kv_heads, int group, int64_t max_keys);
+int run_decode_tc(const AttnArgs& a, int keys, int64_t max_keys, size_t ws_bytes, cudaStream_t s);
+
 }  // namespace kv8
 }  // namespace qq

@@ -7,8 +7,9 @@ W = sum_j w_j |v_j| and S the largest sum_d |q_d k_jd| * scaling of its keys,
   (head_dim + 8) 2^-24 S, which moves a weight by at most twice that, relatively (its own and the sum's),
   and 2^x itself by 2^-22 (2 ulp), also twice;
 * n products are summed in fp32: n 2^-24 W at most, and the row sum the same relative to itself;
-* on the tensor cores the weights are held as two e4m3 numbers: half a step 2^-4 of half a step 2^-4, that is 2^-8
-  relatively, or 2^-21 of the row's largest weight where they fall below the type's normal range; the sum keeps fp32 weights;
+* on the tensor cores the weights (times the scale of V) are held as two e4m3 numbers: half a step 2^-4 of half a
+  step 2^-4, that is 2^-8 relatively, or where the second falls below the type's normal range a fixed part of the row's
+  largest: one token per request 2^-10 / 16 of 128 at least, 2^-21; the row's sum keeps the fp32 weights;
 * the result is rounded once: half a step, 2^-8 in bf16 and 2^-24 in fp32.
 """
 
@@ -359,12 +360,17 @@ def test_no_tokens_is_no_work():
 # ---------------------------------------------------------------- attention
 
 
-def _tolerance(dtype, n, dim, out, weight, spread):
+SMALL_DECODE = 2.0 ** -21
+SMALL_EXTEND = SMALL_DECODE
+
+
+def _tolerance(dtype, n, dim, out, weight, spread, small, part):
     rel = 2 * (dim + 8) * 2.0 ** -24 * spread[:, None] + 2 * 2.0 ** -22 + 2 * n * 2.0 ** -24
+    err = rel * weight
     if dtype == torch.bfloat16:
-        rel = rel + 2.0 ** -8 + n * 2.0 ** -21
+        err = err + 2.0 ** -8 * weight + part * small
     step = torch.finfo(dtype).eps / 2
-    return step * np.abs(out) + (1 + step) * rel * weight + 1e-37
+    return step * np.abs(out) + (1 + step) * err + 1e-37
 
 
 class _Batch:
@@ -405,12 +411,13 @@ class _Batch:
         p = np.asarray(positions)
         return self.table[self.reqs[i], p // self.block] * self.block + p % self.block
 
-    def check(self, got, q, slots):
+    def check(self, got, q, slots, part=SMALL_DECODE):
         k, v = (oracle.rows(c, s, slots) for c, s in ((self.k[0], self.ks[0]), (self.v[0], self.vs[0])))
         q = q.double().numpy()
-        out, weight, spread = oracle.attend(q, k, v, self.scaling)
+        scale = self.vs[0][slots // self.block]
+        out, weight, spread, small = oracle.attend(q, k, v, self.scaling, scale)
         err = np.abs(got.double().cpu().numpy().reshape(out.shape) - out)
-        tol = _tolerance(self.dtype, len(slots), self.dim, out, weight, spread)
+        tol = _tolerance(self.dtype, len(slots), self.dim, out, weight, spread, small, part)
         assert (err <= tol).all(), (float((err - tol).max()), float((err / tol).max()))
 
 
@@ -485,7 +492,7 @@ def test_extend_attention_matches_64_bits(kv, heads, dim, block, dtype, seq, new
             if n > 64 and offsets[i] + t not in probe and t not in (0, m - 1):
                 continue
             row = offsets[i] + t
-            b.check(out[row], q[row], b.slots(i, np.arange(s - m + t + 1)))
+            b.check(out[row], q[row], b.slots(i, np.arange(s - m + t + 1)), SMALL_EXTEND)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
@@ -512,7 +519,7 @@ def test_attention_with_scales_far_apart(dtype):
     b.cache.synchronize()
     for i, s in enumerate(seq):
         b.check(out[i], q[i], b.slots(i, np.arange(s)))
-        b.check(ext[i], q[i], b.slots(i, np.arange(s)))
+        b.check(ext[i], q[i], b.slots(i, np.arange(s)), SMALL_EXTEND)
         b.check(sparse[i], q[i], rows[i, :(130, 77)[i]])
 
 
@@ -528,7 +535,7 @@ def test_attention_of_unequal_queries(dtype, heads):
     ext = b.cache.extend_attention(0, q.to(DEV), b.table_dev, _dev(b.reqs), _dev(seq), _dev([399]), _dev([0]), b.scaling)
     b.cache.synchronize()
     b.check(out[0], q[0], b.slots(0, np.arange(400)))
-    b.check(ext[0], q[0], b.slots(0, np.arange(400)))
+    b.check(ext[0], q[0], b.slots(0, np.arange(400)), SMALL_EXTEND)
 
 
 def test_a_nan_reaches_the_heads_that_see_it_and_no_others():
@@ -570,7 +577,7 @@ def test_attention_reports_bad_entries_and_serves_the_others():
             assert bool((ext[1] == 7.0).all())
             for i in (0, 2):
                 b.check(out[i], q[i], b.slots(i, np.arange(seq[i])))
-                b.check(ext[i], q[i], b.slots(i, np.arange(seq[i])))
+                b.check(ext[i], q[i], b.slots(i, np.arange(seq[i])), SMALL_EXTEND)
         # a block out of range takes no part
         broken = b.table_dev.clone()
         broken[b.reqs[1], 0] = 1 << 20
@@ -586,7 +593,7 @@ def test_attention_reports_bad_entries_and_serves_the_others():
         for i in range(3):
             left = np.arange(64 if i == 1 else 0, seq[i])
             b.check(out[i], q[i], b.slots(i, left))
-            b.check(ext[i], q[i], b.slots(i, left))
+            b.check(ext[i], q[i], b.slots(i, left), SMALL_EXTEND)
         rows = np.stack([b.slots(i, np.arange(64)) for i in range(3)])
         rows[1, 10] = 1 << 30
         out = b.cache.sparse_decode_attention(0, q.to(DEV), _dev(rows, torch.int32), _dev([64, 64, 65], torch.int32),
@@ -612,9 +619,12 @@ def test_attention_takes_strided_queries_tables_and_outputs():
         out = b.cache.decode_attention(0, q, wide[:, ::2], b.reqs.tolist(), seq, b.scaling, out=room[:, 128:-128])
         odd = torch.empty(2 * 8 * 128 + 1, dtype=dtype, device=DEV)[1:].view(2, 8, 128)
         odd.copy_(q)
-        same = b.cache.decode_attention(0, odd, b.table_dev, _dev(b.reqs), _dev(seq), b.scaling, out=odd.view(2, -1))
+        odd_out = torch.empty(2 * 8 * 128 + 1, dtype=dtype, device=DEV)[1:].view(2, 8 * 128)
+        b.cache.decode_attention(0, odd, b.table_dev, _dev(b.reqs), _dev(seq), b.scaling, out=odd_out)
         b.cache.synchronize()
-        assert torch.equal(out, want) and torch.equal(same, want)
+        assert torch.equal(out, want)
+        for i, n in enumerate(seq):  # an unaligned result is another kernel's
+            b.check(odd_out[i], q[i].cpu(), b.slots(i, np.arange(n)))
         assert room[:, :128].count_nonzero() == 0 and room[:, -128:].count_nonzero() == 0
 
 
@@ -697,9 +707,9 @@ def test_a_captured_step_replays_over_new_lengths():
             pos = np.arange(seq[r])
             at = ref.table[r, pos // block] * block + pos % block
             kk, vv = oracle.rows(k_ref, ks_ref, at), oracle.rows(v_ref, vs_ref, at)
-            out, weight, spread = oracle.attend(q[r].double().cpu().numpy(), kk, vv, dim ** -0.5)
-            tol = _tolerance(torch.bfloat16, len(at), dim, out, weight, spread)
-            for got in (one, two):
+            out, *bounds = oracle.attend(q[r].double().cpu().numpy(), kk, vv, dim ** -0.5, vs_ref[at // block])
+            for got, part in ((one, SMALL_DECODE), (two, SMALL_EXTEND)):
+                tol = _tolerance(torch.bfloat16, len(at), dim, out, *bounds, part)
                 assert (np.abs(got[r].double().cpu().numpy().reshape(out.shape) - out) <= tol).all()
 
 
@@ -772,6 +782,6 @@ def test_selection_over_the_8_bit_cache():
         at = mapped[i].cpu().numpy()[pos]
         assert at.tolist() == rows[i, :len(pos)].tolist()
         kk, vv = (oracle.rows(c, s, at.astype(np.int64)) for c, s in zip(codes, scales))
-        want, weight, spread = oracle.attend(q[i].double().cpu().numpy(), kk, vv, dim ** -0.5)
-        tol = _tolerance(torch.bfloat16, len(at), dim, want, weight, spread)
+        want, *bounds = oracle.attend(q[i].double().cpu().numpy(), kk, vv, dim ** -0.5, scales[1][at // page])
+        tol = _tolerance(torch.bfloat16, len(at), dim, want, *bounds, SMALL_DECODE)
         assert (np.abs(out[i].double().cpu().numpy().reshape(want.shape) - want) <= tol).all()
