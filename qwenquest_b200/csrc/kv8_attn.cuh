@@ -48,9 +48,8 @@ __device__ __forceinline__ int64_t entry_keys(const AttnArgs& a, int e, uint32_t
     raise_error(err, QQ_DEV_ERR_BOUNDS);
     return 0;
   }
-  const int64_t n = a.seq[e];
+  const int64_t n = a.seq[e], r = a.reqs[e];
   if (n == 0) return 0;  // a padding entry
-  const int64_t r = a.reqs[e];
   if (n > 0 && n <= a.table_stride << a.c.shift && r >= 0 && r < a.table_rows) return n;
   raise_error(err, QQ_DEV_ERR_BOUNDS);
   return 0;

@@ -63,8 +63,24 @@ enum : int {
   kNumBars = kBarDone + 1
 };
 
-// Tile lo of share c of `ctas`.
-__host__ __device__ __forceinline__ int64_t share_lo(int64_t total, int64_t c, int64_t ctas) { return total * c / ctas; }
+// The tiles in equal shares: the first `more` shares have one tile more.
+struct Shares {
+  int64_t ctas, each, more;
+  __device__ __forceinline__ Shares(int64_t total, int64_t grid) {
+    ctas = min(grid, total);  // no share is empty
+    if (total <= UINT32_MAX) {
+      each = (uint32_t)total / max(1u, (uint32_t)ctas);
+    } else {
+      each = total / ctas;
+    }
+    more = total - each * ctas;
+  }
+  __device__ __forceinline__ int64_t lo(int64_t c) const { return c * each + min(c, more); }
+  __device__ __forceinline__ int64_t owner(int64_t tile) const {  // the share that tile lies in
+    const int64_t cut = more * (each + 1);
+    return tile < cut ? tile / (each + 1) : more + (tile - cut) / each;
+  }
+};
 
 // Steps through a share's tiles: entry e, head h, tile t of the entry's T.  The next entry's length is loaded one
 // entry ahead.
@@ -93,9 +109,29 @@ struct Walk {
   }
 };
 
+// N values per lane reduced over the warp's lanes (N 8 or 16): lanes hold halves
+// of the values in turn, so lane L ends with value L / (32 / N) in N + 1 shuffles.
+template <int N, typename Op>
+__device__ __forceinline__ float reduce_lanes(float (&x)[N], int lane, Op op) {
+  int m = 16;
+#pragma unroll
+  for (int n = N; n > 1; n >>= 1, m >>= 1) {
+#pragma unroll
+    for (int i = 0; i < n / 2; ++i) {
+      const bool up = (lane & m) != 0;
+      const float send = up ? x[i] : x[i + n / 2], keep = up ? x[i + n / 2] : x[i];
+      x[i] = op(keep, __shfl_xor_sync(0xffffffffu, send, m));
+    }
+  }
+#pragma unroll
+  for (; m > 0; m >>= 1) x[0] = op(x[0], __shfl_xor_sync(0xffffffffu, x[0], m));
+  return x[0];
+}
+
 struct DecodeArgs {
   AttnArgs a;
-  int slots;  // 16 KiB slots of the code ring
+  int slots;        // 16 KiB slots of the code ring
+  int64_t* before;  // [bs + 1] tiles of the entries before each, left by CTA 0 for the join
 };
 
 __host__ __device__ constexpr int64_t record_floats(int heads) { return heads * (2 + (int64_t)kTcDim); }
@@ -129,7 +165,9 @@ __device__ __forceinline__ void sum_tiles(const AttnArgs& a, int per, int64_t& b
 
 template <int KEYS, int HEADS>
 __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
-    kv8_decode_kernel(const DecodeArgs g, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+    kv8_decode_kernel(const DecodeArgs g, const __grid_constant__ CUtensorMap map_k,
+                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap row_k,
+                      const __grid_constant__ CUtensorMap row_v) {
   constexpr int NC = 2 * HEADS;               // columns: hi, lo
   constexpr int kColBytes = NC * 128;         // Q or P in shared memory
   constexpr uint32_t kTmemCols = 4 * NC;      // S[2], O[2]
@@ -142,10 +180,12 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
   __shared__ int s_start[3];
   __shared__ float s_ks[kMeta][kMetaN], s_vs[kMeta][kMetaN];
   __shared__ float s_qinv[4][HEADS];  // a pair's stay until the softmax has passed it: two more pairs on
-  __shared__ __align__(16) float s_max[2][4][HEADS];
-  __shared__ float s_sum[4][HEADS];
+  __shared__ __align__(16) float s_max[2][HEADS][4];
+  __shared__ __align__(16) float s_sum[HEADS][4];
   const AttnArgs& a = g.a;
   const Cache& c = a.c;
+  if (threadIdx.x < (KEYS == kRows ? 4 : 2))
+    prefetch_map(threadIdx.x == 0 ? &map_k : threadIdx.x == 1 ? &map_v : threadIdx.x == 2 ? &row_k : &row_v);
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const smem = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t off_q = g.slots * kSlotBytes, off_p = off_q + 2 * kColBytes;
@@ -154,31 +194,8 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
   volatile int* abort_flag = &s_abort;
   auto wait = [&](int i, uint32_t parity) { return mbar_wait(bar(i), parity, abort_flag, a.err); };
 
-  // ---- this CTA's share and where it begins
-  const int per = (a.bs + kThreads - 1) / kThreads;
-  int64_t before, tiles;
-  sum_tiles<KEYS, kThreads>(a, per, before, tiles, blockIdx.x == 0 ? a.err : nullptr);
-  const int64_t total = tiles * c.kv_heads;
-  const int64_t ctas = min((int64_t)gridDim.x, total);  // no share is empty
-  allow_next_grid();
-  if (blockIdx.x >= ctas) return;  // uniform over the CTA
-  const int64_t lo = share_lo(total, blockIdx.x, ctas), hi = share_lo(total, blockIdx.x + 1, ctas);
-  {
-    int64_t at = before * c.kv_heads;
-    for (int j = 0; j < per; ++j) {
-      const int e = threadIdx.x * per + j;
-      if (e >= a.bs || at > lo) break;
-      const int64_t T = (entry_keys<KEYS>(a, e, nullptr) + kTile - 1) / kTile;
-      if (lo < at + T * c.kv_heads) {
-        const int64_t r = lo - at;
-        s_start[0] = e;
-        s_start[1] = (int)(r / T);
-        s_start[2] = (int)(r % T);
-      }
-      at += T * c.kv_heads;
-    }
-  }
-  if (threadIdx.x == 0) {
+  // ---- barriers and tensor memory, then this CTA's share and where it begins
+  if (threadIdx.x == kThreads - 1) {
     s_abort = 0;
     for (int i = 0; i < g.slots; ++i) {
       mbar_init(bar(kBarFull + i), 1);
@@ -199,39 +216,104 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
     mbar_init_fence();
   }
   if (warp == 5) tmem_alloc(smem_u32(&s_tmem), kTmemCols);
+  const int per = (a.bs + kThreads - 1) / kThreads;
+  int64_t before, tiles;
+  sum_tiles<KEYS, kThreads>(a, per, before, tiles, blockIdx.x == 0 ? a.err : nullptr);
+  const Shares shares(tiles * c.kv_heads, gridDim.x);
+  allow_next_grid();
+  if (blockIdx.x == 0) {
+    int64_t at = before;
+    for (int j = 0; j < per; ++j) {
+      const int e = threadIdx.x * per + j;
+      if (e >= a.bs) break;
+      g.before[e] = at;
+      at += (entry_keys<KEYS>(a, e, nullptr) + kTile - 1) / kTile;
+    }
+    if (threadIdx.x == 0) g.before[a.bs] = tiles;
+  }
+  const bool any = blockIdx.x < shares.ctas;
+  const int64_t lo = shares.lo(blockIdx.x);
+  {
+    int64_t at = before * c.kv_heads;
+    for (int j = 0; any && j < per; ++j) {
+      const int e = threadIdx.x * per + j;
+      if (e >= a.bs || at > lo) break;
+      const int T = (int)((entry_keys<KEYS>(a, e, nullptr) + kTile - 1) / kTile);
+      if (lo < at + (int64_t)T * c.kv_heads) {
+        int r = (int)(lo - at), h = 0;
+        if (r >= T) h = r / T, r -= h * T;
+        s_start[0] = e;
+        s_start[1] = h;
+        s_start[2] = r;
+      }
+      at += (int64_t)T * c.kv_heads;
+    }
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (!any) {  // uniform over the CTA
+    if (warp == 5) tmem_dealloc(s_tmem, kTmemCols);
+    return;
+  }
   const uint32_t tmem = s_tmem;
-  const int count = (int)(hi - lo);
+  const int count = (int)(shares.lo(blockIdx.x + 1) - lo);
   Walk<KEYS> w(a, s_start[0], s_start[1], s_start[2]);
   const int64_t pool_rows = (int64_t)c.num_blocks * c.kv_heads * c.block;
 
   if (warp == 4) {
     // ================================================================ codes
+    // the table entries or rows of a tile are loaded one tile ahead
     const int pages = kTile >> c.shift;
     int issued = 0;
-    for (int i = 0; i < count; ++i, w.next()) {
-      int4 row;
-      uint32_t mask = 0xffffffffu;
+    auto fetch = [&](const Walk<KEYS>& x, int32_t (&r)[4]) {
+      r[0] = r[1] = r[2] = r[3] = -1;
       if (KEYS == kTable) {
-        const int64_t j = (int64_t)w.t * kTile + ((int64_t)lane << c.shift);
-        int32_t b = -1;
-        if (lane < pages && j < w.n) b = a.table[a.reqs[w.e] * a.table_stride + (j >> c.shift)];
+        const int64_t j = (int64_t)x.t * kTile + ((int64_t)lane << c.shift);
+        if (lane < pages && j < x.n) r[0] = a.table[a.reqs[x.e] * a.table_stride + (j >> c.shift)];
+      } else {
+        const int64_t j = (int64_t)x.t * kTile + lane * 4;
+        const int32_t* p = a.rows + (int64_t)x.e * a.rows_stride + j;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (j + u < x.n) r[u] = p[u];
+      }
+    };
+    Walk<KEYS> ahead = w;
+    int32_t next[4];
+    fetch(ahead, next);
+    for (int i = 0; i < count; ++i, w.next()) {
+      int32_t r[4] = {next[0], next[1], next[2], next[3]};
+      if (i + 1 < count) {
+        ahead.next();
+        fetch(ahead, next);
+      }
+      int4 row;
+      uint32_t mask, bytes;  // the lanes that copy a box; all bytes of the copies
+      bool single = false;   // this lane copies single rows
+      if (KEYS == kTable) {
+        const int32_t b = r[0];
         const bool in = b >= 0 && b < c.num_blocks;
         mask = __ballot_sync(0xffffffffu, in);
+        bytes = (uint32_t)__popc(mask) << (c.shift + 7);
         row.x = in ? (b * c.kv_heads + w.h) * c.block : 0;
       } else {
-        const int64_t j = (int64_t)w.t * kTile + lane * 4;
-        const int32_t* p = a.rows + (int64_t)w.e * a.rows_stride + j;
-        int32_t r[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          r[u] = j + u < w.n ? p[u] : -1;
           const bool in = r[u] >= 0 && (r[u] >> c.shift) < c.num_blocks;
           r[u] = in ? ((r[u] >> c.shift) * c.kv_heads + w.h) * c.block + (r[u] & (c.block - 1)) : (int32_t)pool_rows;
         }
         row = make_int4(r[0], r[1], r[2], r[3]);
+        // 16 listed rows that follow one another (a page selection's do) are one box of the pool, the others
+        // go four at a time: the copy engine takes a row of a gather as long as several rows of a box
+        const int32_t lead = __shfl_sync(0xffffffffu, r[0], lane & ~3);
+        const bool follow = r[3] < pool_rows && r[0] == lead + 4 * (lane & 3) && r[1] == r[0] + 1 && r[2] == r[0] + 2 &&
+                            r[3] == r[0] + 3;
+        const uint32_t f = __ballot_sync(0xffffffffu, follow);
+        const bool box = (f >> (lane & ~3) & 15u) == 15u;
+        mask = __ballot_sync(0xffffffffu, box && (lane & 3) == 0);
+        single = !box && (r[0] < pool_rows || r[1] < pool_rows || r[2] < pool_rows || r[3] < pool_rows);
+        bytes = (uint32_t)__popc(mask) * 2048u + (uint32_t)__popc(__ballot_sync(0xffffffffu, single)) * 512u;
       }
       bool ok = true;
 #pragma unroll
@@ -241,14 +323,11 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const uint32_t full = bar(kBarFull + s), dst = base + s * kSlotBytes;
-        if (lane == 0)
-          mbar_arrive_expect(full, KEYS == kTable ? (uint32_t)__popc(mask) << (c.shift + 7) : (uint32_t)kSlotBytes);
+        if (lane == 0) mbar_arrive_expect(full, bytes);
         __syncwarp();
-        if (KEYS == kTable) {
-          if (mask >> lane & 1) tma_load_rows(dst + (lane << (c.shift + 7)), v ? &map_v : &map_k, row.x, full);
-        } else {
-          tma_gather_rows(dst + lane * 512, v ? &map_v : &map_k, row, full);
-        }
+        if (mask >> lane & 1)
+          tma_load_rows(dst + (KEYS == kTable ? lane << (c.shift + 7) : lane * 512), v ? &map_v : &map_k, row.x, full);
+        if (KEYS == kRows && single) tma_gather_rows(dst + lane * 512, v ? &row_v : &row_k, row, full);
         ++issued;
       }
       if (!ok) break;
@@ -309,30 +388,43 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
       const int qb = pair & 1;
       if (pair >= 2 && !__all_sync(0xffffffffu, wait(kBarQFree + qb, ((pair >> 1) - 1) & 1))) break;
       uint8_t* dst = smem + off_q + qb * kColBytes;
+      // four lanes per head, 32 channels each
 #pragma unroll
-      for (int r = 0; r < HEADS; ++r) {
-        float x[4] = {};
+      for (int r0 = 0; r0 < HEADS; r0 += 8) {
+        const int r = r0 + (lane >> 2), col = (lane & 3) * 32;
+        float x[32] = {};
         if (r < a.group) {
-          const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(a.q) + w.e * a.q_stride +
-                                                          (int64_t)(w.h * a.group + r) * kTcDim + lane * 4);
-          x[0] = __uint_as_float(u.x << 16), x[1] = __uint_as_float(u.x & 0xFFFF0000u);
-          x[2] = __uint_as_float(u.y << 16), x[3] = __uint_as_float(u.y & 0xFFFF0000u);
+          const uint2* q = reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(a.q) + w.e * a.q_stride +
+                                                          (int64_t)(w.h * a.group + r) * kTcDim + col);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint2 u = q[k];
+            x[4 * k] = __uint_as_float(u.x << 16), x[4 * k + 1] = __uint_as_float(u.x & 0xFFFF0000u);
+            x[4 * k + 2] = __uint_as_float(u.y << 16), x[4 * k + 3] = __uint_as_float(u.y & 0xFFFF0000u);
+          }
         }
         float most = 0.f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < 32; ++k) {
           const bool finite = fabsf(x[k]) <= 3.402823466e38f;
           if (finite) most = fmaxf(most, fabsf(x[k]));
           else x[k] = __uint_as_float(0x7FFFFFFFu);  // an infinite query has no scores either
         }
-        const int k2 = fit_exponent(warp_max(most));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        const int k2 = fit_exponent(most);
         const float up = exp2_int(k2);
-        uint32_t h0, l0, h1, l1;
-        split_e4m3x2(x[0] * up, x[1] * up, kLo, h0, l0);
-        split_e4m3x2(x[2] * up, x[3] * up, kLo, h1, l1);
-        *reinterpret_cast<uint32_t*>(dst + swz(r, lane * 4)) = h0 | (h1 << 16);
-        *reinterpret_cast<uint32_t*>(dst + swz(HEADS + r, lane * 4)) = l0 | (l1 << 16);
-        if (lane == 0) s_qinv[pair & 3][r] = a.scale_log2 * exp2_int(-k2);
+#pragma unroll
+        for (int k = 0; k < 32; k += 16) {
+          uint32_t h[8], l[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) split_e4m3x2(x[k + 2 * u] * up, x[k + 2 * u + 1] * up, kLo, h[u], l[u]);
+          *reinterpret_cast<uint4*>(dst + swz(r, col + k)) =
+              make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+          *reinterpret_cast<uint4*>(dst + swz(HEADS + r, col + k)) =
+              make_uint4(l[0] | l[1] << 16, l[2] | l[3] << 16, l[4] | l[5] << 16, l[6] | l[7] << 16);
+        }
+        if ((lane & 3) == 0) s_qinv[pair & 3][r] = a.scale_log2 * exp2_int(-k2);
       }
       fence_async_shared();
       mbar_arrive(bar(kBarQ + qb));
@@ -341,20 +433,35 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
     }
   } else if (warp == 7) {
     // ================================================================ scales
-    for (int i = 0; i < count; ++i, w.next()) {
-      const int m = i % kMeta;
-      constexpr int N = (kMetaN + 31) / 32;
-      float ks[N], vs[N];
+    // the slots of a tile's tokens are found one tile ahead
+    constexpr int N = (kMetaN + 31) / 32;
+    auto find = [&](const Walk<KEYS>& x, int32_t (&slot)[N]) {
+      const int64_t req = KEYS == kRows ? 0 : a.reqs[x.e];
 #pragma unroll
       for (int u = 0; u < N; ++u) {
         const int k = u * 32 + lane;
-        const int64_t j = KEYS == kRows ? (int64_t)w.t * kTile + k : (int64_t)w.t * kTile + ((int64_t)k << c.shift);
-        int64_t slot = -1;
-        if (k < (KEYS == kRows ? kTile : kTile >> c.shift) && j < w.n)
-          slot = key_slot<KEYS>(a, w.e, KEYS == kRows ? 0 : a.reqs[w.e], j, w.h == 0 ? a.err : nullptr);
-        const int64_t bh = slot < 0 ? 0 : (slot >> c.shift) * c.kv_heads + w.h;
-        ks[u] = slot < 0 ? 0.f : c.k_scale[bh];
-        vs[u] = slot < 0 ? __uint_as_float(kMasked) : c.v_scale[bh];
+        const int64_t j = (int64_t)x.t * kTile + (KEYS == kRows ? k : (int64_t)k << c.shift);
+        slot[u] = -1;
+        if (k < (KEYS == kRows ? kTile : kTile >> c.shift) && j < x.n)
+          slot[u] = (int32_t)key_slot<KEYS>(a, x.e, req, j, x.h == 0 ? a.err : nullptr);
+      }
+    };
+    Walk<KEYS> ahead = w;
+    int32_t next[N];
+    find(ahead, next);
+    for (int i = 0; i < count; ++i, w.next()) {
+      const int m = i % kMeta;
+      float ks[N], vs[N];
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        const bool in = next[u] >= 0;
+        const int64_t bh = in ? (int64_t)(next[u] >> c.shift) * c.kv_heads + w.h : 0;
+        ks[u] = in ? c.k_scale[bh] : 0.f;
+        vs[u] = in ? c.v_scale[bh] : __uint_as_float(kMasked);
+      }
+      if (i + 1 < count) {
+        ahead.next();
+        find(ahead, next);
       }
       if (i >= kMeta && !__all_sync(0xffffffffu, wait(kBarMetaFree + m, ((i / kMeta) - 1) & 1))) break;
 #pragma unroll
@@ -410,14 +517,15 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
       const int ev = seen ? min(126, max(-100, (int)((__float_as_uint(vs) >> 23) & 255) - 127)) : 0;
       const float back = seen ? exp2_int(-ev) : 0.f;
       const float vm = seen ? vs * back * kPScale : 0.f;
-      float u[HEADS];
+      float u[HEADS], most[HEADS];
 #pragma unroll
       for (int r = 0; r < HEADS; ++r) {
         const float s = fmaf(__uint_as_float(v[HEADS + r]), 1.f / kLo, __uint_as_float(v[r])) * (s_qinv[pair & 3][r] * ks);
         u[r] = seen ? s + (float)ev : -INFINITY;
-        const float most = warp_max(u[r]);
-        if (lane == r) s_max[b][warp][r] = most;
+        most[r] = u[r];
       }
+      const float top = reduce_lanes(most, lane, [](float x, float y) { return fmaxf(x, y); });
+      if (lane % (32 / HEADS) == 0) s_max[b][lane / (32 / HEADS)][warp] = top;
       asm volatile("bar.sync 1, 128;" ::: "memory");
       float before_corr[HEADS];
       uint32_t hi8[HEADS / 2], lo8[HEADS / 2];
@@ -427,8 +535,8 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int q = r + k;
-          const float mn =
-              fmaxf(fmaxf(fmaxf(s_max[b][0][q], s_max[b][1][q]), fmaxf(s_max[b][2][q], s_max[b][3][q])), M[q]);
+          const float4 m4 = *reinterpret_cast<const float4*>(s_max[b][q]);
+          const float mn = fmaxf(fmaxf(fmaxf(m4.x, m4.y), fmaxf(m4.z, m4.w)), M[q]);
           const float ref = mn == -INFINITY ? 0.f : mn;
           before_corr[q] = corr[q];
           corr[q] = ex2(M[q] - ref);
@@ -464,24 +572,21 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
 
       // ---- the end of the pair, or of the share: the result, or a record of this part
       add_product(i, corr);
-#pragma unroll
-      for (int r = 0; r < HEADS; ++r) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
-        if (lane == 0) s_sum[warp][r] = l[r];
-      }
+      const float part = reduce_lanes(l, lane, [](float x, float y) { return x + y; });
+      if (lane % (32 / HEADS) == 0) s_sum[lane / (32 / HEADS)][warp] = part;
       asm volatile("bar.sync 1, 128;" ::: "memory");
       if (ok) {
         const bool whole = i >= w.t && first;  // all of the pair's tiles are this CTA's
         float* rec = a.part + ((int64_t)blockIdx.x * 2 + (pair > 0)) * record_floats(HEADS);
 #pragma unroll
         for (int r = 0; r < HEADS; ++r) {
-          const float sum = (s_sum[0][r] + s_sum[1][r]) + (s_sum[2][r] + s_sum[3][r]);
+          const float4 l4 = *reinterpret_cast<const float4*>(s_sum[r]);
+          const float sum = (l4.x + l4.y) + (l4.z + l4.w);
           const float o = O[r] * (1.f / kPScale);
           if (whole) {
             if (r < a.group)
               static_cast<__nv_bfloat16*>(a.out)[w.e * a.out_stride + (int64_t)(w.h * a.group + r) * kTcDim + tok] =
-                  __float2bfloat16_rn(sum == 0.f ? 0.f : o / sum);
+                  __float2bfloat16_rn(sum == 0.f ? 0.f : o * __frcp_rn(sum));
           } else {
             if (tok == 0) rec[r] = M[r], rec[HEADS + r] = sum;
             rec[2 * HEADS + r * kTcDim + tok] = o;
@@ -499,73 +604,92 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
   }
 }
 
-// Joins the records of entry blockIdx.x, KV head blockIdx.y where its tiles
-// lay in several shares; an entry without keys gets zeros.  A warp per query
-// head, four channels per lane; the records' weights first, a lane each.
-constexpr int kJoinThreads = 256;
-template <int KEYS, int HEADS>
+// Joins the records of a pair whose tiles lay in several shares; an entry
+// without keys gets zeros.  Lanes hold four channels.  SPLIT: a CTA per query
+// head, its warps take the records in turn (few pairs, many records each);
+// else a CTA per pair and a warp per query head (a pair has two or three
+// records: 2048 CTAs of the other kind took 15 us where 256 of this take 7).
+// A record's outputs are asked for together with the maxima, so the chain is
+// one load long.
+constexpr int kJoinWarps = 8, kJoinThreads = 32 * kJoinWarps;
+constexpr int kJoinAhead = 4;  // records in flight per warp
+template <int HEADS, bool SPLIT>
 __global__ void __launch_bounds__(kJoinThreads) kv8_decode_join_kernel(const DecodeArgs g, int64_t ctas) {
-  __shared__ int64_t s_before;
+  __shared__ float s_m[kJoinWarps], s_l[kJoinWarps];
+  __shared__ __align__(16) float s_o[kJoinWarps][kTcDim];
   const AttnArgs& a = g.a;
-  const int e = blockIdx.x, h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int per = (a.bs + kJoinThreads - 1) / kJoinThreads;
-  int64_t before, tiles;
-  sum_tiles<KEYS, kJoinThreads>(a, per, before, tiles, nullptr);
-  if (threadIdx.x == e / per) {
-    for (int i = e / per * per; i < e; ++i) before += (entry_keys<KEYS>(a, i, nullptr) + kTile - 1) / kTile;
-    s_before = before;
-  }
-  __syncthreads();
-  const int64_t total = tiles * a.c.kv_heads;
-  const int64_t T = (entry_keys<KEYS>(a, e, nullptr) + kTile - 1) / kTile;
-  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + e * a.out_stride + (int64_t)h * a.group * kTcDim;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int e = blockIdx.x, h = SPLIT ? blockIdx.y / a.group : blockIdx.y;
   wait_prior_grid();
+  const int64_t total = g.before[a.bs] * a.c.kv_heads, T = g.before[e + 1] - g.before[e];
+  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + e * a.out_stride;
   if (T == 0) {
-    for (int i = threadIdx.x; i < a.group * kTcDim; i += kJoinThreads) out[i] = __float2bfloat16_rn(0.f);
+    out += (int64_t)(SPLIT ? blockIdx.y : h * a.group) * kTcDim;
+    for (int i = threadIdx.x; i < (SPLIT ? 1 : a.group) * kTcDim; i += kJoinThreads) out[i] = __float2bfloat16_rn(0.f);
     return;
   }
-  ctas = min(ctas, total);
-  const int64_t first = s_before * a.c.kv_heads + h * T, last = first + T - 1;
-  auto owner = [&](int64_t x) {
-    int64_t c = x * ctas / total;
-    while (share_lo(total, c + 1, ctas) <= x) ++c;
-    while (share_lo(total, c, ctas) > x) --c;
-    return c;
-  };
-  const int64_t c0 = owner(first), c1 = owner(last);
+  const Shares shares(total, ctas);
+  const int64_t first = g.before[e] * a.c.kv_heads + h * T, last = first + T - 1;
+  const int64_t c0 = shares.owner(first), c1 = shares.owner(last);
   if (c0 == c1) return;  // written by its CTA
   const int parts = (int)(c1 - c0 + 1);
-  const int skip = first > share_lo(total, c0, ctas) ? 1 : 0;  // the first CTA's record lies behind another pair's
+  const int skip = first > shares.lo(c0) ? 1 : 0;  // the first CTA's record lies behind another pair's
   auto record = [&](int k) { return a.part + ((c0 + k) * 2 + (k == 0 ? skip : 0)) * record_floats(HEADS); };
-  for (int r = warp; r < a.group; r += kJoinThreads / 32) {
-    float M = -INFINITY;
-    for (int k = lane; k < parts; k += 32) M = fmaxf(M, record(k)[r]);
-    M = warp_max(M);
-    const float ref = M == -INFINITY ? 0.f : M;
-    float sum = 0.f, o[4] = {};
-    for (int k0 = 0; k0 < parts; k0 += 32) {
-      float wgt = 0.f;
-      if (k0 + lane < parts) {
-        const float* p = record(k0 + lane);
-        wgt = ex2(p[r] - ref);
-        sum = fmaf(wgt, p[HEADS + r], sum);
-      }
-      const int n = min(32, parts - k0);
-#pragma unroll 8
-      for (int k = 0; k < n; ++k) {
-        const float f = __shfl_sync(0xffffffffu, wgt, k);
-        const float4 v = *reinterpret_cast<const float4*>(record(k0 + k) + 2 * HEADS + r * kTcDim + lane * 4);
-        o[0] = fmaf(f, v.x, o[0]), o[1] = fmaf(f, v.y, o[1]), o[2] = fmaf(f, v.z, o[2]), o[3] = fmaf(f, v.w, o[3]);
-      }
-    }
+  for (int r = SPLIT ? blockIdx.y - h * a.group : warp; r < a.group; r += kJoinWarps) {
+    const int step = SPLIT ? kJoinWarps : 1;
+    float M = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = SPLIT ? warp : 0; k0 < parts; k0 += step * kJoinAhead) {
+      float m[kJoinAhead], s[kJoinAhead];
+      float4 v[kJoinAhead];
 #pragma unroll
-    for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    *reinterpret_cast<uint2*>(out + r * kTcDim + lane * 4) =
-        make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
+      for (int k = 0; k < kJoinAhead; ++k) {
+        const float* p = record(min(k0 + k * step, parts - 1));
+        m[k] = k0 + k * step < parts ? p[r] : -INFINITY;
+        s[k] = p[HEADS + r];
+        v[k] = *reinterpret_cast<const float4*>(p + 2 * HEADS + r * kTcDim + lane * 4);
+      }
+      float mn = M;
+#pragma unroll
+      for (int k = 0; k < kJoinAhead; ++k) mn = fmaxf(mn, m[k]);
+      const float ref = mn == -INFINITY ? 0.f : mn;
+      const float f0 = ex2(M - ref);
+      l *= f0, o.x *= f0, o.y *= f0, o.z *= f0, o.w *= f0;
+#pragma unroll
+      for (int k = 0; k < kJoinAhead; ++k) {
+        if (k0 + k * step >= parts) break;
+        const float f = ex2(m[k] - ref);
+        l = fmaf(f, s[k], l);
+        o.x = fmaf(f, v[k].x, o.x), o.y = fmaf(f, v[k].y, o.y), o.z = fmaf(f, v[k].z, o.z), o.w = fmaf(f, v[k].w, o.w);
+      }
+      M = mn;
+    }
+    if (!SPLIT) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      *reinterpret_cast<uint2*>(out + (int64_t)(h * a.group + r) * kTcDim + lane * 4) =
+          make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+      continue;
+    }
+    if (lane == 0) s_m[warp] = M, s_l[warp] = l;
+    *reinterpret_cast<float4*>(&s_o[warp][lane * 4]) = o;
+    __syncthreads();
+    if (threadIdx.x < kTcDim) {
+      float mn = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) mn = fmaxf(mn, s_m[w]);
+      const float ref = mn == -INFINITY ? 0.f : mn;
+      float sum = 0.f, x = 0.f;
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) {
+        const float f = ex2(s_m[w] - ref);
+        sum = fmaf(f, s_l[w], sum);
+        x = fmaf(f, s_o[w][threadIdx.x], x);
+      }
+      out[(int64_t)blockIdx.y * kTcDim + threadIdx.x] = __float2bfloat16_rn(sum == 0.f ? 0.f : x / sum);
+    }
+    break;
   }
 }
-
 
 template <int KEYS, int HEADS>
 int launch(DecodeArgs g, int64_t ctas, cudaStream_t s) {
@@ -577,14 +701,23 @@ int launch(DecodeArgs g, int64_t ctas, cudaStream_t s) {
   static SmemLimit limit;
   int rc = limit.ensure((const void*)kv8_decode_kernel<KEYS, HEADS>, smem);
   if (rc != QQ_OK) return rc;
-  CUtensorMap mk, mv;
+  CUtensorMap mk, mv, rk, rv;
   const int64_t rows = (int64_t)g.a.c.num_blocks * g.a.c.kv_heads * g.a.c.block;
-  const int box = KEYS == kTable ? g.a.c.block : 1;
+  const int box = KEYS == kTable ? g.a.c.block : 16;
   if ((rc = encode_rows(&mk, g.a.c.k, rows, box)) != QQ_OK) return rc;
   if ((rc = encode_rows(&mv, g.a.c.v, rows, box)) != QQ_OK) return rc;
-  kv8_decode_kernel<KEYS, HEADS><<<(unsigned)ctas, kThreads, smem, s>>>(g, mk, mv);
+  if (KEYS == kRows) {
+    if ((rc = encode_rows(&rk, g.a.c.k, rows, 1)) != QQ_OK) return rc;
+    if ((rc = encode_rows(&rv, g.a.c.v, rows, 1)) != QQ_OK) return rc;
+  } else {
+    rk = mk, rv = mv;  // not read
+  }
+  kv8_decode_kernel<KEYS, HEADS><<<(unsigned)ctas, kThreads, smem, s>>>(g, mk, mv, rk, rv);
   if ((rc = launch_status()) != QQ_OK) return rc;
-  return launch_pdl(kv8_decode_join_kernel<KEYS, HEADS>, dim3(g.a.bs, g.a.c.kv_heads), dim3(kJoinThreads), 0, s, g, ctas);
+  const int pairs = g.a.bs * g.a.c.kv_heads;
+  if (ctas >= 4 * (int64_t)pairs)
+    return launch_pdl(kv8_decode_join_kernel<HEADS, true>, dim3(g.a.bs, g.a.heads), dim3(kJoinThreads), 0, s, g, ctas);
+  return launch_pdl(kv8_decode_join_kernel<HEADS, false>, dim3(g.a.bs, g.a.c.kv_heads), dim3(kJoinThreads), 0, s, g, ctas);
 }
 
 int64_t decode_ctas(int bs, int kv_heads, int group, int64_t max_keys) {
@@ -602,7 +735,8 @@ bool decode_tc_fits(const AttnArgs& a, int dtype) {
 }
 
 size_t decode_tc_workspace(int bs, int kv_heads, int group, int64_t max_keys) {
-  return sizeof(float) * (size_t)(decode_ctas(bs, kv_heads, group, max_keys) * 2 * record_floats(group <= 8 ? 8 : 16));
+  return sizeof(float) * (size_t)(decode_ctas(bs, kv_heads, group, max_keys) * 2 * record_floats(group <= 8 ? 8 : 16)) +
+         sizeof(int64_t) * (size_t)(bs + 1);
 }
 
 int run_decode_tc(const AttnArgs& a, int keys, int64_t max_keys, size_t ws_bytes, cudaStream_t s) {
@@ -610,6 +744,7 @@ int run_decode_tc(const AttnArgs& a, int keys, int64_t max_keys, size_t ws_bytes
   DecodeArgs g{};
   g.a = a;
   const int64_t ctas = decode_ctas(a.bs, a.c.kv_heads, a.group, max_keys);
+  g.before = reinterpret_cast<int64_t*>(a.part + ctas * 2 * record_floats(a.group <= 8 ? 8 : 16));
   if (a.group <= 8) return keys == kTable ? launch<kTable, 8>(g, ctas, s) : launch<kRows, 8>(g, ctas, s);
   return keys == kTable ? launch<kTable, 16>(g, ctas, s) : launch<kRows, 16>(g, ctas, s);
 }

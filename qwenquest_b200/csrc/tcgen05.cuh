@@ -171,6 +171,9 @@ __device__ __forceinline__ void mbar_arrive_expect(uint32_t bar, uint32_t bytes)
                "r"(bytes)
                : "memory");
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
 // A box of the tensor map from row `row` on; the bytes count on the mbarrier.
 __device__ __forceinline__ void tma_load_rows(uint32_t dst, const CUtensorMap* map, int32_t row, uint32_t bar) {
   asm volatile(

@@ -53,6 +53,7 @@ class _OnDevice:
 
     def __init__(self, device: torch.device, what: str):
         self.device = device
+        self._index = device.index
         self.lib = _lib.load()
         self._what = what
         self._err = DeviceError(torch.zeros(1, dtype=torch.int32).pin_memory())
@@ -71,7 +72,7 @@ class _OnDevice:
 
     def _call(self, fn, *args) -> None:
         """One entry point, launched on the current stream of the object's device (also when another is current)."""
-        index = self.device.index
+        index = self._index
         if torch.cuda.current_device() == index:
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
         else:
@@ -84,7 +85,7 @@ class _OnDevice:
         """A contiguous device vector of `dtype`; lists and tensors elsewhere are copied over."""
         if not isinstance(t, torch.Tensor):
             t = torch.as_tensor(t)
-        if t.dtype != dtype or t.device != self.device:
+        if t.dtype != dtype or t.get_device() != self._index:
             if t.numel() and (t.dtype.is_floating_point or t.dtype == torch.bool):
                 raise ValueError(f"{name}: integers are wanted, got {t.dtype}")
             t = t.to(device=self.device, dtype=dtype)
@@ -159,7 +160,8 @@ class BlockTables(_OnDevice):
         the slots by request and position.  A batch that runs out of blocks raises ``RuntimeError`` at the next
         check; the entries that no longer fit are left as they were.
         """
-        self.check_errors()
+        if self._err_word.value:
+            self.check_errors()
         reqs = self._ints(req_pool_indices, torch.int64, "req_pool_indices")
         bs = reqs.shape[0]
         seq = self._ints(seq_lens, torch.int64, "seq_lens", bs)
@@ -167,8 +169,8 @@ class BlockTables(_OnDevice):
         num_tokens = int(num_tokens)
         if num_tokens < 0:
             raise ValueError("num_tokens must be >= 0")
-        made = torch.empty(num_tokens + bs + 1, dtype=torch.int64, device=self.device)
-        slots, offsets = made[:num_tokens], made[num_tokens:]
+        made = reqs.new_empty(num_tokens + bs + 1)
+        slots, offsets = made.split((num_tokens, bs + 1))
         mapped = (None, 0, 0)
         if req_to_token is not None:
             if (req_to_token.dim() != 2 or req_to_token.dtype != torch.int32 or req_to_token.stride(1) != 1
@@ -176,13 +178,14 @@ class BlockTables(_OnDevice):
                 raise ValueError("req_to_token must be int32 [rows, max_context] with contiguous rows on the device")
             mapped = (req_to_token.data_ptr(), req_to_token.stride(0), req_to_token.shape[0])
         self._call(self.lib.qq_block_plan, self._tables, reqs.data_ptr(), seq.data_ptr(), prefix.data_ptr(), bs,
-                   made.data_ptr(), num_tokens, offsets.data_ptr(), *mapped, self._err_ptr)
+                   made.data_ptr(), num_tokens, made.data_ptr() + 8 * num_tokens, *mapped, self._err_ptr)
         return slots, offsets
 
     def trim(self, req_pool_indices, keep_lens=None) -> None:
         """Requests keep the blocks of their first ``keep_lens[i]`` tokens (``None``: of none, they are finished);
         the others are free again.  A request of -1 is padding."""
-        self.check_errors()
+        if self._err_word.value:
+            self.check_errors()
         reqs = self._ints(req_pool_indices, torch.int64, "req_pool_indices")
         keep = None if keep_lens is None else self._ints(keep_lens, torch.int64, "keep_lens", reqs.shape[0])
         self._call(self.lib.qq_block_trim, self._tables, reqs.data_ptr(), None if keep is None else keep.data_ptr(),
@@ -256,16 +259,18 @@ class KV8Cache(_OnDevice):
 
     # ------------------------------------------------------------------ write and read
 
-    def _tokens(self, t: torch.Tensor, name: str) -> torch.Tensor:
-        """``[n, kv_heads, head_dim]`` with dense 16-byte aligned rows (any distance between tokens)."""
-        if t.dim() != 3 or t.shape[1] != self.kv_heads or t.shape[2] != self.head_dim or t.device != self.device:
+    def _tokens(self, t: torch.Tensor, name: str) -> tuple[torch.Tensor, int, int]:
+        """``[n, kv_heads, head_dim]`` with dense 16-byte aligned rows, its address and the distance between tokens."""
+        if t.dim() != 3 or t.shape[1] != self.kv_heads or t.shape[2] != self.head_dim or t.get_device() != self._index:
             raise ValueError(f"{name} must be [tokens, {self.kv_heads}, {self.head_dim}] on {self.device}, "
                              f"got {tuple(t.shape)} on {t.device}")
-        size = t.element_size()
-        if (t.stride(2) != 1 or t.stride(1) != self.head_dim or t.stride(0) < t.shape[1] * t.shape[2]
-                or t.stride(0) * size % 16 or t.data_ptr() % 16):
-            t = t.contiguous()
-        return t
+        token, head, one = t.stride()
+        row = self.kv_heads * self.head_dim
+        ptr = t.data_ptr()
+        if one != 1 or head != self.head_dim or token < row or (token * t.element_size() | ptr) & 15:
+            t = t.clone(memory_format=torch.contiguous_format)
+            ptr, token = t.data_ptr(), row
+        return t, ptr, token
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """Quantise new tokens (``k``, ``v``: ``[tokens, kv_heads, head_dim]`` bf16 or fp32) into their slots.
@@ -274,22 +279,26 @@ class KV8Cache(_OnDevice):
         :meth:`BlockTables.plan` gives them; a block met twice in one call is an error, raised at the next
         check.  A block's scale is a power of two that only grows until a token is written at its offset 0.
         """
-        self.check_errors()
-        k, v = self._tokens(k, "k"), self._tokens(v, "v")
-        if k.shape[0] != v.shape[0] or k.dtype != v.dtype:
+        if self._err_word.value:
+            self.check_errors()
+        k, k_ptr, k_stride = self._tokens(k, "k")
+        v, v_ptr, v_stride = self._tokens(v, "v")
+        n = k.shape[0]
+        if n != v.shape[0] or k.dtype != v.dtype:
             raise ValueError("k and v must have the same tokens and dtype")
-        slots = self._ints(slots, torch.int64, "slots", k.shape[0])
-        self._call(self.lib.qq_kv8_append, self._layers[layer], k.data_ptr(), v.data_ptr(), dtype_code(k.dtype),
-                   k.stride(0), v.stride(0), slots.data_ptr(), k.shape[0], self._err_ptr)
+        slots = self._ints(slots, torch.int64, "slots", n)
+        self._call(self.lib.qq_kv8_append, self._layers[layer], k_ptr, v_ptr, dtype_code(k.dtype), k_stride, v_stride,
+                   slots.data_ptr(), n, self._err_ptr)
 
     def gather(self, layer: int, slots: torch.Tensor, *, dtype: torch.dtype = torch.bfloat16
                ) -> tuple[torch.Tensor, torch.Tensor]:
         """The keys and values of the slots, ``[n, kv_heads, head_dim]`` each; -1 gives zeros."""
-        self.check_errors()
+        if self._err_word.value:
+            self.check_errors()
         slots = self._ints(slots, torch.int64, "slots")
         n = slots.shape[0]
         code = dtype_code(dtype)
-        k = torch.empty((n, self.kv_heads, self.head_dim), dtype=dtype, device=self.device)
+        k = slots.new_empty((n, self.kv_heads, self.head_dim), dtype=dtype)
         v = torch.empty_like(k)
         self._call(self.lib.qq_kv8_gather, self._layers[layer], slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), code,
                    self._err_ptr)
@@ -297,26 +306,29 @@ class KV8Cache(_OnDevice):
 
     # ------------------------------------------------------------------ attention
 
-    def _query(self, q: torch.Tensor, out: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor, int]:
-        if q.dim() != 3 or q.shape[2] != self.head_dim or q.device != self.device:
+    def _query(self, q: torch.Tensor, out: torch.Tensor | None) -> tuple[torch.Tensor, int, int, torch.Tensor, int]:
+        """The queries with dense 16-byte aligned rows, their address and row distance; the result and its row distance."""
+        if q.dim() != 3 or q.shape[2] != self.head_dim or q.get_device() != self._index:
             raise ValueError(f"q must be [tokens, heads, {self.head_dim}] on {self.device}, got {tuple(q.shape)} "
                              f"on {q.device}")
         n, heads, dim = q.shape
         if heads == 0 or heads % self.kv_heads:
             raise ValueError(f"q_heads {heads} not divisible by kv_heads {self.kv_heads}")
-        code = dtype_code(q.dtype)
-        if (q.stride(2) != 1 or q.stride(1) != dim or q.stride(0) < heads * dim
-                or q.stride(0) * q.element_size() % 16 or q.data_ptr() % 16):
-            q = q.contiguous()
+        token, head, one = q.stride()
+        row = heads * dim
+        ptr = q.data_ptr()
+        if one != 1 or head != dim or token < row or (token * q.element_size() | ptr) & 15:
+            q = q.clone(memory_format=torch.contiguous_format)
+            ptr, token = q.data_ptr(), row
         if out is None:
-            out = torch.empty((n, heads * dim), dtype=q.dtype, device=self.device)
-        elif (tuple(out.shape) != (n, heads * dim) or out.dtype != q.dtype or out.device != self.device
-              or out.stride(1) != 1 or (n > 1 and out.stride(0) < heads * dim)):
-            raise ValueError(f"out must be {q.dtype} [{n}, {heads * dim}] with contiguous rows on {self.device}")
-        return q, out, code
+            return q, ptr, token, q.new_empty((n, row)), row
+        if (tuple(out.shape) != (n, row) or out.dtype != q.dtype or out.device != self.device
+                or out.stride(1) != 1 or (n > 1 and out.stride(0) < row)):
+            raise ValueError(f"out must be {q.dtype} [{n}, {row}] with contiguous rows on {self.device}")
+        return q, ptr, token, out, max(out.stride(0), row)
 
     def _table(self, t: torch.Tensor) -> torch.Tensor:
-        if t.dim() != 2 or t.dtype != torch.int32 or t.device != self.device or t.shape[0] == 0 or t.shape[1] == 0:
+        if t.dim() != 2 or t.dtype != torch.int32 or t.get_device() != self._index or t.shape[0] == 0 or t.shape[1] == 0:
             raise ValueError(f"block_table must be int32 [requests, blocks] on {self.device}")
         # the kernels take the row's stride as its length
         return t if t.stride(1) == 1 and t.stride(0) == t.shape[1] else t.contiguous()
@@ -332,7 +344,7 @@ class KV8Cache(_OnDevice):
         if size == 0:
             return None, 0, None
         # each call has scratch of its own: calls on several streams, or captured graphs, share none
-        ws = torch.empty(size, dtype=torch.uint8, device=self.device)
+        ws = self._state.new_empty(size // 4)
         return ws.data_ptr(), size, ws
 
     def decode_attention(self, layer: int, q: torch.Tensor, block_table: torch.Tensor, req_pool_indices, seq_lens,
@@ -342,9 +354,13 @@ class KV8Cache(_OnDevice):
         ``q``: ``[bs, heads, head_dim]`` bf16 or fp32; ``block_table``: int32 ``[requests, blocks]``.  Returns
         ``[bs, heads * head_dim]`` in ``q``'s dtype; a length of 0 (padding) gives zeros.
         """
-        self.check_errors()
-        q, out, code = self._query(q, out)
-        bs, heads = q.shape[0], q.shape[1]
+        if self._err_word.value:
+            self.check_errors()
+        q, q_ptr, q_stride, out, out_stride = self._query(q, out)
+        bs, heads, _ = q.shape
+        if bs == 0:
+            return out
+        code = dtype_code(q.dtype)
         table = self._table(block_table)
         reqs = self._ints(req_pool_indices, torch.int64, "req_pool_indices", bs)
         seq = self._ints(seq_lens, torch.int64, "seq_lens", bs)
@@ -352,18 +368,21 @@ class KV8Cache(_OnDevice):
         ws, size, keep = self._workspace(heads, code, bs, bs, width * self.block_size, 0)
         self._call(self.lib.qq_kv8_decode_attention, self._layers[layer],
                    _lib.QQBatch(reqs.data_ptr(), seq.data_ptr(), bs), table.data_ptr(), width, table.shape[0],
-                   q.data_ptr(), code, heads, q.stride(0), float(scaling), out.data_ptr(), out.stride(0),
-                   self._err_ptr, ws, size)
+                   q_ptr, code, heads, q_stride, float(scaling), out.data_ptr(), out_stride, self._err_ptr, ws, size)
         return out
 
     def sparse_decode_attention(self, layer: int, q: torch.Tensor, rows: torch.Tensor, lens, scaling: float, *,
                                 out: torch.Tensor | None = None) -> torch.Tensor:
         """The same over the slots ``rows[i, :lens[i]]`` (int32 ``[bs, top_k]``; duplicates counted, a negative row
         takes no part): the rows :meth:`~qwenquest_b200.quest.QuestAlgorithm.select` writes and its ``actual_lens``."""
-        self.check_errors()
-        q, out, code = self._query(q, out)
-        bs, heads = q.shape[0], q.shape[1]
-        if rows.dim() != 2 or rows.shape[0] != bs or rows.shape[1] == 0 or rows.device != self.device:
+        if self._err_word.value:
+            self.check_errors()
+        q, q_ptr, q_stride, out, out_stride = self._query(q, out)
+        bs, heads, _ = q.shape
+        if bs == 0:
+            return out
+        code = dtype_code(q.dtype)
+        if rows.dim() != 2 or rows.shape[0] != bs or rows.shape[1] == 0 or rows.get_device() != self._index:
             raise ValueError(f"rows must be int32 [{bs}, top_k] on {self.device}, got {tuple(rows.shape)}")
         if rows.dtype != torch.int32 or rows.stride(1) != 1 or rows.stride(0) < rows.shape[1]:
             rows = rows.to(torch.int32).contiguous()
@@ -371,8 +390,8 @@ class KV8Cache(_OnDevice):
         top = rows.shape[1]
         ws, size, keep = self._workspace(heads, code, bs, bs, top, 0)
         self._call(self.lib.qq_kv8_sparse_attention, self._layers[layer], bs, rows.data_ptr(), rows.stride(0), top,
-                   lens.data_ptr(), q.data_ptr(), code, heads, q.stride(0), float(scaling), out.data_ptr(),
-                   out.stride(0), self._err_ptr, ws, size)
+                   lens.data_ptr(), q_ptr, code, heads, q_stride, float(scaling), out.data_ptr(), out_stride,
+                   self._err_ptr, ws, size)
         return out
 
     def extend_attention(self, layer: int, q: torch.Tensor, block_table: torch.Tensor, req_pool_indices, seq_lens,
@@ -385,9 +404,11 @@ class KV8Cache(_OnDevice):
         ``token_offsets`` is what :meth:`BlockTables.plan` returns (``[bs + 1]``, or ``[bs]``).  Rows behind the
         last sequence are left as they were: pass ``out`` where they matter.
         """
-        self.check_errors()
-        q, out, code = self._query(q, out)
-        tokens, heads = q.shape[0], q.shape[1]
+        if self._err_word.value:
+            self.check_errors()
+        q, q_ptr, q_stride, out, out_stride = self._query(q, out)
+        tokens, heads, _ = q.shape
+        code = dtype_code(q.dtype)
         table = self._table(block_table)
         reqs = self._ints(req_pool_indices, torch.int64, "req_pool_indices")
         bs = reqs.shape[0]
@@ -401,6 +422,6 @@ class KV8Cache(_OnDevice):
         batch = _lib.QQExtendBatch(reqs.data_ptr(), seq.data_ptr(), prefix.data_ptr(), offsets.data_ptr(), None,
                                    tokens, bs, 0)
         self._call(self.lib.qq_kv8_extend_attention, self._layers[layer], batch, table.data_ptr(), width,
-                   table.shape[0], q.data_ptr(), code, heads, q.stride(0), float(scaling), out.data_ptr(),
-                   out.stride(0), self._err_ptr, ws, size)
+                   table.shape[0], q_ptr, code, heads, q_stride, float(scaling), out.data_ptr(), out_stride,
+                   self._err_ptr, ws, size)
         return out
