@@ -13,6 +13,7 @@
 
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 #include <cuda_fp16.h>
 
@@ -63,7 +64,7 @@ __global__ void __launch_bounds__(kAnyThreads) kv8_attn_any_kernel(AnyArgs g) {
   int e = blockIdx.x;
   int64_t row0 = e, tokens = 1, seen0;  // query rows row0 .., the first sees keys [0, seen0), each next one more
   if (KEYS == kExtend) {
-    const ExtendEntry x = extend_tile(a, blockIdx.x, g.tile_tokens, blockIdx.x == 0 ? err : nullptr);
+    const ExtendEntry x = extend_tile(a, blockIdx.x, g.tile_tokens, 1, blockIdx.x == 0 ? err : nullptr);
     if (x.entry < 0) return;  // past the last tile
     e = x.entry;
     row0 = x.row0 + x.tile * g.tile_tokens;
@@ -90,6 +91,7 @@ __global__ void __launch_bounds__(kAnyThreads) kv8_attn_any_kernel(AnyArgs g) {
 
   auto load_tile = [&](const uint8_t* codes, const float* s_scale) {
     const int per = dim >> 3;
+    int nan = 0;
     for (int i = tid; i < kTileKeys * per; i += kAnyThreads) {
       const int j = i / per, ch = i - j * per;
       const int64_t slot = s_slot[j];
@@ -98,12 +100,16 @@ __global__ void __launch_bounds__(kAnyThreads) kv8_attn_any_kernel(AnyArgs g) {
         const int64_t at = (((slot >> c.shift) * c.kv_heads + kvh) * c.block + (slot & (c.block - 1))) * dim;
         from_e4m3x8(*reinterpret_cast<const uint2*>(codes + at + ch * 8), x);
 #pragma unroll
-        for (int u = 0; u < 8; ++u) x[u] *= s_scale[j];
+        for (int u = 0; u < 8; ++u) {
+          x[u] *= s_scale[j];
+          nan |= isnan(x[u]);
+        }
       }
       float4* d = reinterpret_cast<float4*>(s_kv + j * pitch + ch * 8);
       d[0] = make_float4(x[0], x[1], x[2], x[3]);
       d[1] = make_float4(x[4], x[5], x[6], x[7]);
     }
+    return nan;
   };
 
   for (int64_t j0 = k0; j0 < k1; j0 += kTileKeys) {
@@ -128,7 +134,7 @@ __global__ void __launch_bounds__(kAnyThreads) kv8_attn_any_kernel(AnyArgs g) {
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
           const float4 q4 = *reinterpret_cast<const float4*>(s_q + (r0 + r) * dim + d);
-          s[r] = fmaf(k4.x, q4.x, fmaf(k4.y, q4.y, fmaf(k4.z, q4.z, fmaf(k4.w, q4.w, s[r]))));
+          s[r] += fmaf(k4.x, q4.x, fmaf(k4.y, q4.y, fmaf(k4.z, q4.z, k4.w * q4.w)));
         }
       }
       const bool there = s_slot[j] >= 0;
@@ -139,7 +145,7 @@ __global__ void __launch_bounds__(kAnyThreads) kv8_attn_any_kernel(AnyArgs g) {
       }
     }
     __syncthreads();
-    load_tile(c.v, s_vs);
+    const int nan = load_tile(c.v, s_vs);
     for (int r = warp * 4; r < warp * 4 + 4; ++r) {  // softmax: a warp's four rows
       const float x0 = s_p[r * kTileKeys + lane], x1 = s_p[r * kTileKeys + lane + 32];
       // fmaxf drops NaN: a NaN score must reach the sum through its weight
@@ -160,23 +166,30 @@ __global__ void __launch_bounds__(kAnyThreads) kv8_attn_any_kernel(AnyArgs g) {
         s_l[r] = s_l[r] * corr + l;
       }
     }
-    __syncthreads();
+    const int any_nan = __syncthreads_or(nan);
+    auto product = [&](auto guard) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int d = tid + u * kAnyThreads;
-      if (d >= dim) break;
+      for (int u = 0; u < 2; ++u) {
+        const int d = tid + u * kAnyThreads;
+        if (d >= dim) break;
 #pragma unroll
-      for (int r = 0; r < kRowsPerCta; ++r) acc[u][r] *= s_corr[r];
-      for (int j = 0; j < kTileKeys; j += 4) {
-        const float v0 = s_kv[j * pitch + d], v1 = s_kv[(j + 1) * pitch + d];
-        const float v2 = s_kv[(j + 2) * pitch + d], v3 = s_kv[(j + 3) * pitch + d];
+        for (int r = 0; r < kRowsPerCta; ++r) acc[u][r] *= s_corr[r];
+        // a NaN stays with the rows that see its key
+        auto behind = [&](float p, float v) { return guard.value && p == 0.f ? 0.f : v; };
+        for (int j = 0; j < kTileKeys; j += 4) {
+          const float v0 = s_kv[j * pitch + d], v1 = s_kv[(j + 1) * pitch + d];
+          const float v2 = s_kv[(j + 2) * pitch + d], v3 = s_kv[(j + 3) * pitch + d];
 #pragma unroll
-        for (int r = 0; r < kRowsPerCta; ++r) {
-          const float4 p = *reinterpret_cast<const float4*>(s_p + r * kTileKeys + j);
-          acc[u][r] = fmaf(p.x, v0, fmaf(p.y, v1, fmaf(p.z, v2, fmaf(p.w, v3, acc[u][r]))));
+          for (int r = 0; r < kRowsPerCta; ++r) {
+            const float4 p = *reinterpret_cast<const float4*>(s_p + r * kTileKeys + j);
+            acc[u][r] += fmaf(p.x, behind(p.x, v0), fmaf(p.y, behind(p.y, v1),
+                                                        fmaf(p.z, behind(p.z, v2), p.w * behind(p.w, v3))));
+          }
         }
       }
-    }
+    };
+    if (any_nan) product(std::true_type{});
+    else product(std::false_type{});
   }
   __syncthreads();
   if (g.splits == 1) {
@@ -219,7 +232,7 @@ __global__ void __launch_bounds__(kMaxDim) kv8_attn_join_kernel(AnyArgs g) {
   const int nh = min(g.head_chunk, a.group - chunk * g.head_chunk);
   int64_t row0 = blockIdx.x, tokens = 1;
   if (KEYS == kExtend) {
-    const ExtendEntry x = extend_tile(a, blockIdx.x, g.tile_tokens, nullptr);
+    const ExtendEntry x = extend_tile(a, blockIdx.x, g.tile_tokens, 1, nullptr);
     if (x.entry < 0) return;
     row0 = x.row0 + x.tile * g.tile_tokens;
     tokens = min((int64_t)g.tile_tokens, x.n - x.tile * g.tile_tokens);
@@ -277,6 +290,7 @@ int launch_any(AnyArgs g, int64_t tiles, cudaStream_t s) {
 
 int run(const AttnArgs& a, int keys, int dtype, int64_t max_keys, size_t ws_bytes, cudaStream_t s) {
   if (keys != kExtend && decode_tc_fits(a, dtype)) return run_decode_tc(a, keys, max_keys, ws_bytes, s);
+  if (keys == kExtend && extend_tc_fits(a, dtype)) return run_extend_tc(a, max_keys, ws_bytes, s);
   AnyArgs g = any_shape(a, keys);
   const int64_t tiles = any_tiles(g, keys, a.bs, a.tokens);
   if (tiles > INT32_MAX || (int64_t)a.c.kv_heads * g.chunks > 65535) return QQ_ERR_UNSUPPORTED;
@@ -338,6 +352,12 @@ extern "C" size_t qq_kv8_workspace_bytes(const qq_kv8_cache* cache, int q_heads,
   // enough for either kernel: which one runs depends on the pointers' alignment too
   if (keys != kExtend && decode_tc_fits(a, dtype)) {
     const size_t tc = decode_tc_workspace(bs, a.c.kv_heads, a.group, max_keys);
+    if (tc > need) need = tc;
+  }
+  a.bs = bs;
+  a.tokens = num_tokens;
+  if (keys == kExtend && extend_tc_fits(a, dtype)) {
+    const size_t tc = extend_tc_workspace(bs, a.c.kv_heads, a.group, num_tokens, max_keys);
     if (tc > need) need = tc;
   }
   return need;

@@ -62,9 +62,9 @@ struct ExtendEntry {
   int64_t row0, n, prefix;
 };
 
-// Tile `x` of the batch's tiles of `rows` new tokens each; called by one whole warp, the same in every lane.
-// A bad entry has no tiles and is reported.
-__device__ __forceinline__ ExtendEntry extend_tile(const AttnArgs& a, int64_t x, int rows, uint32_t* err) {
+// Tile `x` of the batch's tiles of `rows` rows each, `per` rows to a new token; called by one whole warp, the same
+// in every lane.  A bad entry has no tiles and is reported.
+__device__ __forceinline__ ExtendEntry extend_tile(const AttnArgs& a, int64_t x, int rows, int per, uint32_t* err) {
   ExtendEntry r{-1, 0, 0, 0, 0};
   const int lane = threadIdx.x & 31;
   int64_t before = 0;
@@ -86,7 +86,7 @@ __device__ __forceinline__ ExtendEntry extend_tile(const AttnArgs& a, int64_t x,
         }
       }
     }
-    const int64_t tiles = (n + rows - 1) / rows;
+    const int64_t tiles = (n * per + rows - 1) / rows;
     int64_t incl = tiles;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -129,6 +129,10 @@ __device__ __forceinline__ int64_t key_slot(const AttnArgs& a, int e, int64_t re
 bool decode_tc_fits(const AttnArgs& a, int dtype);
 size_t decode_tc_workspace(int bs, int kv_heads, int group, int64_t max_keys);
 int run_decode_tc(const AttnArgs& a, int keys, int64_t max_keys, size_t ws_bytes, cudaStream_t s);
+// The same for an extend batch.
+bool extend_tc_fits(const AttnArgs& a, int dtype);
+size_t extend_tc_workspace(int bs, int kv_heads, int group, int64_t tokens, int64_t max_keys);
+int run_extend_tc(const AttnArgs& a, int64_t max_keys, size_t ws_bytes, cudaStream_t s);
 
 }  // namespace kv8
 }  // namespace qq

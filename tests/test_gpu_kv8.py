@@ -9,7 +9,9 @@ W = sum_j w_j |v_j| and S the largest sum_d |q_d k_jd| * scaling of its keys,
 * n products are summed in fp32: n 2^-24 W at most, and the row sum the same relative to itself;
 * on the tensor cores the weights (times the scale of V) are held as two e4m3 numbers: half a step 2^-4 of half a
   step 2^-4, that is 2^-8 relatively, or where the second falls below the type's normal range a fixed part of the row's
-  largest: one token per request 2^-10 / 16 of 128 at least, 2^-21; the row's sum keeps the fp32 weights;
+  largest: 2^-10 / 16 of 128 at least, 2^-21; the row's sum keeps the fp32 weights.  An extend batch holds them in
+  fp16 instead, 2^-11, or 2^-25 of 1 at least, and its queries too: off by 2^-25 of 112 at least (2^-31 of the row's
+  largest) where bf16's 8 bits leave the normal range, which the first bound covers: both bounds below cover both;
 * the result is rounded once: half a step, 2^-8 in bf16 and 2^-24 in fp32.
 """
 
@@ -554,6 +556,25 @@ def test_a_nan_reaches_the_heads_that_see_it_and_no_others():
             bad = o.isnan()
             assert bad[0, 4:].all() and not bad[0, :4].any()
             assert bad[1, 2].all() and not bad[1, :2].any() and not bad[1, 3:].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_nan_of_a_later_token_stays_behind_the_mask(dtype):
+    """Keys and values of token 150 are NaN: the rows up to 149 are what they would be without it."""
+    seq = [200]
+    b = _Batch(seq, 2, 128, 64, seed=12, heads=8, dtype=dtype)
+    at = int(b.slots(0, [150])[0])
+    q = b.queries(200)
+    args = (_dev(b.reqs), _dev(seq), _dev([0]), _dev([0]), b.scaling)
+    want = b.cache.extend_attention(0, q.to(DEV), b.table_dev, *args)
+    for codes in (b.cache.k, b.cache.v):
+        saved = codes[0].clone()
+        codes[0].view(torch.uint8)[at // 64, 1, at % 64, 5] = 0xFF
+        got = b.cache.extend_attention(0, q.to(DEV), b.table_dev, *args).view(200, 8, 128)
+        b.cache.synchronize()
+        assert torch.equal(got[:150].reshape(150, -1), want[:150]) and torch.equal(got[:, :4], want.view(200, 8, 128)[:, :4])
+        assert got[150:, 4:, 5].isnan().all()
+        codes[0].view(torch.uint8).copy_(saved.view(torch.uint8))
 
 
 def test_attention_reports_bad_entries_and_serves_the_others():
