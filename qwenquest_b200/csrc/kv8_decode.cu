@@ -202,15 +202,15 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
       mbar_init(bar(kBarEmpty + i), 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(bar(kBarQ + i), 32);
+      mbar_init(bar(kBarQ + i), 1);
       mbar_init(bar(kBarQFree + i), 1);
       mbar_init(bar(kBarS + i), 1);
-      mbar_init(bar(kBarP + i), kSoft);
+      mbar_init(bar(kBarP + i), kSoft / 32);
       mbar_init(bar(kBarO + i), 1);
     }
     for (int i = 0; i < kMeta; ++i) {
-      mbar_init(bar(kBarMeta + i), 32);
-      mbar_init(bar(kBarMetaFree + i), kSoft);
+      mbar_init(bar(kBarMeta + i), 1);
+      mbar_init(bar(kBarMetaFree + i), kSoft / 32);
     }
     mbar_init(bar(kBarDone), 1);
     mbar_init_fence();
@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
         if ((lane & 3) == 0) s_qinv[pair & 3][r] = a.scale_log2 * exp2_int(-k2);
       }
       fence_async_shared();
-      mbar_arrive(bar(kBarQ + qb));
+      mbar_arrive_warp(bar(kBarQ + qb));
       ++pair;
       first = w.last();
     }
@@ -469,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
         const int k = u * 32 + lane;
         if (k < kMetaN) s_ks[m][k] = ks[u], s_vs[m][k] = vs[u];
       }
-      mbar_arrive(bar(kBarMeta + m));
+      mbar_arrive_warp(bar(kBarMeta + m));
     }
   } else {
     // ================================================================ softmax (warps 0-3)
@@ -507,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
       const float ks = s_ks[m][mk], vs = s_vs[m][mk];
       const bool seen = (int64_t)w.t * kTile + tok < w.n && __float_as_uint(vs) != kMasked;
       ok = __all_sync(0xffffffffu, ok && wait(kBarS + b, (i >> 1) & 1));
-      mbar_arrive(bar(kBarMetaFree + m));
+      mbar_arrive_warp(bar(kBarMetaFree + m));
       uint32_t v[NC] = {};
       if (ok) {
         tc_fence_after();
@@ -565,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
       }
       fence_async_shared();
       tc_fence_before();
-      mbar_arrive(bar(kBarP + b));
+      mbar_arrive_warp(bar(kBarP + b));
       if (!first) add_product(i - 1, before_corr);
       first = w.last();
       if (!first && i + 1 < count) continue;

@@ -44,13 +44,17 @@ constexpr int kTileBytes = 128 * kTcDim * 2; // 32 KiB: 128 rows of fp16, two 64
 constexpr int kHalf = kTileBytes / 2;
 constexpr int kStages = 2;                   // K tiles and V tiles in shared memory
 constexpr int kMeta = 4;
-constexpr int kGroups = kN / 16;
+constexpr int kGroups = kN / 16;               // groups of 16 keys at most in a tile
 constexpr int kWidenWarp = 8, kMmaWarp = 12, kScaleWarp = 14;
-constexpr int kThreads = 15 * 32;
+constexpr int kThreads = 16 * 32;  // four warpgroups
+// Registers per thread: 128 at launch (all 65,536 over 512 threads), then by role.
+constexpr int kRegsSoft = 152, kRegsWiden = 120, kRegsRest = 88;
+static_assert(128 * (2 * kRegsSoft + kRegsWiden + kRegsRest) <= kThreads * 128, "the launch's registers");
 constexpr int kOffQ = 0, kOffK = 2 * kTileBytes, kOffV = kOffK + kStages * kTileBytes;
 constexpr int kDynSmem = kOffV + kStages * kTileBytes + 1024;
 constexpr uint32_t kTmemCols = 512;
-constexpr float kRaise = 8.f;
+constexpr float kRaiseAt = 256.f, kMost = 32768.f;
+constexpr int kPoly = 4;  // one pair in kPoly of the exponentials on the FMA pipe
 
 enum : int {
   kBarQ = 0,                          // [2] queries of a tile written
@@ -61,8 +65,8 @@ enum : int {
   kBarMeta = kBarVFree + kStages,     // [kMeta] scales written
   kBarMetaFree = kBarMeta + kMeta,
   kBarS = kBarMetaFree + kMeta,       // [2] scores made
-  kBarP = kBarS + 2,                  // [2] weights written
-  kBarO = kBarP + 2,                  // [2] a product made
+  kBarP = kBarS + 2,                  // [2][2] weights of a tile's first and second 64 keys written
+  kBarO = kBarP + 4,                  // [2] the product of a tile's first 64 keys made
   kBarDone = kBarO + 2,               // [2] the tile's last MMA has finished
   kNumBars = kBarDone + 2
 };
@@ -84,10 +88,19 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-__device__ __forceinline__ uint32_t widen2(uint32_t codes) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)codes));
-  return r;
+// Four e4m3 codes as two fp16 pairs (exact).
+__device__ __forceinline__ void widen4(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}\n"
+      : "=r"(lo), "=r"(hi)
+      : "r"(codes));
+}
+// acc = 0 h + acc in every half: NaN once one of h is (on the FMA pipe, which has room).
+__device__ __forceinline__ void nan_of(uint32_t& acc, const uint4& h) {
+  asm("fma.rn.f16x2 %0, %1, %5, %0;\n\tfma.rn.f16x2 %0, %2, %5, %0;\n\t"
+      "fma.rn.f16x2 %0, %3, %5, %0;\n\tfma.rn.f16x2 %0, %4, %5, %0;"
+      : "+r"(acc)
+      : "r"(h.x), "r"(h.y), "r"(h.z), "r"(h.w), "r"(0));
 }
 __device__ __forceinline__ float max3(float x, float y, float z) {
   float r;
@@ -95,30 +108,110 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
   return r;
 }
 
-// The CTA's rows and keys.
+// Loads under a predicate that leave their registers alone until they land (a
+// select behind a load would wait for it on the spot).
+__device__ __forceinline__ uint2 load8_or_zero(const void* p, bool there) {
+  uint2 r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %3, 0;\n\tmov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\t"
+      "@p ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];\n\t}\n"
+      : "=&r"(r.x), "=&r"(r.y)
+      : "l"(p), "r"((int)there));
+  return r;
+}
+__device__ __forceinline__ int32_t load_or(const int32_t* p, bool there, int32_t other) {
+  int32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.u32 %0, %3;\n\t@p ld.global.nc.u32 %0, [%1];\n\t}\n"
+      : "=&r"(r)
+      : "l"(p), "r"((int)there), "r"(other));
+  return r;
+}
+
+__device__ __forceinline__ void st_shared16(uint32_t addr, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// Two fp32 numbers in a register pair: one instruction of the fp32 pipe for both.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 both_of(f32x2 x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 x, f32x2 y, f32x2 z) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 x, f32x2 y) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 x, f32x2 y) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+  return r;
+}
+
+// 2^x of both on the FMA pipe, for x <= 9 (below -125: 2^-125; NaN stays NaN):
+// x = r + f with r = round(x) by the 1.5 * 2^23 shift, 2^f a polynomial of
+// degree 3 fitted here (relative error 7.5e-5, against fp16's 2^-11), 2^r from
+// r in the shifted number's low bits.
+__device__ __forceinline__ f32x2 exp2_fma(f32x2 x) {
+  float2 c = both_of(x);
+  asm("max.NaN.f32 %0, %0, 0fC2FA0000;" : "+f"(c.x));  // -125
+  asm("max.NaN.f32 %0, %0, 0fC2FA0000;" : "+f"(c.y));
+  x = pair(c.x, c.y);
+  const f32x2 t = add2(x, pair(12582912.f, 12582912.f));
+  const f32x2 r = add2(t, pair(-12582912.f, -12582912.f));
+  const f32x2 f = fma2(r, pair(-1.f, -1.f), x);
+  f32x2 p = fma2(pair(0.05517166f, 0.05517166f), f, pair(0.24261113f, 0.24261113f));
+  p = fma2(p, f, pair(0.69326097f, 0.69326097f));
+  p = fma2(p, f, pair(0.99992806f, 0.99992806f));
+  const float2 tt = both_of(t);
+  return mul2(p, pair(__uint_as_float(__float_as_uint(tt.x) * 0x800000u + 0x3F800000u),
+                      __uint_as_float(__float_as_uint(tt.y) * 0x800000u + 0x3F800000u)));
+}
+
+// The CTA's rows and keys (all within 32 bits: at most 65535 tiles of 256
+// rows, and positions of a table of less than 2^31 tokens).
 struct Unit {
-  ExtendEntry x;
-  int64_t row0, rows;      // rows [row0, row0 + rows) of the entry's n * group
-  int64_t req;
-  int64_t key_begin, key_end;
+  int entry;               // -1: none
+  int q_row;               // the entry's first query row
+  int prefix;
+  int row0, rows;          // rows [row0, row0 + rows) of the entry's n * group
+  int key_begin, key_end;
   int tiles;
+  const int32_t* table;    // the request's blocks
 };
 __device__ __forceinline__ Unit unit_of(const ExtendArgs& g, int64_t tile, int split, uint32_t* err) {
   const AttnArgs& a = g.a;
   Unit u{};
-  u.x = extend_tile(a, tile, kUnitRows, a.group, err);
-  if (u.x.entry < 0) return u;
-  u.row0 = u.x.tile * kUnitRows;
-  u.rows = min((int64_t)kUnitRows, u.x.n * a.group - u.row0);
-  u.req = a.reqs[u.x.entry];
-  const int64_t keys = u.x.prefix + (u.row0 + u.rows - 1) / a.group + 1;  // what its last row sees
-  const int64_t all = (keys + kN - 1) / kN, each = (all + g.splits - 1) / g.splits;
+  const ExtendEntry x = extend_tile(a, tile, kUnitRows, a.group, err);
+  u.entry = x.entry;
+  if (x.entry < 0) return u;
+  u.q_row = (int)x.row0;
+  u.prefix = (int)x.prefix;
+  u.row0 = (int)x.tile * kUnitRows;
+  u.rows = min(kUnitRows, (int)x.n * a.group - u.row0);
+  u.table = a.table + a.reqs[x.entry] * a.table_stride;
+  const int keys = u.prefix + (u.row0 + u.rows - 1) / a.group + 1;  // what its last row sees
+  const int all = (keys + kN - 1) / kN, each = (all + g.splits - 1) / g.splits;
   u.key_begin = min(all, split * each) * kN;
   u.key_end = min(keys, u.key_begin + each * kN);
-  u.tiles = u.key_end > u.key_begin ? (int)((u.key_end - u.key_begin + kN - 1) / kN) : 0;
+  u.tiles = max(0, (u.key_end - u.key_begin + kN - 1) / kN);
   return u;
 }
 
+// kGroup: keys that share their scales, 16, or 64 where blocks are that long.
+template <int kGroup>
 __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bars[kNumBars];
@@ -146,27 +239,28 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
   if (threadIdx.x == 32) {
     s_abort = 0;
     for (int i = 0; i < 2; ++i) {
-      mbar_init(bar(kBarQ + i), kM);
+      mbar_init(bar(kBarQ + i), 4);
       mbar_init(bar(kBarS + i), 1);
-      mbar_init(bar(kBarP + i), kM);
+      mbar_init(bar(kBarP + 2 * i), 4);
+      mbar_init(bar(kBarP + 2 * i + 1), 4);
       mbar_init(bar(kBarO + i), 1);
       mbar_init(bar(kBarDone + i), 1);
     }
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(bar(kBarK + i), 128);
-      mbar_init(bar(kBarV + i), 128);
+      mbar_init(bar(kBarK + i), 4);
+      mbar_init(bar(kBarV + i), 4);
       mbar_init(bar(kBarKFree + i), 2);
       mbar_init(bar(kBarVFree + i), 2);
     }
     for (int i = 0; i < kMeta; ++i) {
-      mbar_init(bar(kBarMeta + i), 32);
-      mbar_init(bar(kBarMetaFree + i), kUnitRows);
+      mbar_init(bar(kBarMeta + i), 1);
+      mbar_init(bar(kBarMetaFree + i), 8);
     }
     mbar_init_fence();
   }
   __syncthreads();
   const Unit& u = s_unit;
-  if (u.x.entry < 0) return;  // past the last tile, uniform
+  if (u.entry < 0) return;  // past the last tile, uniform
   if (warp == kMmaWarp) tmem_alloc(smem_u32(&s_tmem), kTmemCols);
   tc_fence_before();
   __syncthreads();
@@ -174,155 +268,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
   const uint32_t tmem = s_tmem;
   const int tiles = u.tiles;
 
-  if (warp >= kWidenWarp && warp < kMmaWarp) {
-    // ================================================================ K and V to fp16
-    // Eight lanes per key row, 16 codes each; a warp's 32 rows in eight steps.
-    // The codes of the next tile are on their way while one is widened.
-    const int ww = warp - kWidenWarp, ch = lane & 7;
-    // lane L holds the pool row of key ww * 32 + L of a tile; -1: zeros
-    auto key_row = [&](int j) -> int32_t {
-      const int64_t p = u.key_begin + (int64_t)j * kN + ww * 32 + lane;
-      if (p >= u.key_end) return -1;
-      const int64_t s = key_slot<kTable>(a, u.x.entry, u.req, p, kvh == 0 ? a.err : nullptr);
-      return s < 0 ? -1 : (int32_t)(((s >> c.shift) * c.kv_heads + kvh) * c.block + (s & (c.block - 1)));
-    };
-    auto load = [&](const uint8_t* pool, int32_t rows, uint4 (&w)[8]) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int32_t r = __shfl_sync(0xffffffffu, rows, i * 4 + (lane >> 3));
-        w[i] = r < 0 ? make_uint4(0, 0, 0, 0)
-                     : __ldg(reinterpret_cast<const uint4*>(pool + (int64_t)r * kTcDim + ch * 16));
-      }
-    };
-    auto store = [&](uint32_t off, const uint4 (&w)[8]) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = ww * 32 + i * 4 + (lane >> 3);
-        const uint4 lo = make_uint4(widen2(w[i].x), widen2(w[i].x >> 16), widen2(w[i].y), widen2(w[i].y >> 16));
-        const uint4 hi = make_uint4(widen2(w[i].z), widen2(w[i].z >> 16), widen2(w[i].w), widen2(w[i].w >> 16));
-        // 16-byte pieces 2 ch and 2 ch + 1 of the row's 16; the two blocks of a
-        // row share their banks, so the lanes of the second one start with the odd piece
-        uint8_t* row = smem + off + (ch >> 2) * kHalf + r * 128;
-        const int p0 = (((2 * ch) & 7) ^ (r & 7)) << 4, p1 = (((2 * ch + 1) & 7) ^ (r & 7)) << 4;
-        const bool odd = ch >= 4;
-        *reinterpret_cast<uint4*>(row + (odd ? p1 : p0)) = odd ? hi : lo;
-        *reinterpret_cast<uint4*>(row + (odd ? p0 : p1)) = odd ? lo : hi;
-      }
-      fence_async_shared();
-    };
-    // A weight of zero does not hide a NaN of V from the rows that may not see
-    // its key.  So a key with one gets zeros for V and NaN for K: the rows that
-    // see it become NaN, the scores of the others are masked.
-    auto hide_nan = [&](uint4 (&k)[8], uint4 (&v)[8]) {
-      auto nan4 = [](uint32_t w) { return (w & 0x7F7F7F7Fu) + 0x01010101u; };  // top bits: codes 0x7F and 0xFF
-      auto nan16 = [&](const uint4& w) { return (nan4(w.x) | nan4(w.y) | nan4(w.z) | nan4(w.w)) & 0x80808080u; };
-      uint32_t any = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) any |= nan16(v[i]);
-      if (!__any_sync(0xffffffffu, any != 0)) return;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t m = __ballot_sync(0xffffffffu, nan16(v[i]) != 0);
-        if (m >> (lane & 24) & 255u) {
-          v[i] = make_uint4(0, 0, 0, 0);
-          k[i] = make_uint4(0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu);
-        }
-      }
-    };
-    uint4 wk[8], wv[8];
-    int32_t next = tiles > 0 ? key_row(0) : -1;
-    if (tiles > 0) {
-      load(c.k, next, wk);
-      load(c.v, next, wv);
-    }
-#pragma unroll 1
-    for (int j = 0; j < tiles; ++j) {
-      const int st = j % kStages;
-      const uint32_t turn = ((j / kStages) - 1) & 1;
-      if (j + 1 < tiles) next = key_row(j + 1);
-      hide_nan(wk, wv);
-      if (j >= kStages && !__all_sync(0xffffffffu, wait(kBarKFree + st, turn))) break;
-      store(kOffK + st * kTileBytes, wk);
-      mbar_arrive(bar(kBarK + st));
-      if (j + 1 < tiles) load(c.k, next, wk);
-      if (j >= kStages && !__all_sync(0xffffffffu, wait(kBarVFree + st, turn))) break;
-      store(kOffV + st * kTileBytes, wv);
-      mbar_arrive(bar(kBarV + st));
-      if (j + 1 < tiles) load(c.v, next, wv);
-    }
-  } else if (warp == kScaleWarp) {
-    // ================================================================ scales
-    for (int j = 0; j < tiles; ++j) {
-      const int m = j % kMeta;
-      float4 f = make_float4(0.f, -INFINITY, 0.f, 0.f);
-      const int64_t p = u.key_begin + (int64_t)j * kN + lane * 16;
-      if (lane < kGroups && p < u.key_end) {
-        const int64_t s = key_slot<kTable>(a, u.x.entry, u.req, p, nullptr);
-        if (s >= 0) {
-          const int64_t bh = (s >> c.shift) * c.kv_heads + kvh;
-          f.x = c.k_scale[bh];
-          // 2^-lg stays a normal number
-          f.y = fminf(fmaxf(log2f(c.v_scale[bh]), -100.f), 126.f);
-          if (isnan(c.v_scale[bh])) f.y = c.v_scale[bh];
-          f.z = exp2f(-f.y);
-        }
-      }
-      if (j >= kMeta && !__all_sync(0xffffffffu, wait(kBarMetaFree + m, ((j / kMeta) - 1) & 1))) break;
-      if (lane < kGroups) s_scale[m][lane] = f;
-      mbar_arrive(bar(kBarMeta + m));
-    }
-  } else if (warp >= kMmaWarp) {
-    // ================================================================ MMA issue, one warp per M tile
-    if (lane == 0 && tiles > 0) {
-      const int h = warp - kMmaWarp;
-      const uint32_t tS = tmem + h * 256, tO = tS + 128;
-      const uint64_t dq = desc_k(base + kOffQ + h * kTileBytes);
-      bool ok = wait(kBarQ + h, 0);
-      auto scores = [&](int j) {
-        const int st = j % kStages;
-        ok = ok && wait(kBarK + st, (j / kStages) & 1);
-        if (!ok) return;
-        tc_fence_after();
-        const uint64_t dk = desc_k(base + kOffK + st * kTileBytes);
-        umma_bf16_x4(tS, dq, dk, 2, 2, kIdS, 0u);
-        umma_bf16_x4(tS, dq + (kHalf >> 4), dk + (kHalf >> 4), 2, 2, kIdS, 1u);
-        umma_commit(bar(kBarS + h));
-        umma_commit(bar(kBarKFree + st));
-      };
-      scores(0);
-#pragma unroll 1
-      for (int j = 0; j < tiles && ok; ++j) {
-        const int st = j % kStages;
-        ok = wait(kBarV + st, (j / kStages) & 1) && wait(kBarP + h, j & 1);
-        if (!ok) break;
-        tc_fence_after();
-        const uint64_t dv = desc_mn(base + kOffV + st * kTileBytes, kHalf);
-        umma_bf16_ts_x4(tO, tS, dv, 8, (16 * 128) >> 4, kIdO, j > 0 ? 1u : 0u);
-        umma_bf16_ts_x4(tO, tS + 32, dv + ((64 * 128) >> 4), 8, (16 * 128) >> 4, kIdO, 1u);
-        umma_commit(bar(kBarO + h));
-        umma_commit(bar(kBarVFree + st));
-        if (j + 1 < tiles) scores(j + 1);
-      }
-      umma_commit(bar(kBarDone + h));
-      mbar_wait(bar(kBarDone + h), 0, abort_flag, a.err, true);
-    }
-    __syncwarp();
-  } else {
+  if (warp < kWidenWarp) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoft));
     // ================================================================ softmax (warps 0-7)
     const int h = warp >> 2, r = threadIdx.x;      // row of the CTA's 256
-    const int64_t row = u.row0 + r;
-    const int64_t token = row / a.group;
-    const int head = kvh * a.group + (int)(row - token * a.group);
+    const int token = (u.row0 + r) / a.group;
+    const int head = kvh * a.group + u.row0 + r - token * a.group;
     // ---- this warp's 32 query rows to fp16: four lanes per row, 32 channels each
 #pragma unroll 1
     for (int r0 = 0; r0 < 32; r0 += 8) {
       const int rr = warp * 32 + r0 + (lane >> 2), col = (lane & 3) * 32;
       float x[32] = {};
       if (rr < u.rows) {
-        const int64_t t = (u.row0 + rr) / a.group;
-        const int hd = kvh * a.group + (int)(u.row0 + rr - t * a.group);
+        const int t = (u.row0 + rr) / a.group;
+        const int hd = kvh * a.group + u.row0 + rr - t * a.group;
         const uint4* q = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) +
-                                                        (u.x.row0 + t) * a.q_stride + (int64_t)hd * kTcDim + col);
+                                                        (int64_t)(u.q_row + t) * a.q_stride + (int64_t)hd * kTcDim + col);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const uint4 w = q[k];
@@ -355,120 +316,165 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
       if ((lane & 3) == 0) s_up[rr] = fabsf(a.scale_log2) * exp2_int(-k2);
     }
     fence_async_shared();
-    mbar_arrive(bar(kBarQ + h));
+    mbar_arrive_warp(bar(kBarQ + h));
     __syncwarp();
     const float inv_up = s_up[r];
 
     const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16) + h * 256, tO = tS + 128;
-    const int64_t qpos = u.x.prefix + token;
-    float m_used = -INFINITY, l = 0.f;
+    const int reach = u.prefix + token - u.key_begin;  // the last key this row sees, in its stretch
+    // The weights' reference m need not be the running maximum, only near
+    // enough for fp16 (2^-24 to 2^16) and fp32: it starts as the maximum of the
+    // first tile with a key, and is raised by log2 of a half tile's sum where
+    // that passes 2^kRaise, for the tiles to come.  So the scores are read
+    // once; a half whose sum passes 2^kMost (a weight might not fit fp16) is
+    // made again from the tile's maximum.
+    float m = -INFINITY, l = 0.f, alpha = 1.f;  // O still has to be multiplied by alpha
     bool ok = true;
 #pragma unroll 1
     for (int j = 0; j < tiles; ++j) {
-      const int m = j % kMeta;
-      ok = __all_sync(0xffffffffu, wait(kBarMeta + m, (j / kMeta) & 1) && wait(kBarS + h, j & 1));
+      const int meta = j % kMeta;
+      ok = __all_sync(0xffffffffu, wait(kBarMeta + meta, (j / kMeta) & 1) && wait(kBarS + h, j & 1));
       if (!ok) break;
       tc_fence_after();
       // columns c <= lim are seen by this row
-      const int64_t lim64 = qpos - u.key_begin - (int64_t)j * kN;
-      const int lim = lim64 > kN - 1 ? kN - 1 : (lim64 < -1 ? -1 : (int)lim64);
+      const int lim = max(-1, min(kN - 1, reach - j * kN));
       const bool full = __all_sync(0xffffffffu, lim == kN - 1);
-      float v[64];
-      auto half = [&](int hf) {
-        tmem_ld32(tS + hf * 64, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
-        tmem_ld32(tS + hf * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
-        tmem_ld_wait();
-        if (!full) {
+      uint32_t v[2][32];  // scores in chunks of 32 columns, the next one always on its way
+      float part, sum;    // of the half in hand: what l takes, and the plain sum
+      float most = 0.f;   // the larger of the halves' sums
+      uint32_t pk[32];
+      // The maximum (with its scales) over the chunks from k0 on; the two buffers are free afterwards.
+      auto highest = [&](int k0) {
+        float mb = -INFINITY;
+#pragma unroll 1
+        for (int k = k0; k < 4; ++k) {
+          tmem_ld32(tS + k * 32, v[0]);
+          tmem_wait_ld32(v[0]);
 #pragma unroll
-          for (int e = 0; e < 64; ++e) v[e] = hf * 64 + e <= lim ? v[e] : -INFINITY;
+          for (int q = 0; q < 32; q += kGroup) {
+            const float4 f = s_scale[meta][(k * 32 + q) / kGroup];
+            float y = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < (kGroup < 32 ? kGroup : 32); ++e)
+              y = fmaxf(y, k * 32 + q + e <= lim ? __uint_as_float(v[0][q + e]) : -INFINITY);
+            // a masked group (-inf) stays -inf also where its scale is 0
+            mb = fmaxf(mb, y == -INFINITY ? y : fmaf(y, inv_up * f.x, f.y));
+          }
         }
+        return mb;
       };
-      float mb = -INFINITY;
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        half(hf);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float4 f = s_scale[m][hf * 4 + q];
-          const float* w = v + q * 16;
-          float x = max3(max3(w[0], w[1], w[2]), w[3], w[4]), y = max3(max3(w[5], w[6], w[7]), w[8], w[9]);
-          x = max3(x, w[10], w[11]), y = max3(y, w[12], w[13]);
-          x = max3(x, w[14], w[15]);
-          x = fmaxf(x, y);
-          // a masked group (-inf) stays -inf also where its scale is 0
-          mb = fmaxf(mb, x == -INFINITY ? x : fmaf(x, inv_up * f.x, f.y));
-        }
-      }
-      const bool raise = mb > m_used + kRaise;
-      float alpha = 1.f;
-      if (raise) {
-        alpha = ex2(m_used - mb);
-        m_used = mb;
-        l *= alpha;
-      }
-      if (j > 0 && __any_sync(0xffffffffu, raise)) {
-        ok = __all_sync(0xffffffffu, wait(kBarO + h, (j - 1) & 1));
-        if (!ok) break;
-        tc_fence_after();
-        uint32_t o[32];
+      // O times alpha: no product is under way (S(j) was committed behind O(j - 1))
+      auto rescale = [&]() {
 #pragma unroll 1
         for (int k = 0; k < kTcDim / 32; ++k) {
-          tmem_ld32(tO + k * 32, o);
-          tmem_ld_wait();
+          tmem_ld32(tO + k * 32, v[0]);
+          tmem_wait_ld32(v[0]);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-          tmem_st32(tO + k * 32, o);
+          for (int e = 0; e < 32; ++e) v[0][e] = __float_as_uint(__uint_as_float(v[0][e]) * alpha);
+          tmem_st32(tO + k * 32, v[0]);
         }
         tmem_st_wait();
+        alpha = 1.f;
+      };
+      if (__any_sync(0xffffffffu, m == -INFINITY)) {
+        const float mb = highest(0);
+        if (m == -INFINITY) m = mb;
       }
-      // the second half is still in registers; P of the first half goes over columns the first half has left
-      const float ref = m_used == -INFINITY ? 0.f : m_used;
-      uint32_t pk[32];
-      auto weights = [&](int hf, auto is_full) {
+      if (__any_sync(0xffffffffu, alpha != 1.f)) rescale();
+      tmem_ld32(tS, v[0]);
+
+      // P of chunk k (v[k & 1]) into pk, its sums into part and sum
+      auto chunk = [&](int k, auto is_full) {
+        const uint32_t(&x)[32] = v[k & 1];
+        const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float4 f = s_scale[m][hf * 4 + q];
+        for (int q = 0; q < 32; q += kGroup) {
+          const float4 f = s_scale[meta][(k * 32 + q) / kGroup];
           const float mul = inv_up * f.x, add = f.y - ref;
-          float s0 = 0.f, s1 = 0.f;
+          const f32x2 mul_2 = pair(mul, mul), add_2 = pair(add, add);
+          f32x2 s[2] = {0, 0};
 #pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            float p0 = ex2(fmaf(v[q * 16 + e], mul, add)), p1 = ex2(fmaf(v[q * 16 + e + 1], mul, add));
-            if (!is_full.value) {
-              p0 = hf * 64 + q * 16 + e <= lim ? p0 : 0.f;
-              p1 = hf * 64 + q * 16 + e + 1 <= lim ? p1 : 0.f;
+          for (int e = 0; e < (kGroup < 32 ? kGroup : 32); e += 2) {
+            const f32x2 y = fma2(pair(__uint_as_float(x[q + e]), __uint_as_float(x[q + e + 1])), mul_2, add_2);
+            f32x2 p;
+            if (kPoly > 0 && (e >> 1) % (kPoly > 0 ? kPoly : 1) == 1) {  // some on the FMA pipe: the exponentials' is as busy as the tensor cores
+              p = exp2_fma(y);
+            } else {
+              const float2 t = both_of(y);
+              p = pair(ex2(t.x), ex2(t.y));
             }
-            s0 += p0;
-            s1 += p1;
-            pk[(q * 16 + e) / 2] = pack_f16(p0, p1);
+            float2 w = both_of(p);
+            if (!is_full.value) {
+              w.x = k * 32 + q + e <= lim ? w.x : 0.f;
+              w.y = k * 32 + q + e + 1 <= lim ? w.y : 0.f;
+              p = pair(w.x, w.y);
+            }
+            s[(e >> 1) & 1] = add2(s[(e >> 1) & 1], p);
+            pk[(k & 1) * 16 + (q + e) / 2] = pack_f16(w.x, w.y);
           }
-          l = fmaf(s0 + s1, f.z, l);
+          const float2 s2 = both_of(add2(s[0], s[1]));
+          part = fmaf(s2.x + s2.y, f.z, part);
+          sum += s2.x + s2.y;
         }
       };
-      uint32_t pk1[32];
-      auto both = [&](auto is_full) {
-        weights(1, is_full);
-#pragma unroll
-        for (int e = 0; e < 32; ++e) pk1[e] = pk[e];
-        half(0);
-        weights(0, is_full);
+      // 64 keys: weights, sums, P, and word to the MMA warp.  P goes over columns
+      // whose scores have been read; the product of the first half runs while
+      // the second half's exponentials do.
+      auto half = [&](int hf, auto is_full) {
+        for (int tries = 0;; ++tries) {
+          part = 0.f, sum = 0.f;
+          tmem_wait_ld32(v[0]);
+          tmem_ld32(tS + hf * 64 + 32, v[1]);
+          chunk(2 * hf, is_full);
+          tmem_wait_ld32(v[1]);
+          if (hf == 0) tmem_ld32(tS + 64, v[0]);
+          chunk(2 * hf + 1, is_full);
+          const bool over = sum > kMost;
+          if (tries == 1 || !__any_sync(0xffffffffu, over)) break;
+          if (hf == 0) tmem_wait_ld32(v[0]);
+          const float mb = highest(2 * hf);  // P of the first half lies over its scores by now
+          if (over) {
+            alpha = ex2(m - mb);
+            l *= alpha;
+            most *= alpha;
+            m = mb;
+          }
+          if (hf == 1) ok = __all_sync(0xffffffffu, ok && wait(kBarO + h, j & 1));
+          tc_fence_after();
+          if (ok && (hf == 1 || j > 0)) rescale();
+          alpha = 1.f;
+          tmem_ld32(tS + hf * 64, v[0]);
+        }
+        l += part;
+        tmem_st32(tS + hf * 32, pk);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive_warp(bar(kBarP + 2 * h + hf));
+        most = fmaxf(most, sum);
       };
-      if (full) both(std::true_type{});
-      else both(std::false_type{});
-      tmem_st32(tS, pk);
-      tmem_st32(tS + 32, pk1);
-      tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(bar(kBarP + h));
-      mbar_arrive(bar(kBarMetaFree + m));
+      if (full) {
+        half(0, std::true_type{});
+        half(1, std::true_type{});
+      } else {
+        half(0, std::false_type{});
+        half(1, std::false_type{});
+      }
+      if (most > kRaiseAt) {  // for the tiles to come
+        const float up = __log2f(most);
+        m += up;
+        alpha = ex2(-up);
+        l *= alpha;
+      }
+      mbar_arrive_warp(bar(kBarMetaFree + meta));
     }
     // ---- O / l, or this stretch's record
     ok = __all_sync(0xffffffffu, ok && (tiles == 0 || wait(kBarDone + h, 0)));
     tc_fence_after();
     const bool valid = ok && r < u.rows;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = l == 0.f ? 0.f : alpha / l;
     float* rec = a.part + (((int64_t)tile * c.kv_heads + kvh) * g.splits + blockIdx.z) * kRecord;
-    if (g.splits > 1 && valid) rec[2 * r] = m_used, rec[2 * r + 1] = l;
-    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + (u.x.row0 + token) * a.out_stride + (int64_t)head * kTcDim;
+    if (g.splits > 1 && valid) rec[2 * r] = m, rec[2 * r + 1] = l;
+    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + (int64_t)(u.q_row + token) * a.out_stride + (int64_t)head * kTcDim;
 #pragma unroll 1
     for (int k = 0; k < kTcDim / 32; ++k) {
       uint32_t o[32] = {};
@@ -481,8 +487,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
         float4* w = reinterpret_cast<float4*>(rec + 2 * kUnitRows + (int64_t)r * kTcDim + k * 32);
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          w[e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]),
-                             __uint_as_float(o[4 * e + 3]));
+          w[e] = make_float4(__uint_as_float(o[4 * e]) * alpha, __uint_as_float(o[4 * e + 1]) * alpha,
+                             __uint_as_float(o[4 * e + 2]) * alpha, __uint_as_float(o[4 * e + 3]) * alpha);
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -494,6 +500,151 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
           *reinterpret_cast<uint4*>(dst + k * 32 + e * 8) = w;
         }
       }
+    }
+  } else if (warp < kMmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsWiden));
+    // ================================================================ K and V to fp16
+    // Sixteen lanes per key row, 8 codes each; a warp's 32 rows in sixteen steps.
+    // The codes of the next tile are on their way while one is widened.
+    const int ww = warp - kWidenWarp, hr = lane >> 4, ch = lane & 15;
+    // lane L looks after key ww * 32 + L of a tile: its block (-1 past the end), loaded two tiles ahead, ...
+    const int key0 = u.key_begin + ww * 32 + lane, key_end = u.key_end;
+    const int32_t* const table = u.table;
+    auto key_block = [&](int j) -> int32_t {
+      const int p = key0 + j * kN;
+      return load_or(table + (p >> c.shift), p < key_end, -1);
+    };
+    // ... and its row of the pool; -1: zeros
+    auto key_row = [&](int j, int32_t b) -> int32_t {
+      const int p = key0 + j * kN;
+      if (b >= 0 && b < c.num_blocks) return (b * c.kv_heads + kvh) * c.block + (p & (c.block - 1));
+      if (kvh == 0 && p < key_end) raise_error(a.err, QQ_DEV_ERR_BOUNDS);
+      return -1;
+    };
+    uint2 wk[16], wv[16];
+    auto load = [&](int32_t rows) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int32_t r = __shfl_sync(0xffffffffu, rows, 2 * i + hr);
+        const int64_t at = (int64_t)r * kTcDim + ch * 8;
+        wk[i] = load8_or_zero(c.k + at, r >= 0);
+        wv[i] = load8_or_zero(c.v + at, r >= 0);
+      }
+    };
+    // 8 codes are one 16-byte piece in fp16, swizzled by the row; steps i and i + 4 share a swizzle
+    uint32_t at[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      at[k] = base + (ch >> 3) * kHalf + (ww * 32 + hr) * 128 + (((ch & 7) ^ (2 * k + hr)) << 4);
+    uint32_t nan;  // fp16 pair, NaN once a code of V was
+    auto store = [&](uint32_t off, const uint2 (&w)[16], auto look) {
+      nan = 0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        uint4 h;
+        widen4(w[i].x, h.x, h.y);
+        widen4(w[i].y, h.z, h.w);
+        if (look.value) nan_of(nan, h);
+        st_shared16(at[i & 3] + off + i * 256, h);
+      }
+    };
+    // A weight of zero does not hide a NaN of V from the rows that may not see
+    // its key.  So a key with one gets zeros for V and NaN for K: the rows that
+    // see it become NaN, the scores of the others are masked.
+    auto hide_nan = [&](uint32_t off) {
+      if (!__any_sync(0xffffffffu, (nan & 0x7FFFu) > 0x7C00u || (nan & 0x7FFF0000u) > 0x7C000000u)) return;
+      auto nan4 = [](uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; };  // codes 0x7F and 0xFF
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t m = __ballot_sync(0xffffffffu, (nan4(wv[i].x) | nan4(wv[i].y)) != 0);
+        if (m >> (lane & 16) & 0xFFFFu) {
+          st_shared16(at[i & 3] + off + i * 256, make_uint4(0, 0, 0, 0));
+          wk[i] = make_uint2(0x7F7F7F7Fu, 0x7F7F7F7Fu);
+        }
+      }
+    };
+    int32_t ahead = key_block(1);
+    load(key_row(0, key_block(0)));
+#pragma unroll 1
+    for (int j = 0; j < tiles; ++j) {
+      const int st = j % kStages;
+      const uint32_t turn = ((j / kStages) - 1) & 1;
+      const int32_t next = key_row(j + 1, ahead);
+      ahead = key_block(j + 2);
+      if (j >= kStages && !__all_sync(0xffffffffu, wait(kBarVFree + st, turn))) break;
+      store(kOffV + st * kTileBytes, wv, std::true_type{});
+      hide_nan(kOffV + st * kTileBytes);
+      mbar_arrive_warp(bar(kBarV + st));
+      if (j >= kStages && !__all_sync(0xffffffffu, wait(kBarKFree + st, turn))) break;
+      store(kOffK + st * kTileBytes, wk, std::false_type{});
+      mbar_arrive_warp(bar(kBarK + st));
+      load(next);
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
+    if (warp == kScaleWarp) {
+    // ================================================================ scales
+    for (int j = 0; j < tiles; ++j) {
+      const int m = j % kMeta;
+      float4 f = make_float4(0.f, -INFINITY, 0.f, 0.f);
+      const int p = u.key_begin + j * kN + lane * kGroup;
+      if (lane < kN / kGroup && p < u.key_end) {
+        const int32_t b = u.table[p >> c.shift];
+        if (b >= 0 && b < c.num_blocks) {
+          const int bh = b * c.kv_heads + kvh;
+          f.x = c.k_scale[bh];
+          // 2^-lg stays a normal number
+          f.y = fminf(fmaxf(log2f(c.v_scale[bh]), -100.f), 126.f);
+          if (isnan(c.v_scale[bh])) f.y = c.v_scale[bh];
+          f.z = exp2f(-f.y);
+        }
+      }
+      if (j >= kMeta && !__all_sync(0xffffffffu, wait(kBarMetaFree + m, ((j / kMeta) - 1) & 1))) break;
+      if (lane < kN / kGroup) s_scale[m][lane] = f;
+      mbar_arrive_warp(bar(kBarMeta + m));
+    }
+    } else if (warp < kScaleWarp) {
+    // ================================================================ MMA issue, one warp per M tile
+    if (lane == 0 && tiles > 0) {
+      const int h = warp - kMmaWarp;
+      const uint32_t tS = tmem + h * 256, tO = tS + 128;
+      const uint64_t dq = desc_k(base + kOffQ + h * kTileBytes);
+      bool ok = wait(kBarQ + h, 0);
+      auto scores = [&](int j) {
+        const int st = j % kStages;
+        ok = ok && wait(kBarK + st, (j / kStages) & 1);
+        if (!ok) return;
+        // the widened tiles reach the tensor cores through this thread's fence
+        fence_async_shared();
+        tc_fence_after();
+        const uint64_t dk = desc_k(base + kOffK + st * kTileBytes);
+        umma_bf16_x4(tS, dq, dk, 2, 2, kIdS, 0u);
+        umma_bf16_x4(tS, dq + (kHalf >> 4), dk + (kHalf >> 4), 2, 2, kIdS, 1u);
+        umma_commit(bar(kBarS + h));
+        umma_commit(bar(kBarKFree + st));
+      };
+      scores(0);
+#pragma unroll 1
+      for (int j = 0; j < tiles && ok; ++j) {
+        const int st = j % kStages;
+        ok = wait(kBarV + st, (j / kStages) & 1) && wait(kBarP + 2 * h, j & 1);
+        if (!ok) break;
+        fence_async_shared();
+        tc_fence_after();
+        const uint64_t dv = desc_mn(base + kOffV + st * kTileBytes, kHalf);
+        umma_bf16_ts_x4(tO, tS, dv, 8, (16 * 128) >> 4, kIdO, j > 0 ? 1u : 0u);
+        umma_commit(bar(kBarO + h));
+        ok = wait(kBarP + 2 * h + 1, j & 1);
+        if (!ok) break;
+        tc_fence_after();
+        umma_bf16_ts_x4(tO, tS + 32, dv + ((64 * 128) >> 4), 8, (16 * 128) >> 4, kIdO, 1u);
+        umma_commit(bar(kBarVFree + st));
+        if (j + 1 < tiles) scores(j + 1);
+      }
+      umma_commit(bar(kBarDone + h));
+      mbar_wait(bar(kBarDone + h), 0, abort_flag, a.err, true);
+    }
+    __syncwarp();
     }
   }
   tc_fence_before();
@@ -518,7 +669,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv8_extend_join_kernel(Extend
   wait_prior_grid();
   const Unit& u = s_unit;
   const int r = blockIdx.z * kJoinWarps + warp;
-  if (u.x.entry < 0 || r >= u.rows) return;
+  if (u.entry < 0 || r >= u.rows) return;
   const float* rec = a.part + ((int64_t)blockIdx.x * a.c.kv_heads + kvh) * g.splits * kRecord;
   float M = -INFINITY;
   for (int s = lane; s < g.splits; s += 32) M = fmaxf(M, rec[s * kRecord + 2 * r]);
@@ -535,9 +686,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv8_extend_join_kernel(Extend
     o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int64_t row = u.row0 + r, token = row / a.group;
-  const int head = kvh * a.group + (int)(row - token * a.group);
-  *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + (u.x.row0 + token) * a.out_stride +
+  const int token = (u.row0 + r) / a.group, head = kvh * a.group + u.row0 + r - token * a.group;
+  *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + (int64_t)(u.q_row + token) * a.out_stride +
                             (int64_t)head * kTcDim + lane * 4) =
       make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
 }
@@ -574,11 +724,14 @@ int run_extend_tc(const AttnArgs& a, int64_t max_keys, size_t ws_bytes, cudaStre
   if (g.splits > 1 &&
       (a.part == nullptr || ws_bytes < extend_tc_workspace(a.bs, a.c.kv_heads, a.group, a.tokens, max_keys)))
     return QQ_ERR_WORKSPACE;
-  static SmemLimit limit;
-  int rc = limit.ensure((const void*)kv8_extend_kernel, kDynSmem);
+  static SmemLimit limit16, limit64;
+  int rc = limit16.ensure((const void*)kv8_extend_kernel<16>, kDynSmem);
+  if (rc == QQ_OK) rc = limit64.ensure((const void*)kv8_extend_kernel<64>, kDynSmem);
   if (rc != QQ_OK) return rc;
   const unsigned tiles = (unsigned)unit_tiles(a.bs, a.group, a.tokens);
-  kv8_extend_kernel<<<dim3(a.c.kv_heads, tiles, g.splits), kThreads, kDynSmem, s>>>(g);
+  const dim3 grid(a.c.kv_heads, tiles, g.splits);
+  if (a.c.block >= 64) kv8_extend_kernel<64><<<grid, kThreads, kDynSmem, s>>>(g);
+  else kv8_extend_kernel<16><<<grid, kThreads, kDynSmem, s>>>(g);
   if ((rc = launch_status()) != QQ_OK || g.splits == 1) return rc;
   return launch_pdl(kv8_extend_join_kernel, dim3(tiles, a.c.kv_heads, kUnitRows / kJoinWarps), dim3(kJoinWarps * 32), 0, s, g);
 }
