@@ -53,8 +53,9 @@ static_assert(128 * (2 * kRegsSoft + kRegsWiden + kRegsRest) <= kThreads * 128, 
 constexpr int kOffQ = 0, kOffK = 2 * kTileBytes, kOffV = kOffK + kStages * kTileBytes;
 constexpr int kDynSmem = kOffV + kStages * kTileBytes + 1024;
 constexpr uint32_t kTmemCols = 512;
-constexpr float kRaiseAt = 256.f, kMost = 32768.f;
-constexpr int kPoly = 4;  // one pair in kPoly of the exponentials on the FMA pipe
+constexpr float kRaiseAt = 4096.f, kMost = 32768.f;
+constexpr int kLagHalf = -1;
+constexpr int kPoly = 0;  // one pair in kPoly of the exponentials on the FMA pipe
 
 enum : int {
   kBarQ = 0,                          // [2] queries of a tile written
@@ -68,7 +69,8 @@ enum : int {
   kBarP = kBarS + 2,                  // [2][2] weights of a tile's first and second 64 keys written
   kBarO = kBarP + 4,                  // [2] the product of a tile's first 64 keys made
   kBarDone = kBarO + 2,               // [2] the tile's last MMA has finished
-  kNumBars = kBarDone + 2
+  kBarLag = kBarDone + 2,             // [2] the first tile has come so far (key tiles in turn)
+  kNumBars = kBarLag + 2
 };
 
 struct ExtendArgs {
@@ -224,7 +226,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
   const Cache& c = a.c;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const smem = smem_raw + (base - smem_u32(smem_raw));
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the same in all lanes, and known to be
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
   volatile int* abort_flag = &s_abort;
   auto wait = [&](int i, uint32_t parity) { return mbar_wait(bar(i), parity, abort_flag, a.err); };
@@ -256,6 +259,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
       mbar_init(bar(kBarMeta + i), 1);
       mbar_init(bar(kBarMetaFree + i), 8);
     }
+    mbar_init(bar(kBarLag), 4);
+    mbar_init(bar(kBarLag + 1), 4);
     mbar_init_fence();
   }
   __syncthreads();
@@ -265,8 +270,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = s_tmem;
-  const int tiles = u.tiles;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
+  const int tiles = __shfl_sync(0xffffffffu, u.tiles, 0);
 
   if (warp < kWidenWarp) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoft));
@@ -382,6 +387,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
       }
       if (__any_sync(0xffffffffu, alpha != 1.f)) rescale();
       tmem_ld32(tS, v[0]);
+      if (h == 0 && kLagHalf < 0) mbar_arrive_warp(bar(kBarLag + (j & 1)));
 
       // P of chunk k (v[k & 1]) into pk, its sums into part and sum
       auto chunk = [&](int k, auto is_full) {
@@ -450,6 +456,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive_warp(bar(kBarP + 2 * h + hf));
+        if (h == 0 && hf == kLagHalf) mbar_arrive_warp(bar(kBarLag + (j & 1)));
         most = fmaxf(most, sum);
       };
       if (full) {
@@ -605,46 +612,48 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
     }
     } else if (warp < kScaleWarp) {
     // ================================================================ MMA issue, one warp per M tile
-    if (lane == 0 && tiles > 0) {
+    if (tiles > 0) {
       const int h = warp - kMmaWarp;
       const uint32_t tS = tmem + h * 256, tO = tS + 128;
       const uint64_t dq = desc_k(base + kOffQ + h * kTileBytes);
-      bool ok = wait(kBarQ + h, 0);
+      auto all = [&](int i, uint32_t parity) { return __all_sync(0xffffffffu, wait(i, parity)); };
+      bool ok = all(kBarQ + h, 0);
       auto scores = [&](int j) {
         const int st = j % kStages;
-        ok = ok && wait(kBarK + st, (j / kStages) & 1);
+        // The second tile stays behind the first, so that one's softmax meets the
+        // other's products (in step, both wait for the tensor cores together).
+        ok = ok && (h == 0 || all(kBarLag + (j & 1), (j >> 1) & 1)) && all(kBarK + st, (j / kStages) & 1);
         if (!ok) return;
         // the widened tiles reach the tensor cores through this thread's fence
         fence_async_shared();
         tc_fence_after();
         const uint64_t dk = desc_k(base + kOffK + st * kTileBytes);
-        umma_bf16_x4(tS, dq, dk, 2, 2, kIdS, 0u);
-        umma_bf16_x4(tS, dq + (kHalf >> 4), dk + (kHalf >> 4), 2, 2, kIdS, 1u);
-        umma_commit(bar(kBarS + h));
-        umma_commit(bar(kBarKFree + st));
+        umma_f16_x4_warp(tS, dq, dk, 2, 2, kIdS, 0u);
+        umma_f16_x4_warp(tS, dq + (kHalf >> 4), dk + (kHalf >> 4), 2, 2, kIdS, 1u);
+        umma_commit_warp(bar(kBarS + h));
+        umma_commit_warp(bar(kBarKFree + st));
       };
       scores(0);
 #pragma unroll 1
       for (int j = 0; j < tiles && ok; ++j) {
         const int st = j % kStages;
-        ok = wait(kBarV + st, (j / kStages) & 1) && wait(kBarP + 2 * h, j & 1);
+        ok = all(kBarV + st, (j / kStages) & 1) && all(kBarP + 2 * h, j & 1);
         if (!ok) break;
         fence_async_shared();
         tc_fence_after();
         const uint64_t dv = desc_mn(base + kOffV + st * kTileBytes, kHalf);
-        umma_bf16_ts_x4(tO, tS, dv, 8, (16 * 128) >> 4, kIdO, j > 0 ? 1u : 0u);
-        umma_commit(bar(kBarO + h));
-        ok = wait(kBarP + 2 * h + 1, j & 1);
+        umma_f16_ts_x4_warp(tO, tS, dv, 8, (16 * 128) >> 4, kIdO, j > 0 ? 1u : 0u);
+        umma_commit_warp(bar(kBarO + h));
+        ok = all(kBarP + 2 * h + 1, j & 1);
         if (!ok) break;
         tc_fence_after();
-        umma_bf16_ts_x4(tO, tS + 32, dv + ((64 * 128) >> 4), 8, (16 * 128) >> 4, kIdO, 1u);
-        umma_commit(bar(kBarVFree + st));
+        umma_f16_ts_x4_warp(tO, tS + 32, dv + ((64 * 128) >> 4), 8, (16 * 128) >> 4, kIdO, 1u);
+        umma_commit_warp(bar(kBarVFree + st));
         if (j + 1 < tiles) scores(j + 1);
       }
-      umma_commit(bar(kBarDone + h));
+      umma_commit_warp(bar(kBarDone + h));
       mbar_wait(bar(kBarDone + h), 0, abort_flag, a.err, true);
     }
-    __syncwarp();
     }
   }
   tc_fence_before();
