@@ -320,35 +320,48 @@ struct AppendArgs {
   uint32_t* err;
 };
 
-constexpr int kAppendWarps = 8;
 constexpr int kMaxWindow = 64;
+constexpr int kAppendThreads = 512, kAppendSmall = 256;
 
 // A run is a stretch of tokens whose slots ascend by one inside a block; its
-// first token's CTA quantises it, a warp per (K or V, head): one pass over
-// the run's values for the maximum, one (from L2) that stores the codes.
+// first token's CTA quantises it.  The warps divide the (K or V, head) pairs
+// of the run, several warps to a pair where there are fewer pairs; a lane
+// holds up to kHeld pieces of 8 elements in registers between the pass for
+// the maximum and the one that stores the codes, so the values are read once
+// and all at once (longer runs read them again, from L2).
 // Bound by the values' bytes for a prefill and by the chain slots -> values ->
 // maximum -> codes for a decode step.
 // Two runs of one call that meet in a block would race: a run claims its block
 // with the call's epoch, and the one that finds the epoch there is skipped and
 // reported.  The epoch lives in state[0] and the last CTA to leave advances
 // it, so a captured call gets a new one with every replay.
-template <typename T>
-__global__ void __launch_bounds__(kAppendWarps * 32) kv8_append_kernel(AppendArgs a) {
+template <typename T, int DIM>
+__global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(AppendArgs a) {
+  constexpr int kHeld = sizeof(T) == 2 ? 16 : 8;
+  constexpr int kWords = sizeof(T) == 2 ? 1 : 2;  // 16-byte loads per piece
   __shared__ int64_t s_slots[kMaxWindow + kMaxBlock + 1];
+  __shared__ float s_most[2][kAppendThreads / 32];
   __shared__ int s_conflict;
   const Cache& c = a.c;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
+  const int dim = DIM > 0 ? DIM : c.dim;
+  const int chunks = dim >> 3;  // 8-element pieces of a row
+  const int pairs = 2 * c.kv_heads;
+  int team = 1;  // warps per pair
+  while (team * 2 * pairs <= warps) team *= 2;
+  const int teams = warps / team, mine = warp / team, part = warp - mine * team;
+  const int step = team * 32;
   const int64_t w0 = (int64_t)blockIdx.x * a.window;
   const int64_t total = (int64_t)c.num_blocks << c.shift;
   // s_slots[i] is the slot of token w0 - 1 + i (-1 outside the batch)
-  for (int i = tid; i < a.window + c.block + 1; i += kAppendWarps * 32) {
+  for (int i = tid; i < a.window + c.block + 1; i += blockDim.x) {
     const int64_t t = w0 - 1 + i;
     s_slots[i] = t >= 0 && t < a.n ? a.slots[t] : -1;
   }
   const uint32_t epoch = ld_volatile_u32(c.state) + 1;
   __syncthreads();
-  const int chunks = c.dim >> 3;  // 8-element pieces of a row
   const int last = (int)min((int64_t)a.window, a.n - w0);
+  int turn = 0;
   for (int u = 0; u < last; ++u) {
     const int64_t slot = s_slots[u + 1], prev = s_slots[u];
     if (slot < 0) continue;  // a padding token
@@ -378,37 +391,84 @@ __global__ void __launch_bounds__(kAppendWarps * 32) kv8_append_kernel(AppendArg
       continue;
     }
     const int64_t t0 = w0 + u;
-    for (int p = warp; p < 2 * c.kv_heads; p += kAppendWarps) {
+    const int items = n * chunks;
+    const bool held = items <= step * kHeld;
+    for (int p0 = 0; p0 < pairs; p0 += teams, ++turn) {
+      const int p = p0 + mine;
+      const bool work = mine < teams && p < pairs;
       const bool is_v = p >= c.kv_heads;
       const int h = is_v ? p - c.kv_heads : p;
       const int64_t stride = is_v ? a.v_stride : a.k_stride;
-      const T* src = static_cast<const T*>(is_v ? a.v : a.k) + t0 * stride + (int64_t)h * c.dim;
+      const T* src = static_cast<const T*>(is_v ? a.v : a.k) + t0 * stride + (int64_t)h * dim;
       const int64_t bh = (int64_t)b * c.kv_heads + h;
-      uint8_t* codes = (is_v ? c.v : c.k) + bh * c.block * c.dim;
+      uint8_t* codes = (is_v ? c.v : c.k) + bh * c.block * dim;
       float* scale = (is_v ? c.v_scale : c.k_scale) + bh;
-      const float old = off == 0 ? 0.f : *scale;
-      const int items = n * chunks;
-      float most = 0.f;
-#pragma unroll 4
-      for (int i = lane; i < items; i += 32) {
+      float old = 0.f, most = 0.f;
+      uint4 raw[kHeld * kWords];
+      auto piece = [&](int i) {
         const int r = i / chunks;
-        float x[8];
-        load8(src + r * stride + (i - r * chunks) * 8, x);
+        return reinterpret_cast<const uint4*>(src + r * stride + (i - r * chunks) * 8);
+      };
+      auto unpack = [&](const uint4* w, float (&x)[8]) {
+        const uint32_t lo[4] = {w[0].x, w[0].y, w[0].z, w[0].w};
+        if (kWords == 1) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            x[2 * e] = __uint_as_float(lo[e] << 16), x[2 * e + 1] = __uint_as_float(lo[e] & 0xFFFF0000u);
+        } else {
+          const uint4& v = w[kWords - 1];
+          const uint32_t hi[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(lo[e]), x[4 + e] = __uint_as_float(hi[e]);
+        }
+      };
+      auto raise_most = [&](const float (&x)[8]) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float m = fabsf(x[e]);
           if (m <= 3.402823466e38f) most = fmaxf(most, m);  // infinities and NaN set no scale
         }
-      }
+      };
+      if (work) {
+        if (off != 0) old = *scale;
+        if (held) {
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+          for (int k = 0; k < kHeld; ++k) {
+            const int i = part * 32 + lane + k * step;
+#pragma unroll
+            for (int w = 0; w < kWords; ++w)
+              raw[k * kWords + w] = i < items ? __ldg(piece(i) + w) : make_uint4(0, 0, 0, 0);
+          }
+#pragma unroll
+          for (int k = 0; k < kHeld; ++k) {
+            float x[8];
+            unpack(raw + k * kWords, x);
+            raise_most(x);
+          }
+        } else {
+#pragma unroll 4
+          for (int i = part * 32 + lane; i < items; i += step) {
+            float x[8];
+            load8(reinterpret_cast<const T*>(piece(i)), x);
+            raise_most(x);
+          }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      }
+      if (team > 1) {  // uniform over the CTA
+        if (lane == 0) s_most[turn & 1][warp] = most;
+        __syncthreads();
+        for (int w = 0; w < team; ++w) most = fmaxf(most, s_most[turn & 1][mine * team + w]);
+      }
+      if (!work) continue;
       // most = 1.m * 2^E <= 1.75 * 2^8 * 2^k
       const uint32_t bits = __float_as_uint(most);
       const int e2 = max((int)(bits >> 23) - 127 - ((bits & 0x7FFFFFu) <= 0x600000u ? 8 : 7), -126);
       const float now = fmaxf(old, __uint_as_float((uint32_t)(e2 + 127) << 23));
       if (off != 0 && now != old) {  // the codes already here, in steps of the larger scale
         const float ratio = __fdiv_rn(old, now);
-        for (int i = lane; i < c.block * chunks; i += 32) {
+        for (int i = part * 32 + lane; i < c.block * chunks; i += step) {
           const int r = i / chunks;
           if (r >= off && r < off + n) continue;
           uint2* p8 = reinterpret_cast<uint2*>(codes + (int64_t)i * 8);
@@ -420,22 +480,36 @@ __global__ void __launch_bounds__(kAppendWarps * 32) kv8_append_kernel(AppendArg
                            e4m3x2(x[4], x[5]) | (e4m3x2(x[6], x[7]) << 16));
         }
       }
-      if (lane == 0) *scale = now;
       // dividing by a power of two is multiplying by its inverse; a scale the caller brought may be any number
       const uint32_t nb = __float_as_uint(now);
       const bool pow2 = (nb & 0x7FFFFFu) == 0 && nb != 0;
       const float inv = __fdiv_rn(1.f, now);
-      uint8_t* dst = codes + (int64_t)off * c.dim;
-#pragma unroll 4
-      for (int i = lane; i < items; i += 32) {
-        const int r = i / chunks;
-        float x[8];
-        load8(src + r * stride + (i - r * chunks) * 8, x);
+      uint8_t* dst = codes + (int64_t)off * dim;
+      auto put = [&](int i, float (&x)[8]) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = pow2 ? x[e] * inv : __fdiv_rn(x[e], now);
         *reinterpret_cast<uint2*>(dst + (int64_t)i * 8) = make_uint2(
             e4m3x2(x[0], x[1]) | (e4m3x2(x[2], x[3]) << 16), e4m3x2(x[4], x[5]) | (e4m3x2(x[6], x[7]) << 16));
+      };
+      if (held) {
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k) {
+          const int i = part * 32 + lane + k * step;
+          if (i >= items) break;
+          float x[8];
+          unpack(raw + k * kWords, x);
+          put(i, x);
+        }
+      } else {
+#pragma unroll 4
+        for (int i = part * 32 + lane; i < items; i += step) {
+          float x[8];
+          load8(reinterpret_cast<const T*>(piece(i)), x);
+          put(i, x);
+        }
       }
+      // every warp of the team had read the old scale before the maxima were exchanged
+      if (part == 0 && lane == 0) *scale = now;
     }
   }
   // the epoch advances once every CTA has read it
@@ -459,7 +533,7 @@ __global__ void __launch_bounds__(256) kv8_gather_kernel(Cache c, const int64_t*
   const int64_t total = (int64_t)c.num_blocks << c.shift;
   const int64_t items = n * row;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < items; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t t = i / row;
+    const int64_t t = items <= UINT32_MAX ? (uint32_t)i / (uint32_t)row : i / row;
     const int w = (int)(i - t * row);
     const int h = w / chunks, ch = w - h * chunks;
     const int64_t slot = slots[t];
@@ -590,15 +664,22 @@ extern "C" int qq_kv8_append(const qq_kv8_cache* cache, const void* k, const voi
   a.slots = slots;
   a.n = num_tokens;
   a.err = err;
-  // A CTA per token while there are few (each may be its own run); windows of
-  // more tokens for a prefill, whose runs are whole blocks.
-  a.window = 1;
-  while (a.window < kMaxWindow && num_tokens > 512 * (int64_t)a.window) a.window *= 2;
+  // A CTA per token while there are few (each may be its own run: windows of 8
+  // took 4096 of them one after the other); windows of a block's length for a
+  // longer prefill, whose runs are whole blocks.
+  a.window = num_tokens <= 4096 ? 1 : kMaxWindow;
   const int64_t ctas = (num_tokens + a.window - 1) / a.window;
   if (ctas > INT32_MAX) return QQ_ERR_UNSUPPORTED;
+  const int threads = num_tokens <= 512 ? kAppendSmall : kAppendThreads;
+  const bool d128 = cache->head_dim == 128;
   cudaStream_t s = as_stream(stream);
-  if (dtype == QQ_BF16) kv8_append_kernel<__nv_bfloat16><<<(unsigned)ctas, kAppendWarps * 32, 0, s>>>(a);
-  else kv8_append_kernel<float><<<(unsigned)ctas, kAppendWarps * 32, 0, s>>>(a);
+  if (dtype == QQ_BF16) {
+    if (d128) kv8_append_kernel<__nv_bfloat16, 128><<<(unsigned)ctas, threads, 0, s>>>(a);
+    else kv8_append_kernel<__nv_bfloat16, 0><<<(unsigned)ctas, threads, 0, s>>>(a);
+  } else {
+    if (d128) kv8_append_kernel<float, 128><<<(unsigned)ctas, threads, 0, s>>>(a);
+    else kv8_append_kernel<float, 0><<<(unsigned)ctas, threads, 0, s>>>(a);
+  }
   return launch_status();
 }
 

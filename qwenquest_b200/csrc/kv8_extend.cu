@@ -54,8 +54,6 @@ constexpr int kOffQ = 0, kOffK = 2 * kTileBytes, kOffV = kOffK + kStages * kTile
 constexpr int kDynSmem = kOffV + kStages * kTileBytes + 1024;
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRaiseAt = 4096.f, kMost = 32768.f;
-constexpr int kLagHalf = -1;
-constexpr int kPoly = 0;  // one pair in kPoly of the exponentials on the FMA pipe
 
 enum : int {
   kBarQ = 0,                          // [2] queries of a tile written
@@ -69,7 +67,7 @@ enum : int {
   kBarP = kBarS + 2,                  // [2][2] weights of a tile's first and second 64 keys written
   kBarO = kBarP + 4,                  // [2] the product of a tile's first 64 keys made
   kBarDone = kBarO + 2,               // [2] the tile's last MMA has finished
-  kBarLag = kBarDone + 2,             // [2] the first tile has come so far (key tiles in turn)
+  kBarLag = kBarDone + 2,             // [2] the first tile's softmax is at it (key tiles in turn)
   kNumBars = kBarLag + 2
 };
 
@@ -156,32 +154,6 @@ __device__ __forceinline__ f32x2 add2(f32x2 x, f32x2 y) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
   return r;
 }
-__device__ __forceinline__ f32x2 mul2(f32x2 x, f32x2 y) {
-  f32x2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
-  return r;
-}
-
-// 2^x of both on the FMA pipe, for x <= 9 (below -125: 2^-125; NaN stays NaN):
-// x = r + f with r = round(x) by the 1.5 * 2^23 shift, 2^f a polynomial of
-// degree 3 fitted here (relative error 7.5e-5, against fp16's 2^-11), 2^r from
-// r in the shifted number's low bits.
-__device__ __forceinline__ f32x2 exp2_fma(f32x2 x) {
-  float2 c = both_of(x);
-  asm("max.NaN.f32 %0, %0, 0fC2FA0000;" : "+f"(c.x));  // -125
-  asm("max.NaN.f32 %0, %0, 0fC2FA0000;" : "+f"(c.y));
-  x = pair(c.x, c.y);
-  const f32x2 t = add2(x, pair(12582912.f, 12582912.f));
-  const f32x2 r = add2(t, pair(-12582912.f, -12582912.f));
-  const f32x2 f = fma2(r, pair(-1.f, -1.f), x);
-  f32x2 p = fma2(pair(0.05517166f, 0.05517166f), f, pair(0.24261113f, 0.24261113f));
-  p = fma2(p, f, pair(0.69326097f, 0.69326097f));
-  p = fma2(p, f, pair(0.99992806f, 0.99992806f));
-  const float2 tt = both_of(t);
-  return mul2(p, pair(__uint_as_float(__float_as_uint(tt.x) * 0x800000u + 0x3F800000u),
-                      __uint_as_float(__float_as_uint(tt.y) * 0x800000u + 0x3F800000u)));
-}
-
 // The CTA's rows and keys (all within 32 bits: at most 65535 tiles of 256
 // rows, and positions of a table of less than 2^31 tokens).
 struct Unit {
@@ -387,7 +359,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
       }
       if (__any_sync(0xffffffffu, alpha != 1.f)) rescale();
       tmem_ld32(tS, v[0]);
-      if (h == 0 && kLagHalf < 0) mbar_arrive_warp(bar(kBarLag + (j & 1)));
+      if (h == 0) mbar_arrive_warp(bar(kBarLag + (j & 1)));
 
       // P of chunk k (v[k & 1]) into pk, its sums into part and sum
       auto chunk = [&](int k, auto is_full) {
@@ -402,20 +374,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
 #pragma unroll
           for (int e = 0; e < (kGroup < 32 ? kGroup : 32); e += 2) {
             const f32x2 y = fma2(pair(__uint_as_float(x[q + e]), __uint_as_float(x[q + e + 1])), mul_2, add_2);
-            f32x2 p;
-            if (kPoly > 0 && (e >> 1) % (kPoly > 0 ? kPoly : 1) == 1) {  // some on the FMA pipe: the exponentials' is as busy as the tensor cores
-              p = exp2_fma(y);
-            } else {
-              const float2 t = both_of(y);
-              p = pair(ex2(t.x), ex2(t.y));
-            }
-            float2 w = both_of(p);
+            const float2 t = both_of(y);
+            float2 w = make_float2(ex2(t.x), ex2(t.y));
             if (!is_full.value) {
               w.x = k * 32 + q + e <= lim ? w.x : 0.f;
               w.y = k * 32 + q + e + 1 <= lim ? w.y : 0.f;
-              p = pair(w.x, w.y);
             }
-            s[(e >> 1) & 1] = add2(s[(e >> 1) & 1], p);
+            s[(e >> 1) & 1] = add2(s[(e >> 1) & 1], pair(w.x, w.y));
             pk[(k & 1) * 16 + (q + e) / 2] = pack_f16(w.x, w.y);
           }
           const float2 s2 = both_of(add2(s[0], s[1]));
@@ -456,7 +421,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive_warp(bar(kBarP + 2 * h + hf));
-        if (h == 0 && hf == kLagHalf) mbar_arrive_warp(bar(kBarLag + (j & 1)));
         most = fmaxf(most, sum);
       };
       if (full) {
@@ -620,8 +584,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
       bool ok = all(kBarQ + h, 0);
       auto scores = [&](int j) {
         const int st = j % kStages;
-        // The second tile stays behind the first, so that one's softmax meets the
-        // other's products (in step, both wait for the tensor cores together).
+        // The second tile's scores wait for the first one's softmax, so that one's
+        // exponentials meet the other's products (in step, both wait for the
+        // tensor cores, then both for the exponentials: 627 us where this takes 571).
         ok = ok && (h == 0 || all(kBarLag + (j & 1), (j >> 1) & 1)) && all(kBarK + st, (j / kStages) & 1);
         if (!ok) return;
         // the widened tiles reach the tensor cores through this thread's fence
