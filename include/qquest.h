@@ -322,9 +322,10 @@ int qq_block_trim(const qq_block_tables* tables, const int64_t* req_pool_indices
  * scales [num_blocks][kv_heads]; a value is its code times the scale of its
  * block and head.  block_size 16, 32, 64 or 128, head_dim a multiple of 8 up
  * to 256, codes 16-byte aligned, num_blocks * kv_heads * block_size < 2^31.
- * state (device [2 + num_blocks], zero-filled once) is needed by
- * qq_kv8_append alone.  No reference counterpart: the reference keeps K and V
+ * state (device [QQ_KV8_STATE_WORDS + 2 * kv_heads * num_blocks], zero-filled
+ * once) is needed by qq_kv8_append alone.  No reference counterpart: the reference keeps K and V
  * in the model's dtype (MHATokenToKVPool, memory.py:79-120). */
+#define QQ_KV8_STATE_WORDS 34
 typedef struct qq_kv8_cache {
   uint8_t* k;
   uint8_t* v;

@@ -245,7 +245,8 @@ class KV8Cache(_OnDevice):
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.num_layers = len(k)
         self.num_blocks, self.kv_heads, self.block_size, self.head_dim = shape
-        self._state = torch.zeros((self.num_layers, 2 + self.num_blocks), dtype=torch.int32, device=self.device)
+        words = _lib.QQ_KV8_STATE_WORDS + 2 * self.kv_heads * self.num_blocks
+        self._state = torch.zeros((self.num_layers, words), dtype=torch.int32, device=self.device)
         self._layers = [
             _lib.QQKv8Cache(a.data_ptr(), b.data_ptr(), sa.data_ptr(), sb.data_ptr(), st.data_ptr(), self.num_blocks,
                             self.kv_heads, self.head_dim, self.block_size)
