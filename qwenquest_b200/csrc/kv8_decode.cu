@@ -189,7 +189,8 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const smem = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t off_q = g.slots * kSlotBytes, off_p = off_q + 2 * kColBytes;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the same in all lanes, and known to be
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
   volatile int* abort_flag = &s_abort;
   auto wait = [&](int i, uint32_t parity) { return mbar_wait(bar(i), parity, abort_flag, a.err); };
@@ -256,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
     if (warp == 5) tmem_dealloc(s_tmem, kTmemCols);
     return;
   }
-  const uint32_t tmem = s_tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
   const int count = (int)(shares.lo(blockIdx.x + 1) - lo);
   Walk<KEYS> w(a, s_start[0], s_start[1], s_start[2]);
   const int64_t pool_rows = (int64_t)c.num_blocks * c.kv_heads * c.block;
@@ -337,45 +338,43 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
       mbar_wait(bar(kBarFull + i % g.slots), (i / g.slots) & 1, abort_flag, a.err, true);
   } else if (warp == 5) {
     // ================================================================ MMA issue
-    if (lane == 0) {
-      constexpr uint32_t kIdS = instr_desc_e4m3(0, 0, kTile, NC), kIdO = instr_desc_e4m3(1, 0, kTcDim, NC);
-      bool ok = true;
-      int pair = 0;  // (entry, head) segments so far
-      bool first = true;
-      auto scores = [&](int i) {
-        const int s = (2 * i) % g.slots, qb = pair & 1;
-        ok = ok && (!first || wait(kBarQ + qb, (pair >> 1) & 1)) && wait(kBarFull + s, ((2 * i) / g.slots) & 1);
-        if (!ok) return;
-        tc_fence_after();
-        umma_e4m3_x4(tmem + (i & 1) * NC, desc_k(base + s * kSlotBytes), desc_k(base + off_q + qb * kColBytes), 2, 2,
-                     kIdS, 0u);
-        umma_commit(bar(kBarS + (i & 1)));
-        umma_commit(bar(kBarEmpty + s));
-        first = w.last();
-        if (first) {
-          umma_commit(bar(kBarQFree + qb));
-          ++pair;
-        }
-        w.next();
-      };
-      scores(0);
-      if (count > 1) scores(1);
-      for (int i = 0; i < count && ok; ++i) {
-        const int s = (2 * i + 1) % g.slots;
-        ok = wait(kBarFull + s, ((2 * i + 1) / g.slots) & 1) && wait(kBarP + (i & 1), (i >> 1) & 1);
-        if (!ok) break;
-        tc_fence_after();
-        umma_e4m3_x4(tmem + 2 * NC + (i & 1) * NC, desc_mn(base + s * kSlotBytes, kSlotBytes),
-                     desc_k(base + off_p + (i & 1) * kColBytes), 256, 2, kIdO, 0u);
-        umma_commit(bar(kBarO + (i & 1)));
-        umma_commit(bar(kBarEmpty + s));
-        if (i + 2 < count) scores(i + 2);
+    constexpr uint32_t kIdS = instr_desc_e4m3(0, 0, kTile, NC), kIdO = instr_desc_e4m3(1, 0, kTcDim, NC);
+    auto all = [&](int i, uint32_t parity) { return __all_sync(0xffffffffu, wait(i, parity)); };
+    bool ok = true;
+    int pair = 0;  // (entry, head) segments so far
+    bool first = true;
+    auto scores = [&](int i) {
+      const int s = (2 * i) % g.slots, qb = pair & 1;
+      ok = ok && (!first || all(kBarQ + qb, (pair >> 1) & 1)) && all(kBarFull + s, ((2 * i) / g.slots) & 1);
+      if (!ok) return;
+      tc_fence_after();
+      umma_e4m3_x4_warp(tmem + (i & 1) * NC, desc_k(base + s * kSlotBytes), desc_k(base + off_q + qb * kColBytes), 2, 2,
+                        kIdS, 0u);
+      umma_commit_warp(bar(kBarS + (i & 1)));
+      umma_commit_warp(bar(kBarEmpty + s));
+      first = w.last();
+      if (first) {
+        umma_commit_warp(bar(kBarQFree + qb));
+        ++pair;
       }
-      // the tensor memory is freed after the last MMA that was issued
-      umma_commit(bar(kBarDone));
-      mbar_wait(bar(kBarDone), 0, abort_flag, a.err, true);
+      w.next();
+    };
+    scores(0);
+    if (count > 1) scores(1);
+    for (int i = 0; i < count && ok; ++i) {
+      const int s = (2 * i + 1) % g.slots;
+      ok = all(kBarFull + s, ((2 * i + 1) / g.slots) & 1) && all(kBarP + (i & 1), (i >> 1) & 1);
+      if (!ok) break;
+      tc_fence_after();
+      umma_e4m3_x4_warp(tmem + 2 * NC + (i & 1) * NC, desc_mn(base + s * kSlotBytes, kSlotBytes),
+                        desc_k(base + off_p + (i & 1) * kColBytes), 256, 2, kIdO, 0u);
+      umma_commit_warp(bar(kBarO + (i & 1)));
+      umma_commit_warp(bar(kBarEmpty + s));
+      if (i + 2 < count) scores(i + 2);
     }
-    __syncwarp();
+    // the tensor memory is freed after the last MMA that was issued
+    umma_commit_warp(bar(kBarDone));
+    mbar_wait(bar(kBarDone), 0, abort_flag, a.err, true);
   } else if (warp == 6) {
     // ================================================================ queries
     int pair = 0;

@@ -94,25 +94,11 @@ __device__ __forceinline__ void umma_bf16_ts_x4(uint32_t d_tmem, uint32_t a_tmem
 __host__ __device__ constexpr uint32_t instr_desc_e4m3(uint32_t a_mn_major, uint32_t b_mn_major, uint32_t m, uint32_t n) {
   return (1u << 4) | (a_mn_major << 15) | (b_mn_major << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
-// Four e4m3 MMAs (32 elements of K each) into one accumulator; the descriptors
-// advance by a_step / b_step (in 16-byte units) per MMA, the first accumulates when acc != 0.
-__device__ __forceinline__ void umma_e4m3_x4(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t a_step,
-                                             uint32_t b_step, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p, t;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, %4, %4;\n\t"
-      "add.s64 a1, %1, %5;\n\tadd.s64 a2, a1, %5;\n\tadd.s64 a3, a2, %5;\n\t"
-      "add.s64 b1, %2, %6;\n\tadd.s64 b2, b1, %6;\n\tadd.s64 b3, b2, %6;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a1, b1, %3, t;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a2, b2, %3, t;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a3, b3, %3, t;\n\t}\n" ::"r"(d_tmem),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc), "l"((uint64_t)a_step), "l"((uint64_t)b_step)
-      : "memory");
-}
-// The same MMAs (kind::f16) issued by a converged warp: one elected lane issues,
-// all lanes compute the operands, so that they stay in uniform registers (a
-// single thread's operands are moved there one by one, about 50 cycles an MMA).
+// Four MMAs into one accumulator issued by a converged warp: one elected lane
+// issues, all lanes compute the operands, so that they stay in uniform
+// registers (a single thread's operands are moved there one by one, about 50
+// cycles an MMA).  The operands advance by a_step / b_step per MMA; the first
+// accumulates when acc != 0, the others always.
 __device__ __forceinline__ void umma_f16_x4_warp(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t a_step,
                                                  uint32_t b_step, uint32_t idesc, uint32_t acc) {
   asm volatile(
@@ -139,6 +125,21 @@ __device__ __forceinline__ void umma_f16_ts_x4_warp(uint32_t d_tmem, uint32_t a_
       "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, t;\n\t"
       "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, t;\n\t}\n" ::"r"(d_tmem),
       "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc), "r"(a_step), "l"((uint64_t)b_step)
+      : "memory");
+}
+// e4m3 operands, 32 elements of K per MMA.
+__device__ __forceinline__ void umma_e4m3_x4_warp(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t a_step,
+                                                  uint32_t b_step, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, t, e;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, %4, %4;\n\t"
+      "add.s64 a1, %1, %5;\n\tadd.s64 a2, a1, %5;\n\tadd.s64 a3, a2, %5;\n\t"
+      "add.s64 b1, %2, %6;\n\tadd.s64 b2, b1, %6;\n\tadd.s64 b3, b2, %6;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a1, b1, %3, t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a2, b2, %3, t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a3, b3, %3, t;\n\t}\n" ::"r"(d_tmem),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "l"((uint64_t)a_step), "l"((uint64_t)b_step)
       : "memory");
 }
 // elect.sync picks the same lane for a full warp every time, so the commit follows that lane's MMAs.
