@@ -65,6 +65,8 @@ __global__ void __launch_bounds__(kAnyThreads) kv8_attn_any_kernel(AnyArgs g) {
   int64_t row0 = e, tokens = 1, seen0;  // query rows row0 .., the first sees keys [0, seen0), each next one more
   if (KEYS == kExtend) {
     const ExtendEntry x = extend_tile(a, blockIdx.x, g.tile_tokens, 1, blockIdx.x == 0 ? err : nullptr);
+    if (blockIdx.x == 0 && extend_tiles(a, g.tile_tokens, 1, nullptr) > gridDim.x)
+      raise_error(err, QQ_DEV_ERR_BOUNDS);  // entries share query rows
     if (x.entry < 0) return;  // past the last tile
     e = x.entry;
     row0 = x.row0 + x.tile * g.tile_tokens;

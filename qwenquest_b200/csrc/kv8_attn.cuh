@@ -62,30 +62,40 @@ struct ExtendEntry {
   int64_t row0, n, prefix;
 };
 
-// Tile `x` of the batch's tiles of `rows` rows each, `per` rows to a new token; called by one whole warp, the same
-// in every lane.  A bad entry has no tiles and is reported.
+// Entry `e` of an extend batch: its new tokens (0: a padding or a bad entry, which is reported), its first query row
+// and the keys before it.
+__device__ __forceinline__ int64_t extend_entry(const AttnArgs& a, int e, int64_t& row0, int64_t& pre, uint32_t* err) {
+  if (e >= a.bs) return 0;
+  const int64_t seq = a.seq[e], req = a.reqs[e];
+  row0 = a.offsets[e];
+  pre = a.prefix[e];
+  if (seq == 0) return 0;
+  const int64_t n = seq - pre;
+  if (pre >= 0 && n >= 0 && row0 >= 0 && row0 <= a.tokens && n <= a.tokens - row0 && seq <= a.table_stride << a.c.shift &&
+      req >= 0 && req < a.table_rows)
+    return n;
+  raise_error(err, QQ_DEV_ERR_BOUNDS);
+  return 0;
+}
+
+// The batch's tiles of `rows` rows each, `per` rows to a new token; called by one whole warp.
+__device__ __forceinline__ int64_t extend_tiles(const AttnArgs& a, int rows, int per, uint32_t* err) {
+  int64_t sum = 0, row0, pre;
+#pragma unroll 2
+  for (int e = threadIdx.x & 31; e < a.bs; e += 32) sum += (extend_entry(a, e, row0, pre, err) * per + rows - 1) / rows;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum;
+}
+
+// Tile `x` of those; called by one whole warp, the same in every lane.
 __device__ __forceinline__ ExtendEntry extend_tile(const AttnArgs& a, int64_t x, int rows, int per, uint32_t* err) {
   ExtendEntry r{-1, 0, 0, 0, 0};
   const int lane = threadIdx.x & 31;
   int64_t before = 0;
   for (int e0 = 0; e0 < a.bs; e0 += 32) {
-    const int e = e0 + lane;
-    int64_t n = 0, row0 = 0, pre = 0;
-    if (e < a.bs) {
-      const int64_t seq = a.seq[e];
-      row0 = a.offsets[e];
-      pre = a.prefix[e];
-      if (seq != 0) {  // 0: a padding entry
-        const int64_t req = a.reqs[e];
-        n = seq - pre;
-        const bool good = pre >= 0 && n >= 0 && row0 >= 0 && row0 <= a.tokens && n <= a.tokens - row0 &&
-                          seq <= a.table_stride << a.c.shift && req >= 0 && req < a.table_rows;
-        if (!good) {
-          raise_error(err, QQ_DEV_ERR_BOUNDS);
-          n = 0;
-        }
-      }
-    }
+    int64_t row0 = 0, pre = 0;
+    const int64_t n = extend_entry(a, e0 + lane, row0, pre, err);
     const int64_t tiles = (n * per + rows - 1) / rows;
     int64_t incl = tiles;
 #pragma unroll

@@ -11,8 +11,8 @@
 // Rows: the new tokens of an entry times the query heads of one KV head,
 // token-major; a CTA takes 256 of them (two M tiles of 128) against key tiles
 // of 128, so short chunks fill the tiles with heads and every key tile
-// serves 256 rows.  With few CTAs the keys are cut into `splits` stretches
-// whose (M, l, O) records kv8_extend_join_kernel merges.
+// serves 256 rows.  Where the last units leave SMs idle their keys are cut into
+// stretches whose (M, l, O) records kv8_extend_join_kernel merges.
 // Scales: as in the one-token kernel a score is S ks / up, the weight into
 // the V product 2^(s + lg - M) with lg = log2(vs), and the sum takes that
 // times 2^-lg: constants of a group of 16 keys (no block is shorter).
@@ -24,6 +24,7 @@
 // The running maximum is raised only past a factor of 2^8; O is rescaled then.
 // Every wait is bounded; see the one-token kernel.
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -73,10 +74,12 @@ enum : int {
 
 struct ExtendArgs {
   AttnArgs a;
-  int splits;
+  int tiles;   // units of a KV head at most
+  int sms;
+  int most;    // stretches of a unit at most
 };
 
-// A split's record of a unit: (M, l) of 256 rows, then O [256][128].
+// A stretch's record of a unit: (M, l) of 256 rows, then O [256][128].
 constexpr int64_t kRecord = kUnitRows * (2 + (int64_t)kTcDim);
 
 // fp16 operands, fp32 accumulator.
@@ -119,6 +122,15 @@ __device__ __forceinline__ uint2 load8_or_zero(const void* p, bool there) {
       : "l"(p), "r"((int)there));
   return r;
 }
+__device__ __forceinline__ uint4 load16_or_zero(const void* p, bool there) {
+  uint4 r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\t"
+      "mov.u32 %3, 0;\n\t@p ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}\n"
+      : "=&r"(r.x), "=&r"(r.y), "=&r"(r.z), "=&r"(r.w)
+      : "l"(p), "r"((int)there));
+  return r;
+}
 __device__ __forceinline__ int32_t load_or(const int32_t* p, bool there, int32_t other) {
   int32_t r;
   asm volatile(
@@ -154,33 +166,63 @@ __device__ __forceinline__ f32x2 add2(f32x2 x, f32x2 y) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
   return r;
 }
-// The CTA's rows and keys (all within 32 bits: at most 65535 tiles of 256
+// The units of the batch, the ones with the most keys first: entries and their
+// tiles from the last to the first, KV heads innermost.  SMs take a unit each at
+// a time, so the last units, which would leave SMs idle, are cut into `splits`
+// stretches of the keys, each of at least four key tiles (188 units of 35 to 47
+// key tiles on 148 SMs: 148 + 40 x 3 CTAs in 151 us; all whole 182, all cut in
+// two 175).  A batch with fewer units than SMs is cut throughout.
+struct Units {
+  int tiles, whole, splits;
+};
+__device__ __forceinline__ Units units_of(const ExtendArgs& g, uint32_t* err) {
+  const int64_t tiles = extend_tiles(g.a, kUnitRows, g.a.group, err);
+  if (tiles > g.tiles) raise_error(err, QQ_DEV_ERR_BOUNDS);  // entries share query rows
+  Units x;
+  x.tiles = (int)min(tiles, (int64_t)g.tiles);
+  const int all = x.tiles * g.a.c.kv_heads, rest = all % g.sms;
+  x.splits = rest == 0 ? 1 : min(g.most, g.sms / rest);
+  x.whole = x.splits == 1 ? all : all - rest;
+  return x;
+}
+
+// A unit or a stretch of one (all within 32 bits: at most 65535 tiles of 256
 // rows, and positions of a table of less than 2^31 tokens).
 struct Unit {
   int entry;               // -1: none
+  int kvh;
   int q_row;               // the entry's first query row
   int prefix;
   int row0, rows;          // rows [row0, row0 + rows) of the entry's n * group
+  int splits;              // stretches of the unit, 1: this is all of it
   int key_begin, key_end;
   int tiles;
   const int32_t* table;    // the request's blocks
 };
-__device__ __forceinline__ Unit unit_of(const ExtendArgs& g, int64_t tile, int split, uint32_t* err) {
+// Unit `index`, its stretch `split`; called by one whole warp.
+__device__ __forceinline__ Unit unit_of(const ExtendArgs& g, const Units& all_units, int index, int split) {
   const AttnArgs& a = g.a;
   Unit u{};
-  const ExtendEntry x = extend_tile(a, tile, kUnitRows, a.group, err);
-  u.entry = x.entry;
+  u.entry = -1;
+  const int tile = index / a.c.kv_heads;
+  if (tile >= all_units.tiles) return u;
+  const ExtendEntry x = extend_tile(a, all_units.tiles - 1 - tile, kUnitRows, a.group, nullptr);
   if (x.entry < 0) return u;
+  u.kvh = index - tile * a.c.kv_heads;
   u.q_row = (int)x.row0;
   u.prefix = (int)x.prefix;
   u.row0 = (int)x.tile * kUnitRows;
   u.rows = min(kUnitRows, (int)x.n * a.group - u.row0);
   u.table = a.table + a.reqs[x.entry] * a.table_stride;
   const int keys = u.prefix + (u.row0 + u.rows - 1) / a.group + 1;  // what its last row sees
-  const int all = (keys + kN - 1) / kN, each = (all + g.splits - 1) / g.splits;
-  u.key_begin = min(all, split * each) * kN;
+  const int all = (keys + kN - 1) / kN;
+  const int cuts = index < all_units.whole ? 1 : min(all_units.splits, (all + 3) / 4), each = (all + cuts - 1) / cuts;
+  u.splits = (all + each - 1) / each;
+  if (split >= u.splits) return u;
+  u.entry = x.entry;
+  u.key_begin = split * each * kN;
   u.key_end = min(keys, u.key_begin + each * kN);
-  u.tiles = max(0, (u.key_end - u.key_begin + kN - 1) / kN);
+  u.tiles = (u.key_end - u.key_begin + kN - 1) / kN;
   return u;
 }
 
@@ -192,6 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   __shared__ Unit s_unit;
+  __shared__ int s_record;  // of a stretch
   __shared__ float s_up[kUnitRows];                                   // scale_log2 / up of each row
   __shared__ __align__(16) float4 s_scale[kMeta][kGroups];        // ks, lg, 2^-lg of 16 keys
   const AttnArgs& a = g.a;
@@ -203,13 +246,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
   volatile int* abort_flag = &s_abort;
   auto wait = [&](int i, uint32_t parity) { return mbar_wait(bar(i), parity, abort_flag, a.err); };
-  const int kvh = blockIdx.x;
-  // the last tiles of an entry see the most keys: they start first
-  const int64_t tile = gridDim.y - 1 - blockIdx.y;
 
   if (warp == 0) {
-    const Unit u = unit_of(g, tile, blockIdx.z, blockIdx.x == 0 && tile == 0 && blockIdx.z == 0 ? a.err : nullptr);
-    if (lane == 0) s_unit = u;
+    const Units units = units_of(g, blockIdx.x == 0 ? a.err : nullptr);
+    const int id = blockIdx.x, cut = max(0, id - units.whole);
+    const Unit u = unit_of(g, units, min(id, units.whole) + cut / units.splits, cut % units.splits);
+    if (lane == 0) s_unit = u, s_record = cut;
   }
   if (threadIdx.x == 32) {
     s_abort = 0;
@@ -237,7 +279,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
   }
   __syncthreads();
   const Unit& u = s_unit;
-  if (u.entry < 0) return;  // past the last tile, uniform
+  if (u.entry < 0) return;  // past the last unit, uniform
+  const int kvh = u.kvh;
   if (warp == kMmaWarp) tmem_alloc(smem_u32(&s_tmem), kTmemCols);
   tc_fence_before();
   __syncthreads();
@@ -250,26 +293,31 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
     // ================================================================ softmax (warps 0-7)
     const int h = warp >> 2, r = threadIdx.x;      // row of the CTA's 256
     const int token = (u.row0 + r) / a.group;
-    const int head = kvh * a.group + u.row0 + r - token * a.group;
-    // ---- this warp's 32 query rows to fp16: four lanes per row, 32 channels each
+    // ---- this warp's 32 query rows to fp16: four lanes per row, 32 channels each;
+    // the next eight rows are on their way meanwhile
+    uint4 ask[4];
+    auto query = [&](int r0) {
+      const int rr = warp * 32 + r0 + (lane >> 2);
+      const bool there = r0 < 32 && rr < u.rows;
+      const int t = (u.row0 + rr) / a.group, hd = kvh * a.group + u.row0 + rr - t * a.group;
+      const uint4* q = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) +
+                                                      (int64_t)(u.q_row + t) * a.q_stride + (int64_t)hd * kTcDim + (lane & 3) * 32);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) ask[k] = load16_or_zero(q + k, there);
+    };
+    query(0);
 #pragma unroll 1
     for (int r0 = 0; r0 < 32; r0 += 8) {
-      const int rr = warp * 32 + r0 + (lane >> 2), col = (lane & 3) * 32;
-      float x[32] = {};
-      if (rr < u.rows) {
-        const int t = (u.row0 + rr) / a.group;
-        const int hd = kvh * a.group + u.row0 + rr - t * a.group;
-        const uint4* q = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) +
-                                                        (int64_t)(u.q_row + t) * a.q_stride + (int64_t)hd * kTcDim + col);
+      const int rr = warp * 32 + r0 + (lane >> 2);
+      float x[32];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint4 w = q[k];
-          const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t v[4] = {ask[k].x, ask[k].y, ask[k].z, ask[k].w};
 #pragma unroll
-          for (int b = 0; b < 4; ++b)
-            x[8 * k + 2 * b] = __uint_as_float(v[b] << 16), x[8 * k + 2 * b + 1] = __uint_as_float(v[b] & 0xFFFF0000u);
-        }
+        for (int b = 0; b < 4; ++b)
+          x[8 * k + 2 * b] = __uint_as_float(v[b] << 16), x[8 * k + 2 * b + 1] = __uint_as_float(v[b] & 0xFFFF0000u);
       }
+      query(r0 + 8);
       float most = 0.f;
 #pragma unroll
       for (int k = 0; k < 32; ++k) {
@@ -438,39 +486,58 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
       }
       mbar_arrive_warp(bar(kBarMetaFree + meta));
     }
-    // ---- O / l, or this stretch's record
+    // ---- O / l, or this stretch's record.  The rows go through this warp's part
+    // of Q's memory (the products are done with it), so that 16 lanes write a
+    // row's 256 bytes together.
     ok = __all_sync(0xffffffffu, ok && (tiles == 0 || wait(kBarDone + h, 0)));
     tc_fence_after();
-    const bool valid = ok && r < u.rows;
-    const float inv = l == 0.f ? 0.f : alpha / l;
-    float* rec = a.part + (((int64_t)tile * c.kv_heads + kvh) * g.splits + blockIdx.z) * kRecord;
-    if (g.splits > 1 && valid) rec[2 * r] = m, rec[2 * r + 1] = l;
-    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + (int64_t)(u.q_row + token) * a.out_stride + (int64_t)head * kTcDim;
+    const bool record = u.splits > 1;
+    const float f = record ? alpha : (l == 0.f ? 0.f : alpha / l);
+    float* rec = a.part + (int64_t)s_record * kRecord;
+    if (record && ok && r < u.rows) rec[2 * r] = m, rec[2 * r + 1] = l;
+    const int rows = ok ? u.rows : 0;
+    uint8_t* const stage = smem + kOffQ + warp * (kTileBytes / 4);  // 32 rows of 256 bytes, 16-byte pieces swizzled by the row
 #pragma unroll 1
-    for (int k = 0; k < kTcDim / 32; ++k) {
-      uint32_t o[32] = {};
-      if (tiles > 0 && ok) {
-        tmem_ld32(tO + k * 32, o);
-        tmem_ld_wait();
-      }
-      if (!valid) continue;
-      if (g.splits > 1) {
-        float4* w = reinterpret_cast<float4*>(rec + 2 * kUnitRows + (int64_t)r * kTcDim + k * 32);
+    for (int part = 0; part < 2; ++part) {  // 64 channels: a row of the record's half, or half a row of bf16
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          w[e] = make_float4(__uint_as_float(o[4 * e]) * alpha, __uint_as_float(o[4 * e + 1]) * alpha,
-                             __uint_as_float(o[4 * e + 2]) * alpha, __uint_as_float(o[4 * e + 3]) * alpha);
-      } else {
+      for (int k = 0; k < 2; ++k) {
+        uint32_t o[32] = {};
+        if (tiles > 0 && ok) {
+          tmem_ld32(tO + part * 64 + k * 32, o);
+          tmem_wait_ld32(o);
+        }
+        if (record) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint4 w;
-          w.x = pack_bf16(__uint_as_float(o[8 * e + 0]) * inv, __uint_as_float(o[8 * e + 1]) * inv);
-          w.y = pack_bf16(__uint_as_float(o[8 * e + 2]) * inv, __uint_as_float(o[8 * e + 3]) * inv);
-          w.z = pack_bf16(__uint_as_float(o[8 * e + 4]) * inv, __uint_as_float(o[8 * e + 5]) * inv);
-          w.w = pack_bf16(__uint_as_float(o[8 * e + 6]) * inv, __uint_as_float(o[8 * e + 7]) * inv);
-          *reinterpret_cast<uint4*>(dst + k * 32 + e * 8) = w;
+          for (int e = 0; e < 8; ++e)
+            *reinterpret_cast<float4*>(stage + lane * 256 + (((k * 8 + e) ^ (lane & 15)) << 4)) =
+                make_float4(__uint_as_float(o[4 * e]) * f, __uint_as_float(o[4 * e + 1]) * f,
+                            __uint_as_float(o[4 * e + 2]) * f, __uint_as_float(o[4 * e + 3]) * f);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            *reinterpret_cast<uint4*>(stage + lane * 256 + (((part * 8 + k * 4 + e) ^ (lane & 15)) << 4)) =
+                make_uint4(pack_bf16(__uint_as_float(o[8 * e + 0]) * f, __uint_as_float(o[8 * e + 1]) * f),
+                           pack_bf16(__uint_as_float(o[8 * e + 2]) * f, __uint_as_float(o[8 * e + 3]) * f),
+                           pack_bf16(__uint_as_float(o[8 * e + 4]) * f, __uint_as_float(o[8 * e + 5]) * f),
+                           pack_bf16(__uint_as_float(o[8 * e + 6]) * f, __uint_as_float(o[8 * e + 7]) * f));
         }
       }
+      if (!record && part == 0) continue;
+      __syncwarp();
+#pragma unroll 4
+      for (int k = 0; k < 16; ++k) {  // two rows at a time
+        const int row = 2 * k + (lane >> 4), rr = warp * 32 + row;
+        if (rr >= rows) break;
+        const uint4 w = *reinterpret_cast<const uint4*>(stage + row * 256 + (((lane & 15) ^ (row & 15)) << 4));
+        if (record) {
+          *reinterpret_cast<uint4*>(rec + 2 * kUnitRows + (int64_t)rr * kTcDim + part * 64 + (lane & 15) * 4) = w;
+        } else {
+          const int t = (u.row0 + rr) / a.group, hd = kvh * a.group + u.row0 + rr - t * a.group;
+          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + (int64_t)(u.q_row + t) * a.out_stride +
+                                    (int64_t)hd * kTcDim + (lane & 15) * 8) = w;
+        }
+      }
+      __syncwarp();
     }
   } else if (warp < kMmaWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsWiden));
@@ -629,85 +696,94 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
   }
 }
 
-// Merges the records of a unit's stretches: a warp per query row, four channels per lane.
+// Merges the records of the units that were cut: a warp per query row, four
+// channels per lane.  Launched always (how many units there are is known on the
+// device alone), and done at once where none was cut.
 constexpr int kJoinWarps = 8;
 __global__ void __launch_bounds__(kJoinWarps * 32) kv8_extend_join_kernel(ExtendArgs g) {
   __shared__ Unit s_unit;
+  __shared__ int s_record;
   const AttnArgs& a = g.a;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = blockIdx.y;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 0) {
-    const Unit u = unit_of(g, blockIdx.x, 0, nullptr);
-    if (lane == 0) s_unit = u;
+    const Units units = units_of(g, nullptr);
+    Unit u{};
+    u.entry = -1;
+    if (units.splits > 1) u = unit_of(g, units, units.whole + blockIdx.x, 0);
+    if (lane == 0) s_unit = u, s_record = blockIdx.x * units.splits;
   }
   __syncthreads();
   wait_prior_grid();
   const Unit& u = s_unit;
-  const int r = blockIdx.z * kJoinWarps + warp;
-  if (u.entry < 0 || r >= u.rows) return;
-  const float* rec = a.part + ((int64_t)blockIdx.x * a.c.kv_heads + kvh) * g.splits * kRecord;
-  float M = -INFINITY;
-  for (int s = lane; s < g.splits; s += 32) M = fmaxf(M, rec[s * kRecord + 2 * r]);
-  M = warp_max(M);
-  const float ref = M == -INFINITY ? 0.f : M;
-  float l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (u.entry < 0 || u.splits == 1) return;
+  const int splits = u.splits;
+  for (int r = blockIdx.y * kJoinWarps + warp; r < u.rows; r += gridDim.y * kJoinWarps) {
+    const float* rec = a.part + (int64_t)s_record * kRecord;
+    float M = -INFINITY;
+    for (int s = lane; s < splits; s += 32) M = fmaxf(M, rec[s * kRecord + 2 * r]);
+    M = warp_max(M);
+    const float ref = M == -INFINITY ? 0.f : M;
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (int s = 0; s < g.splits; ++s) {
-    const float* p = rec + s * kRecord;
-    const float f = ex2(p[2 * r] - ref);
-    const float4 v = *reinterpret_cast<const float4*>(p + 2 * kUnitRows + (int64_t)r * kTcDim + lane * 4);
-    l = fmaf(f, p[2 * r + 1], l);
-    o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+    for (int s = 0; s < splits; ++s) {
+      const float* p = rec + s * kRecord;
+      const float f = ex2(p[2 * r] - ref);
+      const float4 v = *reinterpret_cast<const float4*>(p + 2 * kUnitRows + (int64_t)r * kTcDim + lane * 4);
+      l = fmaf(f, p[2 * r + 1], l);
+      o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int token = (u.row0 + r) / a.group, head = u.kvh * a.group + u.row0 + r - token * a.group;
+    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + (int64_t)(u.q_row + token) * a.out_stride +
+                              (int64_t)head * kTcDim + lane * 4) =
+        make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int token = (u.row0 + r) / a.group, head = kvh * a.group + u.row0 + r - token * a.group;
-  *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + (int64_t)(u.q_row + token) * a.out_stride +
-                            (int64_t)head * kTcDim + lane * 4) =
-      make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
 }
 
+// Tiles of a KV head at most: a ragged end per entry.
 int64_t unit_tiles(int bs, int group, int64_t tokens) { return (tokens * group + kUnitRows - 1) / kUnitRows + bs; }
 
-// Stretches of the keys: one CTA per SM at a time, no stretch below four key tiles.
-int extend_splits(int bs, int kv_heads, int group, int64_t tokens, int64_t max_keys) {
-  // about as many units as there are full tiles (the bound counts a ragged end per entry)
-  const int64_t units = unit_tiles(bs, group, tokens) * kv_heads;
-  int64_t s = device_sm_count() / units;
-  const int64_t most = (max_keys + 4 * kN - 1) / (4 * kN);
-  if (s > most) s = most;
-  return (int)(s < 1 ? 1 : s);
+// Stretches of a unit at most: none below four key tiles.
+int64_t most_splits(int64_t max_keys) {
+  return std::min<int64_t>(device_sm_count(), std::max<int64_t>(1, (max_keys + 4 * kN - 1) / (4 * kN)));
 }
 
 }  // namespace
 
 bool extend_tc_fits(const AttnArgs& a, int dtype) {
-  return dtype == QQ_BF16 && a.c.dim == kTcDim && a.c.kv_heads <= 65535 && (a.q_stride * 2) % 16 == 0 &&
-         reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && (a.out_stride * 2) % 16 == 0 &&
-         reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && unit_tiles(a.bs, a.group, a.tokens) <= 65535;
+  const int64_t tiles = unit_tiles(a.bs, a.group, a.tokens);
+  return dtype == QQ_BF16 && a.c.dim == kTcDim && (a.q_stride * 2) % 16 == 0 && reinterpret_cast<uintptr_t>(a.q) % 16 == 0 &&
+         (a.out_stride * 2) % 16 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && tiles <= 65535 &&
+         tiles * a.c.kv_heads <= INT_MAX / 2;
 }
 
+// The stretches' records: at most one per SM.
 size_t extend_tc_workspace(int bs, int kv_heads, int group, int64_t tokens, int64_t max_keys) {
-  const int s = extend_splits(bs, kv_heads, group, tokens, max_keys);
-  return s <= 1 ? 0 : sizeof(float) * (size_t)(unit_tiles(bs, group, tokens) * kv_heads * s * kRecord);
+  const int64_t most = most_splits(max_keys), units = unit_tiles(bs, group, tokens) * kv_heads;
+  return most == 1 ? 0 : sizeof(float) * (size_t)(std::min<int64_t>(device_sm_count(), units * most) * kRecord);
 }
 
 int run_extend_tc(const AttnArgs& a, int64_t max_keys, size_t ws_bytes, cudaStream_t s) {
   ExtendArgs g{};
   g.a = a;
-  g.splits = extend_splits(a.bs, a.c.kv_heads, a.group, a.tokens, max_keys);
-  if (g.splits > 1 &&
-      (a.part == nullptr || ws_bytes < extend_tc_workspace(a.bs, a.c.kv_heads, a.group, a.tokens, max_keys)))
+  g.tiles = (int)unit_tiles(a.bs, a.group, a.tokens);
+  g.sms = device_sm_count();
+  g.most = (int)most_splits(max_keys);
+  if (g.most > 1 && (a.part == nullptr || ws_bytes < extend_tc_workspace(a.bs, a.c.kv_heads, a.group, a.tokens, max_keys)))
     return QQ_ERR_WORKSPACE;
   static SmemLimit limit16, limit64;
   int rc = limit16.ensure((const void*)kv8_extend_kernel<16>, kDynSmem);
   if (rc == QQ_OK) rc = limit64.ensure((const void*)kv8_extend_kernel<64>, kDynSmem);
   if (rc != QQ_OK) return rc;
-  const unsigned tiles = (unsigned)unit_tiles(a.bs, a.group, a.tokens);
-  const dim3 grid(a.c.kv_heads, tiles, g.splits);
+  const int units = g.tiles * a.c.kv_heads;
+  const unsigned grid = (unsigned)(units + (g.most > 1 ? g.sms : 0));
   if (a.c.block >= 64) kv8_extend_kernel<64><<<grid, kThreads, kDynSmem, s>>>(g);
   else kv8_extend_kernel<16><<<grid, kThreads, kDynSmem, s>>>(g);
-  if ((rc = launch_status()) != QQ_OK || g.splits == 1) return rc;
-  return launch_pdl(kv8_extend_join_kernel, dim3(tiles, a.c.kv_heads, kUnitRows / kJoinWarps), dim3(kJoinWarps * 32), 0, s, g);
+  if ((rc = launch_status()) != QQ_OK || g.most == 1) return rc;
+  // as many CTAs to a unit as there may be room for
+  const int cut = std::min(units, g.sms - 1), y = std::max(4, std::min(kUnitRows / kJoinWarps, 8 * g.sms / std::max(1, cut)));
+  return launch_pdl(kv8_extend_join_kernel, dim3(std::max(1, cut), y), dim3(kJoinWarps * 32), 0, s, g);
 }
 
 }  // namespace kv8
