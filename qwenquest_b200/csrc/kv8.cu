@@ -143,6 +143,8 @@ __global__ void __launch_bounds__(kTableThreads) block_plan_kernel(TableArgs a) 
   const int tid = threadIdx.x;
   const int block = 1 << a.shift;
   if (tid == 0) s_taken = 0;
+  wait_prior_grid();
+  allow_next_grid();
   claim_requests(a);
   const int64_t head = a.ring[0], free_count = a.ring[1] - head;
 
@@ -251,6 +253,8 @@ __global__ void __launch_bounds__(kTableThreads) block_trim_kernel(TableArgs a) 
   const TableSmem s = table_smem(smem_raw, a.bs);
   const int tid = threadIdx.x;
   const int block = 1 << a.shift;
+  wait_prior_grid();
+  allow_next_grid();
   claim_requests(a);
   const int64_t tail = a.ring[1], room = a.capacity - (tail - a.ring[0]);
   int32_t back[kTablePer], my_back = 0;
@@ -355,6 +359,8 @@ __global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 2 ? 8 : 4) kv8_ap
   const int64_t stride = is_v ? a.v_stride : a.k_stride;
   const int64_t w0 = (int64_t)blockIdx.x * a.window;
   const int64_t total = (int64_t)c.num_blocks << c.shift;
+  wait_prior_grid();
+  allow_next_grid();
   const uint32_t epoch = ld_volatile_u32(c.state + kEpoch) + 1;
   // s_slots[i] is the slot of token w0 - 1 + i (-1 outside the batch)
   for (int i = tid; i < a.window + c.block + 1; i += kAppendThreads) {
@@ -549,6 +555,8 @@ __global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 2 ? 8 : 4) kv8_ap
 template <typename T>
 __global__ void __launch_bounds__(256) kv8_gather_kernel(Cache c, const int64_t* slots, int64_t n, T* k_out, T* v_out,
                                                          uint32_t* err) {
+  wait_prior_grid();
+  allow_next_grid();
   const int chunks = c.dim >> 3, row = c.kv_heads * chunks;
   const int64_t total = (int64_t)c.num_blocks << c.shift;
   const int64_t items = n * row;
@@ -580,8 +588,7 @@ int launch_gather(const Cache& c, const int64_t* slots, int64_t n, void* k_out, 
   const int64_t items = n * c.kv_heads * (c.dim / 8);
   const int64_t most = (int64_t)device_sm_count() * 32;
   const unsigned ctas = (unsigned)((items + 255) / 256 < most ? (items + 255) / 256 : most);
-  kv8_gather_kernel<T><<<ctas, 256, 0, s>>>(c, slots, n, static_cast<T*>(k_out), static_cast<T*>(v_out), err);
-  return launch_status();
+  return launch_pdl(kv8_gather_kernel<T>, dim3(ctas), dim3(256), 0, s, c, slots, n, static_cast<T*>(k_out), static_cast<T*>(v_out), err);
 }
 
 int check_tables(const qq_block_tables* t, int bs, const int64_t* reqs) {
@@ -644,18 +651,16 @@ extern "C" int qq_block_plan(const qq_block_tables* tables, const int64_t* req_p
   cudaStream_t s = as_stream(stream);
   if (num_slots <= kOneCtaSlots) {
     if ((rc = one.ensure((const void*)block_plan_kernel<true, true>, smem)) != QQ_OK) return rc;
-    block_plan_kernel<true, true><<<1, kTableThreads, smem, s>>>(a);
-    return launch_status();
+    return launch_pdl(block_plan_kernel<true, true>, dim3(1), dim3(kTableThreads), smem, s, a);
   }
   if ((rc = wide.ensure((const void*)block_plan_kernel<false, true>, smem)) != QQ_OK) return rc;
   if ((rc = state.ensure((const void*)block_plan_kernel<true, false>, smem)) != QQ_OK) return rc;
   const int64_t ctas = (num_slots + kTableThreads - 1) / kTableThreads;
   const int most = device_sm_count();
-  block_plan_kernel<false, true><<<(unsigned)(ctas < most ? ctas : most), kTableThreads, smem, s>>>(a);
-  if ((rc = launch_status()) != QQ_OK) return rc;
+  rc = launch_pdl(block_plan_kernel<false, true>, dim3((unsigned)(ctas < most ? ctas : most)), dim3(kTableThreads), smem, s, a);
+  if (rc != QQ_OK) return rc;
   a.err = nullptr;  // what is wrong has been reported
-  block_plan_kernel<true, false><<<1, kTableThreads, smem, s>>>(a);
-  return launch_status();
+  return launch_pdl(block_plan_kernel<true, false>, dim3(1), dim3(kTableThreads), smem, s, a);
 }
 
 extern "C" int qq_block_trim(const qq_block_tables* tables, const int64_t* req_pool_indices, const int64_t* keep_lens,
@@ -668,8 +673,7 @@ extern "C" int qq_block_trim(const qq_block_tables* tables, const int64_t* req_p
   static SmemLimit limit;
   const size_t smem = table_smem_bytes(bs);
   if ((rc = limit.ensure((const void*)block_trim_kernel, smem)) != QQ_OK) return rc;
-  block_trim_kernel<<<1, kTableThreads, smem, as_stream(stream)>>>(a);
-  return launch_status();
+  return launch_pdl(block_trim_kernel, dim3(1), dim3(kTableThreads), smem, as_stream(stream), a);
 }
 
 extern "C" int qq_kv8_append(const qq_kv8_cache* cache, const void* k, const void* v, int dtype, int64_t k_stride,
@@ -704,14 +708,11 @@ extern "C" int qq_kv8_append(const qq_kv8_cache* cache, const void* k, const voi
   const dim3 grid((unsigned)ctas, pairs);
   const bool d128 = cache->head_dim == 128;
   cudaStream_t s = as_stream(stream);
-  if (dtype == QQ_BF16) {
-    if (d128) kv8_append_kernel<__nv_bfloat16, 128><<<grid, kAppendThreads, 0, s>>>(a);
-    else kv8_append_kernel<__nv_bfloat16, 0><<<grid, kAppendThreads, 0, s>>>(a);
-  } else {
-    if (d128) kv8_append_kernel<float, 128><<<grid, kAppendThreads, 0, s>>>(a);
-    else kv8_append_kernel<float, 0><<<grid, kAppendThreads, 0, s>>>(a);
-  }
-  return launch_status();
+  if (dtype == QQ_BF16)
+    return d128 ? launch_pdl(kv8_append_kernel<__nv_bfloat16, 128>, dim3(grid), dim3(kAppendThreads), 0, s, a)
+                : launch_pdl(kv8_append_kernel<__nv_bfloat16, 0>, dim3(grid), dim3(kAppendThreads), 0, s, a);
+  return d128 ? launch_pdl(kv8_append_kernel<float, 128>, dim3(grid), dim3(kAppendThreads), 0, s, a)
+              : launch_pdl(kv8_append_kernel<float, 0>, dim3(grid), dim3(kAppendThreads), 0, s, a);
 }
 
 extern "C" int qq_kv8_gather(const qq_kv8_cache* cache, const int64_t* slots, int64_t num_tokens, void* k_out,

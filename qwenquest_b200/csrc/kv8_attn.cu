@@ -4,12 +4,16 @@
 //
 //   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^(scale_log2 q.k_j - m)
 //
-// One CTA takes up to 16 query rows that share a KV head (the heads of a
-// group, and for an extend batch several new tokens) and one of `splits`
-// equal stretches of their keys; tiles of 64 keys are dequantised to fp32 in
-// shared memory once for all rows.  The maximum m and the sum run along with
-// the tiles; split stretches leave (m, sum, O) records that a second kernel
-// joins.  Bound by the fp32 FMAs and their shared-memory operands.
+// One CTA takes up to 4, 8 or 16 query rows that share a KV head (the heads of a
+// group, and for an extend batch several new tokens: 16 rows) and one of
+// `splits` equal stretches of their keys; tiles of 64 keys are dequantised to
+// fp32 in shared memory once for all rows.  The maximum m and the sum run along
+// with the tiles; split stretches leave (m, sum, O) records that a second
+// kernel joins.  One token per request is bound by the chain of a tile (table,
+// codes, scores, weights, product), so stretches go down to a tile and K and V
+// are asked for together (5 x up to 2500 keys of 2 heads of 64 for 8 query
+// heads: XX us; 53 with 16 rows always, one tile in hand and stretches of four).
+// An extend batch is bound by the fp32 FMAs and their shared-memory operands.
 
 #include <climits>
 #include <cmath>
@@ -24,37 +28,56 @@ namespace {
 
 using namespace kv8;
 
-constexpr int kRowsPerCta = 16;
+constexpr int kMostRows = 16;
 constexpr int kTileKeys = 64;
 constexpr int kAnyThreads = 128;
+constexpr int kMostSplits = 256;
 
 struct AnyArgs {
   AttnArgs a;
+  int rows;         // query rows per CTA at most: 4, 8 or 16
   int head_chunk;   // query heads per CTA
   int chunks;       // CTAs per KV head along its group
   int tile_tokens;  // query tokens per CTA
+  int key_groups;   // the product's threads: key groups x channels
   int splits;
 };
 
-// Records of a unit (row tile, KV head, head chunk) and split: 16 x (m, l), then 16 x dim.
-__host__ __device__ inline int64_t any_record(int dim) { return kRowsPerCta * (2 + (int64_t)dim); }
+// Records of a unit (row tile, KV head, head chunk) and split: rows x (m, l), then rows x dim.
+__host__ __device__ inline int64_t any_record(int rows, int dim) { return rows * (2 + (int64_t)dim); }
 
-inline size_t any_smem(int dim) {
-  return sizeof(float) * (kRowsPerCta * dim + kTileKeys * (dim + 4) + kRowsPerCta * kTileKeys);
+// K and V of a tile at once, but for 16 rows, whose CTAs would no longer be four to an SM.
+__host__ __device__ constexpr bool any_both(int rows) { return rows < 16; }
+inline int any_tile_floats(int rows, int dim, int key_groups) {
+  const int tile = kTileKeys * (dim + 4) * (any_both(rows) ? 2 : 1), sums = key_groups * rows * dim;
+  return tile > sums ? tile : sums;
+}
+inline size_t any_smem(const AnyArgs& g) {
+  const int dim = g.a.c.dim;
+  return sizeof(float) * (g.rows * dim + any_tile_floats(g.rows, dim, g.key_groups) + g.rows * kTileKeys);
 }
 
-template <typename T, int KEYS>
+// The keys of a stretch when `tiles` tiles are cut into at most `splits`.
+__device__ __forceinline__ int64_t stretch_keys(int64_t keys, int splits) {
+  return ((keys + kTileKeys - 1) / kTileKeys + splits - 1) / splits * kTileKeys;
+}
+
+template <typename T, int KEYS, int ROWS>
 __global__ void __launch_bounds__(kAnyThreads) kv8_attn_any_kernel(AnyArgs g) {
+  constexpr bool kBoth = any_both(ROWS);
   extern __shared__ __align__(16) float s_buf[];
-  __shared__ float s_m[kRowsPerCta], s_l[kRowsPerCta], s_corr[kRowsPerCta];
+  __shared__ float s_m[ROWS], s_l[ROWS], s_corr[ROWS];
   __shared__ int64_t s_slot[kTileKeys];
   __shared__ float s_ks[kTileKeys], s_vs[kTileKeys];
   const AttnArgs& a = g.a;
   const Cache& c = a.c;
   const int dim = c.dim, pitch = dim + 4, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  float* s_q = s_buf;                      // [16][dim], times scale_log2
-  float* s_kv = s_q + kRowsPerCta * dim;   // [64][pitch]
-  float* s_p = s_kv + kTileKeys * pitch;   // [16][64]
+  float* s_q = s_buf;                      // [ROWS][dim], times scale_log2
+  float* s_p = s_q + ROWS * dim;           // [ROWS][64]
+  float* s_k = s_p + ROWS * kTileKeys;     // [64][pitch]
+  float* s_v = kBoth ? s_k + kTileKeys * pitch : s_k;
+  wait_prior_grid();
+  allow_next_grid();
 
   const int kvh = blockIdx.y / g.chunks, chunk = blockIdx.y - kvh * g.chunks;
   const int h0 = kvh * a.group + chunk * g.head_chunk;
@@ -78,89 +101,113 @@ __global__ void __launch_bounds__(kAnyThreads) kv8_attn_any_kernel(AnyArgs g) {
   const int R = (int)tokens * nh;
   const int64_t L = seen0 > 0 ? seen0 + tokens - 1 : 0;
   const int64_t req = KEYS == kRows ? 0 : (L > 0 ? a.reqs[e] : 0);
-  const int64_t stretch = ((L + kTileKeys - 1) / kTileKeys + g.splits - 1) / g.splits * kTileKeys;
+  const int64_t stretch = stretch_keys(L, g.splits);
   const int64_t k0 = blockIdx.z * stretch, k1 = min(L, k0 + stretch);
+  if (k0 >= k1 && blockIdx.z > 0) return;  // nothing left for this one, uniform
 
   for (int i = tid; i < R * dim; i += kAnyThreads) {
     const int r = i / dim, d = i - r * dim;
     const T* q = static_cast<const T*>(a.q) + (row0 + r / nh) * a.q_stride + (int64_t)(h0 + r % nh) * dim;
     s_q[i] = Elem<T>::load(q + d) * a.scale_log2;
   }
-  for (int i = R * dim + tid; i < kRowsPerCta * dim; i += kAnyThreads) s_q[i] = 0.f;
-  if (tid < kRowsPerCta) s_m[tid] = -INFINITY, s_l[tid] = 0.f;
-  float acc[2][kRowsPerCta] = {};
+  for (int i = R * dim + tid; i < ROWS * dim; i += kAnyThreads) s_q[i] = 0.f;
+  if (tid < ROWS) s_m[tid] = -INFINITY, s_l[tid] = 0.f;
+  float acc[2][ROWS] = {};
+  const int lanes = kAnyThreads / g.key_groups, group = tid / lanes, d0 = tid - group * lanes;
   uint32_t* kerr = blockIdx.y == 0 ? a.err : nullptr;
 
-  auto load_tile = [&](const uint8_t* codes, const float* s_scale) {
+  // codes of a tile to fp32, K or V or both; whether V held a NaN
+  auto load_tile = [&](auto keys, auto values) {
     const int per = dim >> 3;
     int nan = 0;
+#pragma unroll 4
     for (int i = tid; i < kTileKeys * per; i += kAnyThreads) {
       const int j = i / per, ch = i - j * per;
       const int64_t slot = s_slot[j];
-      float x[8] = {};
+      uint2 ck = make_uint2(0, 0), cv = make_uint2(0, 0);
       if (slot >= 0) {
-        const int64_t at = (((slot >> c.shift) * c.kv_heads + kvh) * c.block + (slot & (c.block - 1))) * dim;
-        from_e4m3x8(*reinterpret_cast<const uint2*>(codes + at + ch * 8), x);
+        const int64_t at = (((slot >> c.shift) * c.kv_heads + kvh) * c.block + (slot & (c.block - 1))) * dim + ch * 8;
+        if (keys.value) ck = __ldg(reinterpret_cast<const uint2*>(c.k + at));
+        if (values.value) cv = __ldg(reinterpret_cast<const uint2*>(c.v + at));
+      }
+      float x[8];
+      if (keys.value) {
+        from_e4m3x8(ck, x);
+        const float f = s_ks[j];
+        float4* d = reinterpret_cast<float4*>(s_k + j * pitch + ch * 8);
+        d[0] = make_float4(x[0] * f, x[1] * f, x[2] * f, x[3] * f);
+        d[1] = make_float4(x[4] * f, x[5] * f, x[6] * f, x[7] * f);
+      }
+      if (values.value) {
+        from_e4m3x8(cv, x);
+        const float f = s_vs[j];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-          x[u] *= s_scale[j];
+          x[u] *= f;
           nan |= isnan(x[u]);
         }
+        float4* d = reinterpret_cast<float4*>(s_v + j * pitch + ch * 8);
+        d[0] = make_float4(x[0], x[1], x[2], x[3]);
+        d[1] = make_float4(x[4], x[5], x[6], x[7]);
       }
-      float4* d = reinterpret_cast<float4*>(s_kv + j * pitch + ch * 8);
-      d[0] = make_float4(x[0], x[1], x[2], x[3]);
-      d[1] = make_float4(x[4], x[5], x[6], x[7]);
     }
     return nan;
   };
 
+  // the places and scales of a tile are asked for while the one before is at work
+  int64_t slot = -1;
+  float ks = 0.f, vs = 0.f;
+  auto place = [&](int64_t j0) {
+    slot = -1, ks = 0.f, vs = 0.f;
+    if (tid >= kTileKeys || j0 + tid >= k1) return;
+    slot = key_slot<KEYS>(a, e, req, j0 + tid, kerr);
+    if (slot < 0) return;
+    const int64_t bh = (slot >> c.shift) * c.kv_heads + kvh;
+    ks = c.k_scale[bh];
+    vs = c.v_scale[bh];
+  };
+  place(k0);
   for (int64_t j0 = k0; j0 < k1; j0 += kTileKeys) {
     __syncthreads();
-    if (tid < kTileKeys) {
-      int64_t slot = -1;
-      if (j0 + tid < k1) slot = key_slot<KEYS>(a, e, req, j0 + tid, kerr);
-      s_slot[tid] = slot;
-      const int64_t bh = slot < 0 ? 0 : (slot >> c.shift) * c.kv_heads + kvh;
-      s_ks[tid] = slot < 0 ? 0.f : c.k_scale[bh];
-      s_vs[tid] = slot < 0 ? 0.f : c.v_scale[bh];
-    }
+    if (tid < kTileKeys) s_slot[tid] = slot, s_ks[tid] = ks, s_vs[tid] = vs;
     __syncthreads();
-    load_tile(c.k, s_ks);
+    int nan = load_tile(std::true_type{}, std::bool_constant<kBoth>{});
+    place(j0 + kTileKeys);
     __syncthreads();
     {  // scores: thread = key x half of the rows
-      const int j = tid & 63, r0 = (tid >> 6) * 8;
-      float s[8] = {};
-      const float* kp = s_kv + j * pitch;
+      constexpr int kHalf = ROWS / 2;
+      const int j = tid & 63, r0 = (tid >> 6) * kHalf;
+      float s[kHalf] = {};
+      const float* kp = s_k + j * pitch;
       for (int d = 0; d < dim; d += 4) {
         const float4 k4 = *reinterpret_cast<const float4*>(kp + d);
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
+        for (int r = 0; r < kHalf; ++r) {
           const float4 q4 = *reinterpret_cast<const float4*>(s_q + (r0 + r) * dim + d);
           s[r] += fmaf(k4.x, q4.x, fmaf(k4.y, q4.y, fmaf(k4.z, q4.z, k4.w * q4.w)));
         }
       }
       const bool there = s_slot[j] >= 0;
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
+      for (int r = 0; r < kHalf; ++r) {
         const bool seen = there && r0 + r < R && j0 + j < seen0 + (KEYS == kExtend ? (r0 + r) / nh : 0);
         s_p[(r0 + r) * kTileKeys + j] = seen ? s[r] : -INFINITY;
       }
     }
     __syncthreads();
-    const int nan = load_tile(c.v, s_vs);
-    for (int r = warp * 4; r < warp * 4 + 4; ++r) {  // softmax: a warp's four rows
-      const float x0 = s_p[r * kTileKeys + lane], x1 = s_p[r * kTileKeys + lane + 32];
-      // fmaxf drops NaN: a NaN score must reach the sum through its weight
-      float m = fmaxf(x0, x1);
+    if (!kBoth) nan = load_tile(std::false_type{}, std::true_type{});
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const float mo = s_m[r], mn = fmaxf(mo, m), base = mn == -INFINITY ? 0.f : mn;
+    for (int r = warp * (ROWS / 4); r < (warp + 1) * (ROWS / 4); ++r) {  // softmax: a warp's rows
+      const float x0 = s_p[r * kTileKeys + lane], x1 = s_p[r * kTileKeys + lane + 32];
+      // the maximum drops NaN: a NaN score must reach the sum through its weight
+      const float mo = s_m[r], mn = fmaxf(mo, warp_max(fmaxf(x0, x1))), base = mn == -INFINITY ? 0.f : mn;
       const float p0 = exp2f(x0 - base), p1 = exp2f(x1 - base);
       float l = p0 + p1;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
       s_p[r * kTileKeys + lane] = p0;
       s_p[r * kTileKeys + lane + 32] = p1;
+      __syncwarp();
       if (lane == 0) {
         const float corr = exp2f(mo - base);
         s_corr[r] = corr;
@@ -172,17 +219,18 @@ __global__ void __launch_bounds__(kAnyThreads) kv8_attn_any_kernel(AnyArgs g) {
     auto product = [&](auto guard) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int d = tid + u * kAnyThreads;
+        const int d = d0 + u * kAnyThreads;
         if (d >= dim) break;
 #pragma unroll
-        for (int r = 0; r < kRowsPerCta; ++r) acc[u][r] *= s_corr[r];
+        for (int r = 0; r < ROWS; ++r) acc[u][r] *= s_corr[r];
         // a NaN stays with the rows that see its key
         auto behind = [&](float p, float v) { return guard.value && p == 0.f ? 0.f : v; };
-        for (int j = 0; j < kTileKeys; j += 4) {
-          const float v0 = s_kv[j * pitch + d], v1 = s_kv[(j + 1) * pitch + d];
-          const float v2 = s_kv[(j + 2) * pitch + d], v3 = s_kv[(j + 3) * pitch + d];
+        const int keys = kTileKeys / g.key_groups;
+        for (int j = group * keys; j < (group + 1) * keys; j += 4) {
+          const float v0 = s_v[j * pitch + d], v1 = s_v[(j + 1) * pitch + d];
+          const float v2 = s_v[(j + 2) * pitch + d], v3 = s_v[(j + 3) * pitch + d];
 #pragma unroll
-          for (int r = 0; r < kRowsPerCta; ++r) {
+          for (int r = 0; r < ROWS; ++r) {
             const float4 p = *reinterpret_cast<const float4*>(s_p + r * kTileKeys + j);
             acc[u][r] += fmaf(p.x, behind(p.x, v0), fmaf(p.y, behind(p.y, v1),
                                                         fmaf(p.z, behind(p.z, v2), p.w * behind(p.w, v3))));
@@ -194,64 +242,85 @@ __global__ void __launch_bounds__(kAnyThreads) kv8_attn_any_kernel(AnyArgs g) {
     else product(std::false_type{});
   }
   __syncthreads();
-  if (g.splits == 1) {
+  float* rec = a.part + (((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * g.splits + blockIdx.z) * any_record(ROWS, dim);
+  const bool whole = stretch >= L;  // all keys are in this stretch
+  if (!whole && tid < R) rec[2 * tid] = s_m[tid], rec[2 * tid + 1] = s_l[tid];
+  if (g.key_groups > 1) {  // the groups' sums meet in the first one's threads
+    if (d0 < dim)
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int d = tid + u * kAnyThreads;
-      if (d >= dim) break;
+      for (int r = 0; r < ROWS; ++r) s_k[(group * ROWS + r) * dim + d0] = acc[0][r];
+    __syncthreads();
+    if (group > 0 || d0 >= dim) return;
 #pragma unroll
-      for (int r = 0; r < kRowsPerCta; ++r) {
-        if (r >= R) break;
-        T* o = static_cast<T*>(a.out) + (row0 + r / nh) * a.out_stride + (int64_t)(h0 + r % nh) * dim;
-        const float l = s_l[r];
-        Elem<T>::store(o + d, l == 0.f ? 0.f : acc[u][r] / l);
-      }
-    }
-    return;
-  }
-  float* rec = a.part + (((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * g.splits + blockIdx.z) * any_record(dim);
-  if (tid < kRowsPerCta) {
-    rec[2 * tid] = s_m[tid];
-    rec[2 * tid + 1] = s_l[tid];
+    for (int r = 0; r < ROWS; ++r)
+      for (int k = 1; k < g.key_groups; ++k) acc[0][r] += s_k[(k * ROWS + r) * dim + d0];
   }
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    const int d = tid + u * kAnyThreads;
+    const int d = d0 + u * kAnyThreads;
     if (d >= dim) break;
 #pragma unroll
-    for (int r = 0; r < kRowsPerCta; ++r)
-      if (r < R) rec[2 * kRowsPerCta + r * dim + d] = acc[u][r];
+    for (int r = 0; r < ROWS; ++r) {
+      if (r >= R) break;
+      if (whole) {
+        T* o = static_cast<T*>(a.out) + (row0 + r / nh) * a.out_stride + (int64_t)(h0 + r % nh) * dim;
+        const float l = s_l[r];
+        Elem<T>::store(o + d, l == 0.f ? 0.f : acc[u][r] / l);
+      } else {
+        rec[2 * ROWS + r * dim + d] = acc[u][r];
+      }
+    }
   }
 }
 
-// Joins the splits of unit (blockIdx.x, blockIdx.y): thread = channel, the rows in turn.
+// Joins the splits of unit (blockIdx.x, blockIdx.y): a warp per row, a lane per
+// split for the weights and per channel for the sums.
+constexpr int kAnyJoinWarps = 4;
 template <typename T, int KEYS>
-__global__ void __launch_bounds__(kMaxDim) kv8_attn_join_kernel(AnyArgs g) {
+__global__ void __launch_bounds__(kAnyJoinWarps * 32) kv8_attn_join_kernel(AnyArgs g) {
+  __shared__ float s_w[kAnyJoinWarps][kMostSplits];
   const AttnArgs& a = g.a;
-  const int dim = a.c.dim, d = threadIdx.x;
+  const int dim = a.c.dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kvh = blockIdx.y / g.chunks, chunk = blockIdx.y - kvh * g.chunks;
   const int h0 = kvh * a.group + chunk * g.head_chunk;
   const int nh = min(g.head_chunk, a.group - chunk * g.head_chunk);
-  int64_t row0 = blockIdx.x, tokens = 1;
+  wait_prior_grid();
+  allow_next_grid();
+  int64_t row0 = blockIdx.x, tokens = 1, seen0;
   if (KEYS == kExtend) {
     const ExtendEntry x = extend_tile(a, blockIdx.x, g.tile_tokens, 1, nullptr);
     if (x.entry < 0) return;
     row0 = x.row0 + x.tile * g.tile_tokens;
     tokens = min((int64_t)g.tile_tokens, x.n - x.tile * g.tile_tokens);
+    seen0 = x.prefix + x.tile * g.tile_tokens + 1;
+  } else {
+    seen0 = entry_keys<KEYS>(a, blockIdx.x, nullptr);
   }
-  const float* rec = a.part + ((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * g.splits * any_record(dim);
-  for (int r = 0; r < (int)tokens * nh; ++r) {
-    float m = -INFINITY, l = 0.f, o = 0.f;
-    for (int s = 0; s < g.splits; ++s) m = fmaxf(m, rec[s * any_record(dim) + 2 * r]);
+  const int64_t L = seen0 > 0 ? seen0 + tokens - 1 : 0, stretch = stretch_keys(L, g.splits);
+  if (stretch >= L) return;  // written by its CTA
+  const int splits = (int)((L + stretch - 1) / stretch);
+  const int64_t record = any_record(g.rows, dim);
+  const float* rec = a.part + ((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * g.splits * record;
+  for (int r = warp; r < (int)tokens * nh; r += kAnyJoinWarps) {
+    float m = -INFINITY, l = 0.f;
+    for (int s = lane; s < splits; s += 32) m = fmaxf(m, rec[s * record + 2 * r]);
+    m = warp_max(m);
     const float base = m == -INFINITY ? 0.f : m;
-    for (int s = 0; s < g.splits; ++s) {
-      const float* p = rec + s * any_record(dim);
-      const float w = exp2f(p[2 * r] - base);
-      l = fmaf(w, p[2 * r + 1], l);
-      if (d < dim) o = fmaf(w, p[2 * kRowsPerCta + r * dim + d], o);
+    __syncwarp();
+    for (int s = lane; s < splits; s += 32) {
+      const float w = exp2f(rec[s * record + 2 * r] - base);
+      s_w[warp][s] = w;
+      l = fmaf(w, rec[s * record + 2 * r + 1], l);
     }
-    if (d < dim) {
-      T* out = static_cast<T*>(a.out) + (row0 + r / nh) * a.out_stride + (int64_t)(h0 + r % nh) * dim;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    __syncwarp();
+    T* out = static_cast<T*>(a.out) + (row0 + r / nh) * a.out_stride + (int64_t)(h0 + r % nh) * dim;
+    for (int d = lane; d < dim; d += 32) {
+      const float* p = rec + 2 * g.rows + r * dim + d;
+      float o = 0.f;
+#pragma unroll 8
+      for (int s = 0; s < splits; ++s) o = fmaf(s_w[warp][s], p[s * record], o);
       Elem<T>::store(out + d, l == 0.f ? 0.f : o / l);
     }
   }
@@ -260,9 +329,12 @@ __global__ void __launch_bounds__(kMaxDim) kv8_attn_join_kernel(AnyArgs g) {
 AnyArgs any_shape(const AttnArgs& a, int keys) {
   AnyArgs g{};
   g.a = a;
-  g.head_chunk = a.group < kRowsPerCta ? a.group : kRowsPerCta;
+  g.head_chunk = a.group < kMostRows ? a.group : kMostRows;
   g.chunks = (a.group + g.head_chunk - 1) / g.head_chunk;
-  g.tile_tokens = keys == kExtend ? kRowsPerCta / g.head_chunk : 1;
+  g.tile_tokens = keys == kExtend ? kMostRows / g.head_chunk : 1;
+  g.rows = keys == kExtend || g.head_chunk > 8 ? 16 : g.head_chunk > 4 ? 8 : 4;
+  g.key_groups = 1;
+  while (g.key_groups < 8 && 2 * g.key_groups * a.c.dim <= kAnyThreads) g.key_groups *= 2;
   return g;
 }
 int64_t any_tiles(const AnyArgs& g, int keys, int bs, int64_t tokens) {
@@ -272,22 +344,35 @@ int64_t any_tiles(const AnyArgs& g, int keys, int bs, int64_t tokens) {
 int any_splits(const AnyArgs& g, int64_t tiles, int kv_heads, int64_t max_keys) {
   const int64_t units = tiles * kv_heads * g.chunks;
   int64_t s = units > 0 ? (4 * (int64_t)device_sm_count() + units - 1) / units : 1;
-  const int64_t most = (max_keys + 4 * kTileKeys - 1) / (4 * kTileKeys);  // no stretch below four tiles
+  const int64_t most = (max_keys + kTileKeys - 1) / kTileKeys;
   if (s > most) s = most;
-  return (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
+  return (int)(s < 1 ? 1 : (s > kMostSplits ? kMostSplits : s));
+}
+int64_t any_workspace(const AnyArgs& g, int64_t tiles) {
+  return g.splits == 1 ? 0 : (int64_t)sizeof(float) * tiles * g.a.c.kv_heads * g.chunks * g.splits * any_record(g.rows, g.a.c.dim);
 }
 
-template <typename T, int KEYS>
-int launch_any(AnyArgs g, int64_t tiles, cudaStream_t s) {
+template <typename T, int KEYS, int ROWS>
+int launch_any(const AnyArgs& g, int64_t tiles, cudaStream_t s) {
   static SmemLimit limit;
-  const size_t smem = any_smem(g.a.c.dim);
-  const int rc = limit.ensure((const void*)kv8_attn_any_kernel<T, KEYS>, smem);
+  const size_t smem = any_smem(g);
+  int rc = limit.ensure((const void*)kv8_attn_any_kernel<T, KEYS, ROWS>, smem);
   if (rc != QQ_OK) return rc;
   const dim3 grid((unsigned)tiles, g.a.c.kv_heads * g.chunks, g.splits);
-  kv8_attn_any_kernel<T, KEYS><<<grid, kAnyThreads, smem, s>>>(g);
-  if (g.splits > 1)
-    kv8_attn_join_kernel<T, KEYS><<<dim3(grid.x, grid.y), (g.a.c.dim + 31) / 32 * 32, 0, s>>>(g);
-  return launch_status();
+  rc = launch_pdl(kv8_attn_any_kernel<T, KEYS, ROWS>, grid, dim3(kAnyThreads), smem, s, g);
+  if (rc != QQ_OK || g.splits == 1) return rc;
+  return launch_pdl(kv8_attn_join_kernel<T, KEYS>, dim3(grid.x, grid.y), dim3(kAnyJoinWarps * 32), 0, s, g);
+}
+template <typename T>
+int launch_any(const AnyArgs& g, int keys, int64_t tiles, cudaStream_t s) {
+  if (keys == kExtend) return launch_any<T, kExtend, 16>(g, tiles, s);
+  if (keys == kTable)
+    return g.rows == 4   ? launch_any<T, kTable, 4>(g, tiles, s)
+           : g.rows == 8 ? launch_any<T, kTable, 8>(g, tiles, s)
+                         : launch_any<T, kTable, 16>(g, tiles, s);
+  return g.rows == 4   ? launch_any<T, kRows, 4>(g, tiles, s)
+         : g.rows == 8 ? launch_any<T, kRows, 8>(g, tiles, s)
+                       : launch_any<T, kRows, 16>(g, tiles, s);
 }
 
 int run(const AttnArgs& a, int keys, int dtype, int64_t max_keys, size_t ws_bytes, cudaStream_t s) {
@@ -297,18 +382,8 @@ int run(const AttnArgs& a, int keys, int dtype, int64_t max_keys, size_t ws_byte
   const int64_t tiles = any_tiles(g, keys, a.bs, a.tokens);
   if (tiles > INT32_MAX || (int64_t)a.c.kv_heads * g.chunks > 65535) return QQ_ERR_UNSUPPORTED;
   g.splits = any_splits(g, tiles, a.c.kv_heads, max_keys);
-  if (g.splits > 1) {
-    const size_t need =
-        sizeof(float) * (size_t)(tiles * a.c.kv_heads * g.chunks * g.splits * any_record(a.c.dim));
-    if (a.part == nullptr || ws_bytes < need) return QQ_ERR_WORKSPACE;
-  }
-  if (dtype == QQ_BF16)
-    return keys == kTable  ? launch_any<__nv_bfloat16, kTable>(g, tiles, s)
-           : keys == kRows ? launch_any<__nv_bfloat16, kRows>(g, tiles, s)
-                           : launch_any<__nv_bfloat16, kExtend>(g, tiles, s);
-  return keys == kTable  ? launch_any<float, kTable>(g, tiles, s)
-         : keys == kRows ? launch_any<float, kRows>(g, tiles, s)
-                         : launch_any<float, kExtend>(g, tiles, s);
+  if (g.splits > 1 && (a.part == nullptr || ws_bytes < (size_t)any_workspace(g, tiles))) return QQ_ERR_WORKSPACE;
+  return dtype == QQ_BF16 ? launch_any<__nv_bfloat16>(g, keys, tiles, s) : launch_any<float>(g, keys, tiles, s);
 }
 
 // Checks the arguments the three entries share and fills them in.
@@ -348,9 +423,7 @@ extern "C" size_t qq_kv8_workspace_bytes(const qq_kv8_cache* cache, int q_heads,
   AnyArgs g = any_shape(a, keys);
   const int64_t tiles = any_tiles(g, keys, bs, num_tokens);
   g.splits = any_splits(g, tiles, a.c.kv_heads, max_keys);
-  size_t need = 0;
-  if (g.splits > 1)
-    need = sizeof(float) * (size_t)(tiles * a.c.kv_heads * g.chunks * g.splits * any_record(a.c.dim));
+  size_t need = (size_t)any_workspace(g, tiles);
   // enough for either kernel: which one runs depends on the pointers' alignment too
   if (keys != kExtend && decode_tc_fits(a, dtype)) {
     const size_t tc = decode_tc_workspace(bs, a.c.kv_heads, a.group, max_keys);

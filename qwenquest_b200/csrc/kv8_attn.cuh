@@ -38,6 +38,12 @@ struct AttnArgs {
   uint32_t* err;
 };
 
+__device__ __forceinline__ float warp_max(float x) {
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // The keys of one-token entry `e`; 0 when there is nothing to attend to (a
 // bad entry is reported by the caller that passes err and attends to nothing).
 template <int KEYS>

@@ -217,6 +217,7 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
     mbar_init_fence();
   }
   if (warp == 5) tmem_alloc(smem_u32(&s_tmem), kTmemCols);
+  wait_prior_grid();
   const int per = (a.bs + kThreads - 1) / kThreads;
   int64_t before, tiles;
   sum_tiles<KEYS, kThreads>(a, per, before, tiles, blockIdx.x == 0 ? a.err : nullptr);
@@ -620,6 +621,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_decode_join_kernel(const Dec
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int e = blockIdx.x, h = SPLIT ? blockIdx.y / a.group : blockIdx.y;
   wait_prior_grid();
+  allow_next_grid();
   const int64_t total = g.before[a.bs] * a.c.kv_heads, T = g.before[e + 1] - g.before[e];
   __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + e * a.out_stride;
   if (T == 0) {
@@ -711,8 +713,8 @@ int launch(DecodeArgs g, int64_t ctas, cudaStream_t s) {
   } else {
     rk = mk, rv = mv;  // not read
   }
-  kv8_decode_kernel<KEYS, HEADS><<<(unsigned)ctas, kThreads, smem, s>>>(g, mk, mv, rk, rv);
-  if ((rc = launch_status()) != QQ_OK) return rc;
+  rc = launch_pdl(kv8_decode_kernel<KEYS, HEADS>, dim3((unsigned)ctas), dim3(kThreads), smem, s, g, mk, mv, rk, rv);
+  if (rc != QQ_OK) return rc;
   const int pairs = g.a.bs * g.a.c.kv_heads;
   if (ctas >= 4 * (int64_t)pairs)
     return launch_pdl(kv8_decode_join_kernel<HEADS, true>, dim3(g.a.bs, g.a.heads), dim3(kJoinThreads), 0, s, g, ctas);

@@ -246,6 +246,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
   volatile int* abort_flag = &s_abort;
   auto wait = [&](int i, uint32_t parity) { return mbar_wait(bar(i), parity, abort_flag, a.err); };
+  wait_prior_grid();
+  allow_next_grid();
 
   if (warp == 0) {
     const Units units = units_of(g, blockIdx.x == 0 ? a.err : nullptr);
@@ -714,6 +716,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv8_extend_join_kernel(Extend
   }
   __syncthreads();
   wait_prior_grid();
+  allow_next_grid();
   const Unit& u = s_unit;
   if (u.entry < 0 || u.splits == 1) return;
   const int splits = u.splits;
@@ -778,9 +781,9 @@ int run_extend_tc(const AttnArgs& a, int64_t max_keys, size_t ws_bytes, cudaStre
   if (rc != QQ_OK) return rc;
   const int units = g.tiles * a.c.kv_heads;
   const unsigned grid = (unsigned)(units + (g.most > 1 ? g.sms : 0));
-  if (a.c.block >= 64) kv8_extend_kernel<64><<<grid, kThreads, kDynSmem, s>>>(g);
-  else kv8_extend_kernel<16><<<grid, kThreads, kDynSmem, s>>>(g);
-  if ((rc = launch_status()) != QQ_OK || g.most == 1) return rc;
+  rc = a.c.block >= 64 ? launch_pdl(kv8_extend_kernel<64>, dim3(grid), dim3(kThreads), kDynSmem, s, g)
+                       : launch_pdl(kv8_extend_kernel<16>, dim3(grid), dim3(kThreads), kDynSmem, s, g);
+  if (rc != QQ_OK || g.most == 1) return rc;
   // as many CTAs to a unit as there may be room for
   const int cut = std::min(units, g.sms - 1), y = std::max(4, std::min(kUnitRows / kJoinWarps, 8 * g.sms / std::max(1, cut)));
   return launch_pdl(kv8_extend_join_kernel, dim3(std::max(1, cut), y), dim3(kJoinWarps * 32), 0, s, g);

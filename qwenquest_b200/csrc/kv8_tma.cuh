@@ -61,11 +61,5 @@ __device__ __forceinline__ int fit_exponent(float amax) {
 }
 __device__ __forceinline__ float exp2_int(int k) { return __uint_as_float((uint32_t)(k + 127) << 23); }
 
-__device__ __forceinline__ float warp_max(float x) {
-  float r;
-  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
-  return r;
-}
-
 }  // namespace kv8
 }  // namespace qq
