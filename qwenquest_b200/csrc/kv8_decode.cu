@@ -66,19 +66,20 @@ enum : int {
 // The tiles in equal shares: the first `more` shares have one tile more.
 struct Shares {
   int64_t ctas, each, more;
+  bool narrow;  // 32 bits hold all of it: a 64-bit division takes four times as long
   __device__ __forceinline__ Shares(int64_t total, int64_t grid) {
     ctas = min(grid, total);  // no share is empty
-    if (total <= UINT32_MAX) {
-      each = (uint32_t)total / max(1u, (uint32_t)ctas);
-    } else {
-      each = total / ctas;
-    }
+    narrow = total <= UINT32_MAX;
+    each = ratio(total, max((int64_t)1, ctas));
     more = total - each * ctas;
+  }
+  __device__ __forceinline__ int64_t ratio(int64_t x, int64_t y) const {
+    return narrow ? (uint32_t)x / (uint32_t)y : x / y;
   }
   __device__ __forceinline__ int64_t lo(int64_t c) const { return c * each + min(c, more); }
   __device__ __forceinline__ int64_t owner(int64_t tile) const {  // the share that tile lies in
     const int64_t cut = more * (each + 1);
-    return tile < cut ? tile / (each + 1) : more + (tile - cut) / each;
+    return tile < cut ? ratio(tile, each + 1) : more + ratio(tile - cut, each);
   }
 };
 
@@ -136,15 +137,18 @@ struct DecodeArgs {
 
 __host__ __device__ constexpr int64_t record_floats(int heads) { return heads * (2 + (int64_t)kTcDim); }
 
-// The tiles of all entries before this thread's and in all; every thread of the block calls it.
+// The tiles of this thread's first entry, of all entries before it, and in all; every thread of the block calls it.
 template <int KEYS, int THREADS>
-__device__ __forceinline__ void sum_tiles(const AttnArgs& a, int per, int64_t& before, int64_t& total, uint32_t* err) {
+__device__ __forceinline__ void sum_tiles(const AttnArgs& a, int per, int64_t& own, int64_t& before, int64_t& total,
+                                          uint32_t* err) {
   __shared__ int64_t s_sum[THREADS / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int64_t mine = 0;
+  own = 0;
   for (int j = 0; j < per; ++j) {
     const int e = threadIdx.x * per + j;
     if (e < a.bs) mine += (entry_keys<KEYS>(a, e, err) + kTile - 1) / kTile;
+    if (j == 0) own = mine;
   }
   int64_t incl = mine;
 #pragma unroll
@@ -161,6 +165,43 @@ __device__ __forceinline__ void sum_tiles(const AttnArgs& a, int per, int64_t& b
     if (w < warp) before += s_sum[w];
     total += s_sum[w];
   }
+}
+
+// CH channels from `col` on of query head r of (entry, KV head) (zeros past the group) as hi and lo columns of Q;
+// called by all lanes of the warps that hold the head's 128 / CH pieces side by side.
+template <int HEADS, int CH>
+__device__ __forceinline__ void write_query(const AttnArgs& a, int e, int h, int r, int col, uint8_t* dst, float* qinv) {
+  float x[CH] = {};
+  if (r < a.group) {
+    const uint2* q = reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(a.q) + e * a.q_stride +
+                                                    (int64_t)(h * a.group + r) * kTcDim + col);
+#pragma unroll
+    for (int k = 0; k < CH / 4; ++k) {
+      const uint2 u = q[k];
+      x[4 * k] = __uint_as_float(u.x << 16), x[4 * k + 1] = __uint_as_float(u.x & 0xFFFF0000u);
+      x[4 * k + 2] = __uint_as_float(u.y << 16), x[4 * k + 3] = __uint_as_float(u.y & 0xFFFF0000u);
+    }
+  }
+  float most = 0.f;
+#pragma unroll
+  for (int k = 0; k < CH; ++k) {
+    const bool finite = fabsf(x[k]) <= 3.402823466e38f;
+    if (finite) most = fmaxf(most, fabsf(x[k]));
+    else x[k] = __uint_as_float(0x7FFFFFFFu);  // an infinite query has no scores either
+  }
+#pragma unroll
+  for (int o = 1; o < kTcDim / CH; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  const int k2 = fit_exponent(most);
+  const float up = exp2_int(k2);
+#pragma unroll
+  for (int k = 0; k < CH; k += 8) {
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) split_e4m3x2(x[k + 2 * u] * up, x[k + 2 * u + 1] * up, kLo, hi[u], lo[u]);
+    *reinterpret_cast<uint2*>(dst + swz(r, col + k)) = make_uint2(hi[0] | hi[1] << 16, hi[2] | hi[3] << 16);
+    *reinterpret_cast<uint2*>(dst + swz(HEADS + r, col + k)) = make_uint2(lo[0] | lo[1] << 16, lo[2] | lo[3] << 16);
+  }
+  if (col == 0) qinv[r] = a.scale_log2 * exp2_int(-k2);
 }
 
 template <int KEYS, int HEADS>
@@ -219,8 +260,11 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
   if (warp == 5) tmem_alloc(smem_u32(&s_tmem), kTmemCols);
   wait_prior_grid();
   const int per = (a.bs + kThreads - 1) / kThreads;
-  int64_t before, tiles;
-  sum_tiles<KEYS, kThreads>(a, per, before, tiles, blockIdx.x == 0 ? a.err : nullptr);
+  int64_t own, before, tiles;
+  sum_tiles<KEYS, kThreads>(a, per, own, before, tiles, blockIdx.x == 0 ? a.err : nullptr);
+  auto entry_tiles = [&](int j) {  // of this thread's entry j
+    return j == 0 ? own : (entry_keys<KEYS>(a, threadIdx.x * per + j, nullptr) + kTile - 1) / kTile;
+  };
   const Shares shares(tiles * c.kv_heads, gridDim.x);
   allow_next_grid();
   if (blockIdx.x == 0) {
@@ -229,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
       const int e = threadIdx.x * per + j;
       if (e >= a.bs) break;
       g.before[e] = at;
-      at += (entry_keys<KEYS>(a, e, nullptr) + kTile - 1) / kTile;
+      at += entry_tiles(j);
     }
     if (threadIdx.x == 0) g.before[a.bs] = tiles;
   }
@@ -240,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
     for (int j = 0; any && j < per; ++j) {
       const int e = threadIdx.x * per + j;
       if (e >= a.bs || at > lo) break;
-      const int T = (int)((entry_keys<KEYS>(a, e, nullptr) + kTile - 1) / kTile);
+      const int T = (int)entry_tiles(j);
       if (lo < at + (int64_t)T * c.kv_heads) {
         int r = (int)(lo - at), h = 0;
         if (r >= T) h = r / T, r -= h * T;
@@ -381,55 +425,17 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
     int pair = 0;
     bool first = true;
     for (int i = 0; i < count; ++i, w.next()) {
-      if (!first) {
-        first = w.last();
-        continue;
-      }
-      const int qb = pair & 1;
-      if (pair >= 2 && !__all_sync(0xffffffffu, wait(kBarQFree + qb, ((pair >> 1) - 1) & 1))) break;
-      uint8_t* dst = smem + off_q + qb * kColBytes;
-      // four lanes per head, 32 channels each
+      const bool begins = first;
+      first = w.last();
+      if (!begins) continue;
+      const int p = pair++, qb = p & 1;
+      if (p == 0) continue;  // the softmax warps write that one
+      if (p >= 2 && !__all_sync(0xffffffffu, wait(kBarQFree + qb, ((p >> 1) - 1) & 1))) break;
 #pragma unroll
-      for (int r0 = 0; r0 < HEADS; r0 += 8) {
-        const int r = r0 + (lane >> 2), col = (lane & 3) * 32;
-        float x[32] = {};
-        if (r < a.group) {
-          const uint2* q = reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(a.q) + w.e * a.q_stride +
-                                                          (int64_t)(w.h * a.group + r) * kTcDim + col);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint2 u = q[k];
-            x[4 * k] = __uint_as_float(u.x << 16), x[4 * k + 1] = __uint_as_float(u.x & 0xFFFF0000u);
-            x[4 * k + 2] = __uint_as_float(u.y << 16), x[4 * k + 3] = __uint_as_float(u.y & 0xFFFF0000u);
-          }
-        }
-        float most = 0.f;
-#pragma unroll
-        for (int k = 0; k < 32; ++k) {
-          const bool finite = fabsf(x[k]) <= 3.402823466e38f;
-          if (finite) most = fmaxf(most, fabsf(x[k]));
-          else x[k] = __uint_as_float(0x7FFFFFFFu);  // an infinite query has no scores either
-        }
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        const int k2 = fit_exponent(most);
-        const float up = exp2_int(k2);
-#pragma unroll
-        for (int k = 0; k < 32; k += 16) {
-          uint32_t h[8], l[8];
-#pragma unroll
-          for (int u = 0; u < 8; ++u) split_e4m3x2(x[k + 2 * u] * up, x[k + 2 * u + 1] * up, kLo, h[u], l[u]);
-          *reinterpret_cast<uint4*>(dst + swz(r, col + k)) =
-              make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
-          *reinterpret_cast<uint4*>(dst + swz(HEADS + r, col + k)) =
-              make_uint4(l[0] | l[1] << 16, l[2] | l[3] << 16, l[4] | l[5] << 16, l[6] | l[7] << 16);
-        }
-        if ((lane & 3) == 0) s_qinv[pair & 3][r] = a.scale_log2 * exp2_int(-k2);
-      }
+      for (int r0 = 0; r0 < HEADS; r0 += 8)  // four lanes per head, 32 channels each
+        write_query<HEADS, 32>(a, w.e, w.h, r0 + (lane >> 2), (lane & 3) * 32, smem + off_q + qb * kColBytes, s_qinv[p & 3]);
       fence_async_shared();
       mbar_arrive_warp(bar(kBarQ + qb));
-      ++pair;
-      first = w.last();
     }
   } else if (warp == 7) {
     // ================================================================ scales
@@ -495,6 +501,12 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
       for (int r = 0; r < HEADS; ++r)
         O[r] = fmaf(O[r], by[r], fmaf(__uint_as_float(v[HEADS + r]), 1.f / kLo, __uint_as_float(v[r])));
     };
+    // the first queries by all four warps: nothing else can go on before them (1.8 us with one warp)
+    constexpr int kCh = kTcDim * HEADS / kSoft;
+    write_query<HEADS, kCh>(a, w.e, w.h, tok / (kTcDim / kCh), tok % (kTcDim / kCh) * kCh, smem + off_q, s_qinv[0]);
+    fence_async_shared();
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    if (warp == 0) mbar_arrive_warp(bar(kBarQ));
     for (int i = 0; i < count; ++i, w.next()) {
       const int b = i & 1, m = i % kMeta;
       if (first) {
@@ -611,10 +623,11 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
 // records: 2048 CTAs of the other kind took 15 us where 256 of this take 7).
 // A record's outputs are asked for together with the maxima, so the chain is
 // one load long.
-constexpr int kJoinWarps = 8, kJoinThreads = 32 * kJoinWarps;
-constexpr int kJoinAhead = 4;  // records in flight per warp
+constexpr int join_warps(bool split) { return split ? 16 : 8; }
 template <int HEADS, bool SPLIT>
-__global__ void __launch_bounds__(kJoinThreads) kv8_decode_join_kernel(const DecodeArgs g, int64_t ctas) {
+__global__ void __launch_bounds__(32 * join_warps(SPLIT)) kv8_decode_join_kernel(const DecodeArgs g, int64_t ctas) {
+  constexpr int kJoinWarps = SPLIT ? 16 : 8, kJoinThreads = 32 * kJoinWarps;
+  constexpr int kJoinAhead = SPLIT ? 5 : 4;  // records in flight per warp (80 of a pair: its part of 148 x 2 CTAs)
   __shared__ float s_m[kJoinWarps], s_l[kJoinWarps];
   __shared__ __align__(16) float s_o[kJoinWarps][kTcDim];
   const AttnArgs& a = g.a;
@@ -717,8 +730,8 @@ int launch(DecodeArgs g, int64_t ctas, cudaStream_t s) {
   if (rc != QQ_OK) return rc;
   const int pairs = g.a.bs * g.a.c.kv_heads;
   if (ctas >= 4 * (int64_t)pairs)
-    return launch_pdl(kv8_decode_join_kernel<HEADS, true>, dim3(g.a.bs, g.a.heads), dim3(kJoinThreads), 0, s, g, ctas);
-  return launch_pdl(kv8_decode_join_kernel<HEADS, false>, dim3(g.a.bs, g.a.c.kv_heads), dim3(kJoinThreads), 0, s, g, ctas);
+    return launch_pdl(kv8_decode_join_kernel<HEADS, true>, dim3(g.a.bs, g.a.heads), dim3(32 * join_warps(true)), 0, s, g, ctas);
+  return launch_pdl(kv8_decode_join_kernel<HEADS, false>, dim3(g.a.bs, g.a.c.kv_heads), dim3(32 * join_warps(false)), 0, s, g, ctas);
 }
 
 int64_t decode_ctas(int bs, int kv_heads, int group, int64_t max_keys) {
