@@ -322,10 +322,11 @@ int qq_block_trim(const qq_block_tables* tables, const int64_t* req_pool_indices
  * scales [num_blocks][kv_heads]; a value is its code times the scale of its
  * block and head.  block_size 16, 32, 64 or 128, head_dim a multiple of 8 up
  * to 256, codes 16-byte aligned, num_blocks * kv_heads * block_size < 2^31.
- * state (device [QQ_KV8_STATE_WORDS + 2 * kv_heads * num_blocks], zero-filled
- * once) is needed by qq_kv8_append alone.  No reference counterpart: the reference keeps K and V
- * in the model's dtype (MHATokenToKVPool, memory.py:79-120). */
-#define QQ_KV8_STATE_WORDS 34
+ * state (device [QQ_KV8_STATE_WORDS + 2 * kv_heads * num_blocks], 8-byte
+ * aligned, zero-filled once) is needed by qq_kv8_append alone.  No reference
+ * counterpart: the reference keeps K and V in the model's dtype
+ * (MHATokenToKVPool, memory.py:79-120). */
+#define QQ_KV8_STATE_WORDS 66
 typedef struct qq_kv8_cache {
   uint8_t* k;
   uint8_t* v;
@@ -347,7 +348,8 @@ typedef struct qq_kv8_cache {
  * block anew.  Infinities are stored as +-448 s, NaN as NaN.  The tokens of a
  * block stand next to each other in ascending slots: a block met twice in one
  * call, like a slot out of range, is QQ_DEV_ERR_BOUNDS and one of the two
- * stretches is not written.  Calls on one layer are ordered on one stream. */
+ * stretches is not written.  Calls of several streams may overlap where they
+ * write different blocks (a block that two of them write at once is not found). */
 int qq_kv8_append(const qq_kv8_cache* cache, const void* k, const void* v, int dtype, int64_t k_stride,
                   int64_t v_stride, const int64_t* slots, int64_t num_tokens, uint32_t* err, void* stream);
 
@@ -387,7 +389,9 @@ int qq_kv8_sparse_attention(const qq_kv8_cache* cache, int bs, const int32_t* ro
  * of its request, read through block_table (the new tokens are in the cache
  * already).  out_cache_loc and max_seq_len are not read.  Rows behind the
  * last sequence are left as they were, like those of an entry whose lengths,
- * offset or request do not fit (QQ_DEV_ERR_BOUNDS). */
+ * offset or request do not fit (QQ_DEV_ERR_BOUNDS).  Entries share no query
+ * rows: those that do leave them undefined, and more of it than num_tokens
+ * and bs allow for is QQ_DEV_ERR_BOUNDS. */
 int qq_kv8_extend_attention(const qq_kv8_cache* cache, const qq_extend_batch* batch, const int32_t* block_table,
                             int64_t table_stride, int64_t table_rows, const void* q, int dtype, int q_heads,
                             int64_t q_stride, float scaling, void* out, int64_t out_stride, uint32_t* err,

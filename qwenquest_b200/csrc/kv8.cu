@@ -326,10 +326,33 @@ struct AppendArgs {
 
 constexpr int kMaxWindow = 64;
 constexpr int kAppendThreads = 128;
-// The words of `state`: the epoch, a count of full counters, 32 counters of
-// CTAs that are done (one would be 8 us of atomics for 8192 CTAs), the claims.
-constexpr int kEpoch = 0, kFull = 1, kCounters = 2, kNumCounters = 32, kClaims = kCounters + kNumCounters;
+// The words of `state`: 64 bits that count calls in units of 2^-32, 32 such
+// counters for grids of many CTAs (one would be 8 us of atomics for 8192), the
+// claims.  Each CTA of a call adds its part when it is done, and the parts of a
+// call add up to one: the upper half advances when the last CTA leaves, and
+// stays right when calls on several streams overlap, whose parts mix.
+constexpr int kNumCounters = 32, kClaims = 2 + 2 * kNumCounters;
+constexpr uint32_t kFewCtas = 256;
 static_assert(kClaims == QQ_KV8_STATE_WORDS, "the header's size");
+
+__device__ __forceinline__ unsigned long long part_of_one(uint32_t shares, bool first) {
+  const unsigned long long each = (1ull << 32) / shares;
+  return first ? (1ull << 32) - each * (shares - 1) : each;
+}
+__device__ __forceinline__ void count_cta(uint32_t* state) {
+  auto* words = reinterpret_cast<unsigned long long*>(state);
+  const uint32_t ctas = gridDim.x * gridDim.y, id = blockIdx.y * gridDim.x + blockIdx.x;
+  if (ctas < kFewCtas) {
+    atomicAdd(words, part_of_one(ctas, id == 0));
+    return;
+  }
+  const uint32_t mine = id % kNumCounters;
+  const unsigned long long part = part_of_one((ctas - mine + kNumCounters - 1) / kNumCounters, id < kNumCounters);
+  const unsigned long long was = atomicAdd(words + 1 + mine, part);
+  if (was >> 32 != (was + part) >> 32) atomicAdd(words, (1ull << 32) / kNumCounters);
+}
+// What a call's claims are marked with: 0 is none.
+__device__ __forceinline__ uint32_t epoch_of(const uint32_t* state) { return ld_volatile_u32(state + 1) | 0x80000000u; }
 
 // A run is a stretch of tokens whose slots ascend by one inside a block; the
 // CTAs of its first token quantise it, one per K or V and head (blockIdx.y).
@@ -340,8 +363,9 @@ static_assert(kClaims == QQ_KV8_STATE_WORDS, "the header's size");
 // maximum -> codes for a decode step.
 // Two runs of one call that meet in a block would race: a run claims its block
 // with the call's epoch, and the one that finds the epoch there is skipped and
-// reported.  The last CTA to leave advances the epoch, so a captured call gets
-// a new one with every replay.
+// reported.  The device counts the epochs, so a captured call gets a new one
+// with every replay.  (Calls that overlap may share an epoch or use two; they
+// write different blocks, so no claim is wrong.)
 template <typename T, int DIM>
 __global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 2 ? 8 : 4) kv8_append_kernel(AppendArgs a) {
   constexpr int kHeld = 8;
@@ -361,7 +385,7 @@ __global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 2 ? 8 : 4) kv8_ap
   const int64_t total = (int64_t)c.num_blocks << c.shift;
   wait_prior_grid();
   allow_next_grid();
-  const uint32_t epoch = ld_volatile_u32(c.state + kEpoch) + 1;
+  const uint32_t epoch = epoch_of(c.state);
   // s_slots[i] is the slot of token w0 - 1 + i (-1 outside the batch)
   for (int i = tid; i < a.window + c.block + 1; i += kAppendThreads) {
     const int64_t t = w0 - 1 + i;
@@ -531,20 +555,7 @@ __global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 2 ? 8 : 4) kv8_ap
     }
     if (tid == 0) *scale = now;
   }
-  // the epoch advances once every CTA has read it
-  if (tid == 0) {
-    __threadfence();
-    const uint32_t ctas = gridDim.x * gridDim.y, id = blockIdx.y * gridDim.x + blockIdx.x, mine = id % kNumCounters;
-    const uint32_t share = (ctas - mine + kNumCounters - 1) / kNumCounters, counters = min(ctas, (uint32_t)kNumCounters);
-    if (atomicAdd(c.state + kCounters + mine, 1u) == share - 1) {
-      c.state[kCounters + mine] = 0;
-      __threadfence();
-      if (atomicAdd(c.state + kFull, 1u) == counters - 1) {
-        c.state[kFull] = 0;
-        c.state[kEpoch] = epoch == 0xFFFFFFFFu ? 0u : epoch;  // 0 is never an epoch: the claims start at 0
-      }
-    }
-  }
+  if (tid == 0) count_cta(c.state);  // its epoch was read long ago
 }
 
 // ------------------------------------------------------------------ gather
@@ -687,7 +698,7 @@ extern "C" int qq_kv8_append(const qq_kv8_cache* cache, const void* k, const voi
   if (k == nullptr || v == nullptr || slots == nullptr || k_stride < row || v_stride < row) return QQ_ERR_INVALID;
   const int size = dtype == QQ_BF16 ? 2 : 4;
   if ((k_stride * size) % 16 != 0 || (v_stride * size) % 16 != 0 || reinterpret_cast<uintptr_t>(k) % 16 != 0 ||
-      reinterpret_cast<uintptr_t>(v) % 16 != 0)
+      reinterpret_cast<uintptr_t>(v) % 16 != 0 || reinterpret_cast<uintptr_t>(cache->state) % 8 != 0)
     return QQ_ERR_UNSUPPORTED;
   AppendArgs a{};
   a.c = kv8::view(*cache);

@@ -44,6 +44,7 @@ constexpr int kSoft = 128;                     // softmax threads
 constexpr int kThreads = 256;
 constexpr int kMeta = 4;                       // tiles of scales in flight
 constexpr int kMaxSlots = 12;
+constexpr int kInv = 4;                        // pairs of which the softmax may not have seen the queries' scales
 constexpr uint32_t kMasked = 0xFFFFFFFFu;      // a V scale's bits where the token takes no part
 constexpr float kLo = 16.f;
 constexpr float kPScale = 128.f;               // weights (at most 2) times this are e4m3's upper binades
@@ -54,7 +55,8 @@ enum : int {
   kBarEmpty = kBarFull + kMaxSlots,  // [slots] codes have been read
   kBarQ = kBarEmpty + kMaxSlots,     // [2] queries written
   kBarQFree = kBarQ + 2,             // [2] queries read
-  kBarMeta = kBarQFree + 2,          // [kMeta] scales written
+  kBarInv = kBarQFree + 2,           // [kInv] the same for the softmax, which may be up to three pairs behind
+  kBarMeta = kBarInv + kInv,          // [kMeta] scales written
   kBarMetaFree = kBarMeta + kMeta,   // [kMeta] scales read
   kBarS = kBarMetaFree + kMeta,      // [2] scores made
   kBarP = kBarS + 2,                 // [2] weights written
@@ -220,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
   __shared__ int s_abort;
   __shared__ int s_start[3];
   __shared__ float s_ks[kMeta][kMetaN], s_vs[kMeta][kMetaN];
-  __shared__ float s_qinv[4][HEADS];  // a pair's stay until the softmax has passed it: two more pairs on
+  __shared__ float s_qinv[kInv][HEADS];
   __shared__ __align__(16) float s_max[2][HEADS][4];
   __shared__ __align__(16) float s_sum[HEADS][4];
   const AttnArgs& a = g.a;
@@ -250,6 +252,7 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
       mbar_init(bar(kBarP + i), kSoft / 32);
       mbar_init(bar(kBarO + i), 1);
     }
+    for (int i = 0; i < kInv; ++i) mbar_init(bar(kBarInv + i), 1);
     for (int i = 0; i < kMeta; ++i) {
       mbar_init(bar(kBarMeta + i), 1);
       mbar_init(bar(kBarMetaFree + i), kSoft / 32);
@@ -433,9 +436,11 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
       if (p >= 2 && !__all_sync(0xffffffffu, wait(kBarQFree + qb, ((p >> 1) - 1) & 1))) break;
 #pragma unroll
       for (int r0 = 0; r0 < HEADS; r0 += 8)  // four lanes per head, 32 channels each
-        write_query<HEADS, 32>(a, w.e, w.h, r0 + (lane >> 2), (lane & 3) * 32, smem + off_q + qb * kColBytes, s_qinv[p & 3]);
+        write_query<HEADS, 32>(a, w.e, w.h, r0 + (lane >> 2), (lane & 3) * 32, smem + off_q + qb * kColBytes,
+                               s_qinv[p % kInv]);
       fence_async_shared();
       mbar_arrive_warp(bar(kBarQ + qb));
+      mbar_arrive_warp(bar(kBarInv + p % kInv));
     }
   } else if (warp == 7) {
     // ================================================================ scales
@@ -506,13 +511,19 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
     write_query<HEADS, kCh>(a, w.e, w.h, tok / (kTcDim / kCh), tok % (kTcDim / kCh) * kCh, smem + off_q, s_qinv[0]);
     fence_async_shared();
     asm volatile("bar.sync 1, 128;" ::: "memory");
-    if (warp == 0) mbar_arrive_warp(bar(kBarQ));
+    if (warp == 0) {
+      mbar_arrive_warp(bar(kBarQ));
+      mbar_arrive_warp(bar(kBarInv));
+    }
     for (int i = 0; i < count; ++i, w.next()) {
       const int b = i & 1, m = i % kMeta;
       if (first) {
 #pragma unroll
         for (int r = 0; r < HEADS; ++r) M[r] = -INFINITY, l[r] = 0.f, O[r] = 0.f, corr[r] = 0.f;
-        ok = ok && wait(kBarQ + (pair & 1), (pair >> 1) & 1);
+        // Q's own barrier may be two phases on by now: with a tile to a pair the
+        // scores run two pairs ahead of this, and the queries two more.  The
+        // scales of pair p + kInv are written after S(p + 2), so after P(p).
+        ok = ok && wait(kBarInv + pair % kInv, (pair / kInv) & 1);
       }
       ok = ok && wait(kBarMeta + m, (i / kMeta) & 1);
       const int mk = KEYS == kRows ? tok : tok >> c.shift;
@@ -532,7 +543,7 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
       float u[HEADS], most[HEADS];
 #pragma unroll
       for (int r = 0; r < HEADS; ++r) {
-        const float s = fmaf(__uint_as_float(v[HEADS + r]), 1.f / kLo, __uint_as_float(v[r])) * (s_qinv[pair & 3][r] * ks);
+        const float s = fmaf(__uint_as_float(v[HEADS + r]), 1.f / kLo, __uint_as_float(v[r])) * (s_qinv[pair % kInv][r] * ks);
         u[r] = seen ? s + (float)ev : -INFINITY;
         most[r] = u[r];
       }

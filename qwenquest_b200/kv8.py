@@ -21,7 +21,8 @@ A step::
 
 Nothing here waits for the GPU.  What a kernel finds wrong (an index out of range, no free block) is kept in an
 error word and raised by the next call on the object or by ``check_errors``; ``synchronize`` waits first.
-Calls run on the current stream of the object's device.
+Calls run on the current stream of the object's device.  Plans and trims of one set of tables go one after another;
+appends of several streams may overlap where they write different blocks, and attention calls share nothing.
 """
 
 from __future__ import annotations
@@ -170,7 +171,7 @@ class BlockTables(_OnDevice):
         if num_tokens < 0:
             raise ValueError("num_tokens must be >= 0")
         made = reqs.new_empty(num_tokens + bs + 1)
-        slots, offsets = made.split((num_tokens, bs + 1))
+        slots, offsets = made.split_with_sizes((num_tokens, bs + 1))
         mapped = (None, 0, 0)
         if req_to_token is not None:
             if (req_to_token.dim() != 2 or req_to_token.dtype != torch.int32 or req_to_token.stride(1) != 1
@@ -262,9 +263,10 @@ class KV8Cache(_OnDevice):
 
     def _tokens(self, t: torch.Tensor, name: str) -> tuple[torch.Tensor, int, int]:
         """``[n, kv_heads, head_dim]`` with dense 16-byte aligned rows, its address and the distance between tokens."""
-        if t.dim() != 3 or t.shape[1] != self.kv_heads or t.shape[2] != self.head_dim or t.get_device() != self._index:
+        shape = t.shape
+        if len(shape) != 3 or shape[1] != self.kv_heads or shape[2] != self.head_dim or t.get_device() != self._index:
             raise ValueError(f"{name} must be [tokens, {self.kv_heads}, {self.head_dim}] on {self.device}, "
-                             f"got {tuple(t.shape)} on {t.device}")
+                             f"got {tuple(shape)} on {t.device}")
         token, head, one = t.stride()
         row = self.kv_heads * self.head_dim
         ptr = t.data_ptr()
@@ -309,10 +311,11 @@ class KV8Cache(_OnDevice):
 
     def _query(self, q: torch.Tensor, out: torch.Tensor | None) -> tuple[torch.Tensor, int, int, torch.Tensor, int]:
         """The queries with dense 16-byte aligned rows, their address and row distance; the result and its row distance."""
-        if q.dim() != 3 or q.shape[2] != self.head_dim or q.get_device() != self._index:
-            raise ValueError(f"q must be [tokens, heads, {self.head_dim}] on {self.device}, got {tuple(q.shape)} "
+        shape = q.shape
+        if len(shape) != 3 or shape[2] != self.head_dim or q.get_device() != self._index:
+            raise ValueError(f"q must be [tokens, heads, {self.head_dim}] on {self.device}, got {tuple(shape)} "
                              f"on {q.device}")
-        n, heads, dim = q.shape
+        n, heads, dim = shape
         if heads == 0 or heads % self.kv_heads:
             raise ValueError(f"q_heads {heads} not divisible by kv_heads {self.kv_heads}")
         token, head, one = q.stride()
@@ -329,10 +332,11 @@ class KV8Cache(_OnDevice):
         return q, ptr, token, out, max(out.stride(0), row)
 
     def _table(self, t: torch.Tensor) -> torch.Tensor:
-        if t.dim() != 2 or t.dtype != torch.int32 or t.get_device() != self._index or t.shape[0] == 0 or t.shape[1] == 0:
+        shape = t.shape
+        if len(shape) != 2 or t.dtype != torch.int32 or t.get_device() != self._index or 0 in shape:
             raise ValueError(f"block_table must be int32 [requests, blocks] on {self.device}")
         # the kernels take the row's stride as its length
-        return t if t.stride(1) == 1 and t.stride(0) == t.shape[1] else t.contiguous()
+        return t if t.stride() == (shape[1], 1) else t.contiguous()
 
     def _workspace(self, heads: int, code: int, bs: int, tokens: int, max_keys: int, extend: int):
         key = (heads, code, bs, tokens, max_keys, extend)
@@ -340,8 +344,9 @@ class KV8Cache(_OnDevice):
         if size is None:
             if len(self._ws_bytes) > 4096:  # sizes only: cheap to ask for again
                 self._ws_bytes.clear()
-            size = self._ws_bytes[key] = int(self.lib.qq_kv8_workspace_bytes(
-                self._layers[0], heads, code, bs, tokens, max_keys, extend))
+            with torch.cuda.device(self._index):  # the size depends on the device
+                size = self._ws_bytes[key] = int(self.lib.qq_kv8_workspace_bytes(
+                    self._layers[0], heads, code, bs, tokens, max_keys, extend))
         if size == 0:
             return None, 0, None
         # each call has scratch of its own: calls on several streams, or captured graphs, share none

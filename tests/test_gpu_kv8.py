@@ -308,6 +308,59 @@ def test_append_takes_strided_rows_and_other_layers_stay():
         _assert_cache(cache, layer, k[layer], v[layer], ks[layer], vs[layer])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_append_takes_values_off_the_16_byte_grid(dtype):
+    """Contiguous rows at an odd element: the kernel's wide loads get an aligned copy."""
+    cache, k, v, ks, vs = _cache(4, 2, 16, 24, seed=8)
+    x = torch.randn(20 * 48 + 3, dtype=dtype, device=DEV)
+    slots = np.arange(16, 36)
+    rows = [x[i:i + 20 * 48].view(20, 2, 24) for i in (1, 3)]
+    assert all(r.data_ptr() % 16 for r in rows)
+    cache.append(0, *rows, _dev(slots))
+    cache.synchronize()
+    oracle.append(k[0], ks[0], rows[0].double().cpu().numpy(), slots)
+    oracle.append(v[0], vs[0], rows[1].double().cpu().numpy(), slots)
+    _assert_cache(cache, 0, k[0], v[0], ks[0], vs[0])
+
+
+def test_appends_of_two_streams_into_one_layer():
+    """Calls of few and of many thread blocks that overlap, in blocks of their own; afterwards a block met twice is
+    found as before, so no call's count was lost."""
+    block, kv, dim, blocks = 16, 4, 32, 800
+    cache, k, v, ks, vs = _cache(blocks, kv, block, dim, seed=9)
+    rng = np.random.default_rng(10)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    todo = [[], []]
+    for i in range(2):
+        own = rng.permutation(np.arange(i * blocks // 2, (i + 1) * blocks // 2))
+        for n in (1, 3, 40, 300, 30, 2, 350) * 3:  # blocks: 8 to 2800 thread blocks
+            slots = np.concatenate([b * block + np.arange(rng.integers(1, 4)) for b in rng.permutation(own)[:n]])
+            x = torch.from_numpy(rng.standard_normal((len(slots), kv, dim))).to(torch.bfloat16)
+            todo[i].append((x.to(DEV), _dev(slots), x.double().numpy(), slots))
+    torch.cuda.synchronize()
+    for a, b in zip(*todo):
+        for s, (x, slots, _, _) in zip(streams, (a, b)):
+            with torch.cuda.stream(s):
+                cache.append(0, x, x, slots)
+    torch.cuda.synchronize()
+    cache.check_errors()
+    for calls in todo:
+        for _, _, x, slots in calls:
+            oracle.append(k[0], ks[0], x, slots)
+            oracle.append(v[0], vs[0], x, slots)
+    _assert_cache(cache, 0, k[0], v[0], ks[0], vs[0])
+    words = cache._state[0, :2].tolist()  # 64 bits: whole calls, none left in parts
+    assert words == [0, sum(len(calls) for calls in todo)]
+    x = torch.randn(2, kv, dim, device=DEV)
+    for _ in range(2):
+        cache.append(0, x, x, _dev([3, 3]))
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError):
+            cache.check_errors()
+        cache.append(0, x[:1], x[:1], _dev([3]))
+        cache.synchronize()
+
+
 @pytest.mark.parametrize("slots", [
     [3, 3],              # a slot twice
     [3, 5],              # a block in two stretches
@@ -658,6 +711,96 @@ def test_results_do_not_depend_on_the_batch_or_the_call():
     first = b.cache.decode_attention(0, q, *args, b.scaling)
     again = b.cache.decode_attention(0, q, *args, b.scaling)
     assert torch.equal(first, again)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_extend_of_ragged_chunks_in_every_cut(dtype):
+    """From fewer query tiles than SMs, all of whose keys are cut, to whole tiles with a cut rest (bf16: 256 rows)."""
+    kv, heads, dim, block = 4, 32, 128, 64
+    for seq, new in (([2600], [3]), ([700, 2000], [300, 600]), ([900, 1500, 1300], [900, 500, 10])):
+        if dtype == torch.float32 and len(seq) == 3:
+            continue
+        b = _Batch(seq, kv, dim, block, seed=sum(new), heads=heads, dtype=dtype)
+        offsets = np.concatenate([[0], np.cumsum(new)])
+        q = b.queries(int(offsets[-1]))
+        out = b.cache.extend_attention(0, q.to(DEV), b.table_dev, _dev(b.reqs), _dev(seq), _dev(np.subtract(seq, new)),
+                                       _dev(offsets), b.scaling)
+        b.cache.synchronize()
+        for i, (s, m) in enumerate(zip(seq, new)):
+            for t in sorted({0, 1, m // 2, m - 2, m - 1} & set(range(m))):
+                row = offsets[i] + t
+                b.check(out[row], q[row], b.slots(i, np.arange(s - m + t + 1)), SMALL_EXTEND)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_extend_reports_entries_that_share_rows(dtype):
+    n = 512
+    b = _Batch([n, n, n], 4, 128, 64, seed=41, heads=32, dtype=dtype)
+    q = b.queries(n).to(DEV)
+    lens = _dev([n, n, n]), _dev([0, 0, 0])
+    b.cache.extend_attention(0, q, b.table_dev, _dev(b.reqs), *lens, _dev([0, 0, 0]), b.scaling)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError):
+        b.cache.check_errors()
+    one = b.cache.extend_attention(0, q, b.table_dev, _dev(b.reqs[:1]), lens[0][:1], lens[1][:1], _dev([0]), b.scaling)
+    b.cache.synchronize()
+    b.check(one[n - 1], q[n - 1].cpu(), b.slots(0, np.arange(n)), SMALL_EXTEND)
+
+
+@pytest.mark.parametrize(("kv", "heads", "dim", "dtype"), [(4, 8, 128, torch.bfloat16), (2, 4, 32, torch.float32)])
+def test_attention_of_the_largest_batch(kv, heads, dim, dtype):
+    bs = 4096
+    rng = np.random.default_rng(2)
+    seq = rng.integers(0, 40, bs)
+    b = _Batch(seq, kv, dim, 16, seed=43, heads=heads, dtype=dtype)
+    q = b.queries(bs)
+    reqs, lens = _dev(b.reqs), _dev(seq)
+    out = b.cache.decode_attention(0, q.to(DEV), b.table_dev, reqs, lens, b.scaling)
+    prefix = np.maximum(seq - 1, 0)
+    offsets = np.concatenate([[0], np.cumsum(seq - prefix)])
+    few = q[:offsets[-1]]
+    ext = b.cache.extend_attention(0, few.to(DEV), b.table_dev, reqs, lens, _dev(prefix), _dev(offsets), b.scaling)
+    b.cache.synchronize()
+    for i in [*range(0, bs, 97), bs - 1]:
+        if seq[i] == 0:
+            assert not out[i].count_nonzero()
+            continue
+        b.check(out[i], q[i], b.slots(i, np.arange(seq[i])))
+        b.check(ext[offsets[i]], few[offsets[i]], b.slots(i, np.arange(seq[i])), SMALL_EXTEND)
+
+
+def test_a_cache_past_32_bits_of_codes():
+    """Blocks whose codes lie beyond 2^32 bytes: written, read back and attended to."""
+    kv, heads, dim, block = 4, 32, 128, 64
+    blocks = 2 ** 32 // (kv * block * dim) + 40
+    cache = KV8Cache(1, blocks, kv, dim, DEV, block_size=block)
+    n = 10 * block + 5
+    chosen = [blocks - 1 - 3 * i for i in range(11)]
+    slots = np.concatenate([b * block + np.arange(block) for b in chosen])[:n]
+    rng = np.random.default_rng(12)
+    k, v = (torch.from_numpy(rng.standard_normal((n, kv, dim))).to(torch.bfloat16) for _ in range(2))
+    cache.append(0, k.to(DEV), v.to(DEV), _dev(slots))
+    q = torch.from_numpy(rng.standard_normal((1, heads, dim))).to(torch.bfloat16)
+    table = _dev([chosen], torch.int32)
+    outs = [cache.decode_attention(0, q.to(DEV), table, [0], [n], dim ** -0.5),
+            cache.sparse_decode_attention(0, q.to(DEV), _dev([slots], torch.int32), [n], dim ** -0.5),
+            cache.extend_attention(0, q.to(DEV), table, [0], [n], [n - 1], [0], dim ** -0.5)]
+    wide = cache.decode_attention(0, q.float().to(DEV), table, [0], [n], dim ** -0.5)
+    got = cache.gather(0, _dev(slots), dtype=torch.float32)
+    cache.synchronize()
+    small = [np.zeros((11, kv, block, dim), dtype=np.uint8) for _ in range(2)]
+    scales = [np.zeros((11, kv), dtype=np.float32) for _ in range(2)]
+    place = np.arange(n)
+    rows = []
+    for c, s, x in zip(small, scales, (k, v)):
+        oracle.append(c, s, x.double().numpy(), place)
+        rows.append(oracle.rows(c, s, place))
+    for g, want in zip(got, rows):
+        assert np.array_equal(g.double().cpu().numpy(), want)
+    out, *bounds = oracle.attend(q[0].double().numpy(), *rows, dim ** -0.5, scales[1][place // block])
+    for o, dtype in [(x, torch.bfloat16) for x in outs] + [(wide, torch.float32)]:
+        tol = _tolerance(dtype, n, dim, out, *bounds, SMALL_DECODE)
+        assert (np.abs(o[0].double().cpu().numpy().reshape(out.shape) - out) <= tol).all()
 
 
 # ---------------------------------------------------------------- streams, graphs, the step as a whole
