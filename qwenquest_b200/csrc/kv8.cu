@@ -560,46 +560,53 @@ __global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 2 ? 8 : 4) kv8_ap
 
 // ------------------------------------------------------------------ gather
 
-// out[i] = the values of slot slots[i] (code times scale): 8 elements of K and
-// of V per thread and step (16 took 17.4 us where 8 take 15.5, for 22.8K
-// tokens of 4 x 128), bound by the bytes.  A slot of -1 gives zeros.
-template <typename T>
-__global__ void __launch_bounds__(256) kv8_gather_kernel(Cache c, const int64_t* slots, int64_t n, T* k_out, T* v_out,
-                                                         uint32_t* err) {
+// out[i] = the values of slot slots[i] (code times scale): a warp per token, so
+// the slot's place is found once for its row of K and of V, 8 elements of each
+// per lane and step.  Bound by the bytes (22.8K tokens of 4 x 128: 12.5 us
+// cold; a thread per piece took 17.3, three quarters of the issue slots for its
+// divisions).  A slot of -1 gives zeros.
+constexpr int kGatherWarps = 4;
+template <typename T, int DIM>
+__global__ void __launch_bounds__(32 * kGatherWarps) kv8_gather_kernel(Cache c, const int64_t* slots, int64_t n, T* k_out,
+                                                                       T* v_out, uint32_t* err) {
   wait_prior_grid();
   allow_next_grid();
-  const int chunks = c.dim >> 3, row = c.kv_heads * chunks;
+  const int dim = DIM > 0 ? DIM : c.dim, lane = threadIdx.x & 31;
+  const int chunks = dim >> 3, row = c.kv_heads * chunks;
   const int64_t total = (int64_t)c.num_blocks << c.shift;
-  const int64_t items = n * row;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < items; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t t = items <= UINT32_MAX ? (uint32_t)i / (uint32_t)row : i / row;
-    const int w = (int)(i - t * row);
-    const int h = w / chunks, ch = w - h * chunks;
+  for (int64_t t = (int64_t)blockIdx.x * kGatherWarps + (threadIdx.x >> 5); t < n; t += (int64_t)gridDim.x * kGatherWarps) {
     const int64_t slot = slots[t];
-    float kx[8] = {}, vx[8] = {};
-    if (slot >= 0 && slot < total) {
-      const int64_t bh = (slot >> c.shift) * c.kv_heads + h;
-      const int64_t at = (bh * c.block + (slot & (c.block - 1))) * c.dim + ch * 8;
-      const float ks = c.k_scale[bh], vs = c.v_scale[bh];
-      from_e4m3x8(*reinterpret_cast<const uint2*>(c.k + at), kx);
-      from_e4m3x8(*reinterpret_cast<const uint2*>(c.v + at), vx);
+    const bool in = slot >= 0 && slot < total;
+    if (!in && slot != -1 && lane == 0) raise_error(err, QQ_DEV_ERR_BOUNDS);
+    const int64_t bh0 = in ? (slot >> c.shift) * c.kv_heads : 0;
+    const int64_t at0 = (bh0 * c.block + (slot & (c.block - 1))) * dim;
+#pragma unroll 1
+    for (int w = lane; w < row; w += 32) {
+      float kx[8] = {}, vx[8] = {};
+      if (in) {
+        const int h = w / chunks;
+        const int64_t at = at0 + ((int64_t)h * c.block * chunks + (w - h * chunks)) * 8;
+        const uint2 kc = *reinterpret_cast<const uint2*>(c.k + at), vc = *reinterpret_cast<const uint2*>(c.v + at);
+        const float ks = c.k_scale[bh0 + h], vs = c.v_scale[bh0 + h];
+        from_e4m3x8(kc, kx);
+        from_e4m3x8(vc, vx);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) kx[e] *= ks, vx[e] *= vs;
-    } else if (slot != -1) {
-      raise_error(err, QQ_DEV_ERR_BOUNDS);
+        for (int e = 0; e < 8; ++e) kx[e] *= ks, vx[e] *= vs;
+      }
+      store8(k_out + (t * row + w) * 8, kx);
+      store8(v_out + (t * row + w) * 8, vx);
     }
-    store8(k_out + i * 8, kx);
-    store8(v_out + i * 8, vx);
   }
 }
 
 template <typename T>
 int launch_gather(const Cache& c, const int64_t* slots, int64_t n, void* k_out, void* v_out, uint32_t* err,
                   cudaStream_t s) {
-  const int64_t items = n * c.kv_heads * (c.dim / 8);
-  const int64_t most = (int64_t)device_sm_count() * 32;
-  const unsigned ctas = (unsigned)((items + 255) / 256 < most ? (items + 255) / 256 : most);
-  return launch_pdl(kv8_gather_kernel<T>, dim3(ctas), dim3(256), 0, s, c, slots, n, static_cast<T*>(k_out), static_cast<T*>(v_out), err);
+  const int64_t most = (int64_t)device_sm_count() * 32, ctas = (n + kGatherWarps - 1) / kGatherWarps;
+  const dim3 grid((unsigned)(ctas < most ? ctas : most)), block(32 * kGatherWarps);
+  T *k = static_cast<T*>(k_out), *v = static_cast<T*>(v_out);
+  return c.dim == 128 ? launch_pdl(kv8_gather_kernel<T, 128>, grid, block, 0, s, c, slots, n, k, v, err)
+                      : launch_pdl(kv8_gather_kernel<T, 0>, grid, block, 0, s, c, slots, n, k, v, err);
 }
 
 int check_tables(const qq_block_tables* t, int bs, const int64_t* reqs) {
