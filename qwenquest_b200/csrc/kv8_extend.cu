@@ -357,6 +357,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
     // made again from the tile's maximum.
     float m = -INFINITY, l = 0.f, alpha = 1.f;  // O still has to be multiplied by alpha
     bool ok = true;
+    const int sees = __reduce_min_sync(0xffffffffu, reach);  // the last key that all of the warp's rows see
 #pragma unroll 1
     for (int j = 0; j < tiles; ++j) {
       const int meta = j % kMeta;
@@ -365,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
       tc_fence_after();
       // columns c <= lim are seen by this row
       const int lim = max(-1, min(kN - 1, reach - j * kN));
-      const bool full = __all_sync(0xffffffffu, lim == kN - 1);
+      const bool full = j * kN + kN - 1 <= sees;
       uint32_t v[2][32];  // scores in chunks of 32 columns, the next one always on its way
       float part, sum;    // of the half in hand: what l takes, and the plain sum
       float most = 0.f;   // the larger of the halves' sums
@@ -403,11 +404,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
         tmem_st_wait();
         alpha = 1.f;
       };
-      if (__any_sync(0xffffffffu, m == -INFINITY)) {
+      if (__any_sync(0xffffffffu, m == -INFINITY || alpha != 1.f)) {
         const float mb = highest(0);
         if (m == -INFINITY) m = mb;
+        if (j > 0) rescale();
+        alpha = 1.f;
       }
-      if (__any_sync(0xffffffffu, alpha != 1.f)) rescale();
       tmem_ld32(tS, v[0]);
       if (h == 0) mbar_arrive_warp(bar(kBarLag + (j & 1)));
 
