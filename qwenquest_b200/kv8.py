@@ -74,11 +74,30 @@ class _OnDevice:
     def _call(self, fn, *args) -> None:
         """One entry point, launched on the current stream of the object's device (also when another is current)."""
         index = self._index
-        if torch.cuda.current_device() == index:
+        if torch._C._cuda_getDevice() == index:
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
         else:
             with torch.cuda.device(index):
                 rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        if rc:
+            check(rc, fn.__name__)
+
+    def _call_with_scratch(self, size: int, fn, *args) -> None:
+        """The same with `size` bytes of scratch, the call's own: calls on several streams, or captured graphs,
+        share none.  Asked of the allocator that tensors come from, on the launching stream, and handed back as a
+        tensor would be (a tensor around it takes 2 us more)."""
+        if not size:
+            return self._call(fn, *args, None, 0)
+        index = self._index
+        if torch._C._cuda_getDevice() != index:
+            with torch.cuda.device(index):
+                return self._call_with_scratch(size, fn, *args)
+        stream = torch._C._cuda_getCurrentRawStream(index)
+        scratch = torch._C._cuda_cudaCachingAllocator_raw_alloc(size, stream)
+        try:
+            rc = fn(*args, scratch, size, stream)
+        finally:
+            torch._C._cuda_cudaCachingAllocator_raw_delete(scratch)
         if rc:
             check(rc, fn.__name__)
 
@@ -301,7 +320,7 @@ class KV8Cache(_OnDevice):
         slots = self._ints(slots, torch.int64, "slots")
         n = slots.shape[0]
         code = dtype_code(dtype)
-        k = slots.new_empty((n, self.kv_heads, self.head_dim), dtype=dtype)
+        k = slots.new_empty(n, self.kv_heads, self.head_dim, dtype=dtype)
         v = torch.empty_like(k)
         self._call(self.lib.qq_kv8_gather, self._layers[layer], slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), code,
                    self._err_ptr)
@@ -325,7 +344,7 @@ class KV8Cache(_OnDevice):
             q = q.clone(memory_format=torch.contiguous_format)
             ptr, token = q.data_ptr(), row
         if out is None:
-            return q, ptr, token, q.new_empty((n, row)), row
+            return q, ptr, token, q.new_empty(n, row), row
         if (tuple(out.shape) != (n, row) or out.dtype != q.dtype or out.device != self.device
                 or out.stride(1) != 1 or (n > 1 and out.stride(0) < row)):
             raise ValueError(f"out must be {q.dtype} [{n}, {row}] with contiguous rows on {self.device}")
@@ -338,7 +357,7 @@ class KV8Cache(_OnDevice):
         # the kernels take the row's stride as its length
         return t if t.stride() == (shape[1], 1) else t.contiguous()
 
-    def _workspace(self, heads: int, code: int, bs: int, tokens: int, max_keys: int, extend: int):
+    def _workspace(self, heads: int, code: int, bs: int, tokens: int, max_keys: int, extend: int) -> int:
         key = (heads, code, bs, tokens, max_keys, extend)
         size = self._ws_bytes.get(key)
         if size is None:
@@ -347,11 +366,7 @@ class KV8Cache(_OnDevice):
             with torch.cuda.device(self._index):  # the size depends on the device
                 size = self._ws_bytes[key] = int(self.lib.qq_kv8_workspace_bytes(
                     self._layers[0], heads, code, bs, tokens, max_keys, extend))
-        if size == 0:
-            return None, 0, None
-        # each call has scratch of its own: calls on several streams, or captured graphs, share none
-        ws = self._state.new_empty(size // 4)
-        return ws.data_ptr(), size, ws
+        return size
 
     def decode_attention(self, layer: int, q: torch.Tensor, block_table: torch.Tensor, req_pool_indices, seq_lens,
                          scaling: float, *, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -371,10 +386,11 @@ class KV8Cache(_OnDevice):
         reqs = self._ints(req_pool_indices, torch.int64, "req_pool_indices", bs)
         seq = self._ints(seq_lens, torch.int64, "seq_lens", bs)
         width = table.shape[1]
-        ws, size, keep = self._workspace(heads, code, bs, bs, width * self.block_size, 0)
-        self._call(self.lib.qq_kv8_decode_attention, self._layers[layer],
-                   _lib.QQBatch(reqs.data_ptr(), seq.data_ptr(), bs), table.data_ptr(), width, table.shape[0],
-                   q_ptr, code, heads, q_stride, float(scaling), out.data_ptr(), out_stride, self._err_ptr, ws, size)
+        size = self._workspace(heads, code, bs, bs, width * self.block_size, 0)
+        self._call_with_scratch(size, self.lib.qq_kv8_decode_attention, self._layers[layer],
+                                _lib.QQBatch(reqs.data_ptr(), seq.data_ptr(), bs), table.data_ptr(), width,
+                                table.shape[0], q_ptr, code, heads, q_stride, float(scaling), out.data_ptr(),
+                                out_stride, self._err_ptr)
         return out
 
     def sparse_decode_attention(self, layer: int, q: torch.Tensor, rows: torch.Tensor, lens, scaling: float, *,
@@ -394,10 +410,10 @@ class KV8Cache(_OnDevice):
             rows = rows.to(torch.int32).contiguous()
         lens = self._ints(lens, torch.int32, "lens", bs)
         top = rows.shape[1]
-        ws, size, keep = self._workspace(heads, code, bs, bs, top, 0)
-        self._call(self.lib.qq_kv8_sparse_attention, self._layers[layer], bs, rows.data_ptr(), rows.stride(0), top,
-                   lens.data_ptr(), q_ptr, code, heads, q_stride, float(scaling), out.data_ptr(), out_stride,
-                   self._err_ptr, ws, size)
+        size = self._workspace(heads, code, bs, bs, top, 0)
+        self._call_with_scratch(size, self.lib.qq_kv8_sparse_attention, self._layers[layer], bs, rows.data_ptr(),
+                                rows.stride(0), top, lens.data_ptr(), q_ptr, code, heads, q_stride, float(scaling),
+                                out.data_ptr(), out_stride, self._err_ptr)
         return out
 
     def extend_attention(self, layer: int, q: torch.Tensor, block_table: torch.Tensor, req_pool_indices, seq_lens,
@@ -424,10 +440,10 @@ class KV8Cache(_OnDevice):
         if offsets.shape[0] not in (bs, bs + 1):
             raise ValueError(f"token_offsets must be [{bs}] or [{bs + 1}], got {tuple(offsets.shape)}")
         width = table.shape[1]
-        ws, size, keep = self._workspace(heads, code, bs, tokens, width * self.block_size, 1)
+        size = self._workspace(heads, code, bs, tokens, width * self.block_size, 1)
         batch = _lib.QQExtendBatch(reqs.data_ptr(), seq.data_ptr(), prefix.data_ptr(), offsets.data_ptr(), None,
                                    tokens, bs, 0)
-        self._call(self.lib.qq_kv8_extend_attention, self._layers[layer], batch, table.data_ptr(), width,
-                   table.shape[0], q_ptr, code, heads, q_stride, float(scaling), out.data_ptr(), out_stride,
-                   self._err_ptr, ws, size)
+        self._call_with_scratch(size, self.lib.qq_kv8_extend_attention, self._layers[layer], batch, table.data_ptr(),
+                                width, table.shape[0], q_ptr, code, heads, q_stride, float(scaling), out.data_ptr(),
+                                out_stride, self._err_ptr)
         return out
