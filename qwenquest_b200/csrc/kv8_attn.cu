@@ -15,6 +15,7 @@
 // heads: 17 us; 53 with 16 rows always, one tile in hand and stretches of four).
 // An extend batch is bound by the fp32 FMAs and their shared-memory operands.
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -273,14 +274,17 @@ __global__ void __launch_bounds__(kAnyThreads) kv8_attn_any_kernel(AnyArgs g) {
   }
 }
 
-// Joins the splits of unit (blockIdx.x, blockIdx.y): a warp per row, a lane per
-// split for the weights and per channel for the sums.
-constexpr int kAnyJoinWarps = 4;
+// Joins the splits of unit (blockIdx.x, blockIdx.y), the CTAs of blockIdx.z
+// taking its rows in turn: a thread per split for the weights, then four
+// channels per thread and the splits over groups of threads, so that a row is
+// a few loads long (a warp per row: 14 us for 40 splits, this 8).
+constexpr int kAnyJoinThreads = 128;
 template <typename T, int KEYS>
-__global__ void __launch_bounds__(kAnyJoinWarps * 32) kv8_attn_join_kernel(AnyArgs g) {
-  __shared__ float s_w[kAnyJoinWarps][kMostSplits];
+__global__ void __launch_bounds__(kAnyJoinThreads) kv8_attn_join_kernel(AnyArgs g) {
+  __shared__ float s_w[kMostSplits], s_m[kAnyJoinThreads / 32], s_l[kAnyJoinThreads / 32];
+  __shared__ float4 s_o[kAnyJoinThreads];
   const AttnArgs& a = g.a;
-  const int dim = a.c.dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int dim = a.c.dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int kvh = blockIdx.y / g.chunks, chunk = blockIdx.y - kvh * g.chunks;
   const int h0 = kvh * a.group + chunk * g.head_chunk;
   const int nh = min(g.head_chunk, a.group - chunk * g.head_chunk);
@@ -301,28 +305,49 @@ __global__ void __launch_bounds__(kAnyJoinWarps * 32) kv8_attn_join_kernel(AnyAr
   const int splits = (int)((L + stretch - 1) / stretch);
   const int64_t record = any_record(g.rows, dim);
   const float* rec = a.part + ((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * g.splits * record;
-  for (int r = warp; r < (int)tokens * nh; r += kAnyJoinWarps) {
+  int pieces = 2;  // of four channels, to a power of two
+  while (pieces * 4 < dim) pieces *= 2;
+  const int piece = tid & (pieces - 1), group = tid / pieces, groups = kAnyJoinThreads / pieces;
+  for (int r = blockIdx.z; r < (int)tokens * nh; r += gridDim.z) {
     float m = -INFINITY, l = 0.f;
-    for (int s = lane; s < splits; s += 32) m = fmaxf(m, rec[s * record + 2 * r]);
+    for (int s = tid; s < splits; s += kAnyJoinThreads) m = fmaxf(m, rec[s * record + 2 * r]);
     m = warp_max(m);
+    if (lane == 0) s_m[warp] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
     const float base = m == -INFINITY ? 0.f : m;
-    __syncwarp();
-    for (int s = lane; s < splits; s += 32) {
+    for (int s = tid; s < splits; s += kAnyJoinThreads) {
       const float w = exp2f(rec[s * record + 2 * r] - base);
-      s_w[warp][s] = w;
+      s_w[s] = w;
       l = fmaf(w, rec[s * record + 2 * r + 1], l);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    __syncwarp();
-    T* out = static_cast<T*>(a.out) + (row0 + r / nh) * a.out_stride + (int64_t)(h0 + r % nh) * dim;
-    for (int d = lane; d < dim; d += 32) {
-      const float* p = rec + 2 * g.rows + r * dim + d;
-      float o = 0.f;
+    if (lane == 0) s_l[warp] = l;
+    __syncthreads();
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (piece * 4 < dim) {
+      const float* p = rec + 2 * g.rows + r * dim + piece * 4;
 #pragma unroll 8
-      for (int s = 0; s < splits; ++s) o = fmaf(s_w[warp][s], p[s * record], o);
-      Elem<T>::store(out + d, l == 0.f ? 0.f : o / l);
+      for (int s = group; s < splits; s += groups) {
+        const float4 v = *reinterpret_cast<const float4*>(p + s * record);
+        const float w = s_w[s];
+        o.x = fmaf(w, v.x, o.x), o.y = fmaf(w, v.y, o.y), o.z = fmaf(w, v.z, o.z), o.w = fmaf(w, v.w, o.w);
+      }
     }
+    s_o[tid] = o;
+    __syncthreads();
+    if (group == 0 && piece * 4 < dim) {
+      for (int k = 1; k < groups; ++k) {
+        const float4 v = s_o[k * pieces + piece];
+        o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
+      }
+      const float sum = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]), x[4] = {o.x, o.y, o.z, o.w};
+      T* out = static_cast<T*>(a.out) + (row0 + r / nh) * a.out_stride + (int64_t)(h0 + r % nh) * dim + piece * 4;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) Elem<T>::store(out + e, sum == 0.f ? 0.f : x[e] / sum);
+    }
+    __syncthreads();  // the next row's numbers go to the same places
   }
 }
 
@@ -361,7 +386,9 @@ int launch_any(const AnyArgs& g, int64_t tiles, cudaStream_t s) {
   const dim3 grid((unsigned)tiles, g.a.c.kv_heads * g.chunks, g.splits);
   rc = launch_pdl(kv8_attn_any_kernel<T, KEYS, ROWS>, grid, dim3(kAnyThreads), smem, s, g);
   if (rc != QQ_OK || g.splits == 1) return rc;
-  return launch_pdl(kv8_attn_join_kernel<T, KEYS>, dim3(grid.x, grid.y), dim3(kAnyJoinWarps * 32), 0, s, g);
+  const int64_t units = tiles * grid.y, per = 4 * (int64_t)device_sm_count() / units;  // CTAs to a unit
+  const unsigned z = (unsigned)std::max<int64_t>(1, std::min<int64_t>(per, g.rows));
+  return launch_pdl(kv8_attn_join_kernel<T, KEYS>, dim3(grid.x, grid.y, z), dim3(kAnyJoinThreads), 0, s, g);
 }
 template <typename T>
 int launch_any(const AnyArgs& g, int keys, int64_t tiles, cudaStream_t s) {
