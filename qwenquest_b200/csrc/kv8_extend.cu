@@ -175,16 +175,6 @@ __device__ __forceinline__ f32x2 add2(f32x2 x, f32x2 y) {
 struct Units {
   int tiles, whole, splits;
 };
-__device__ __forceinline__ Units units_of(const ExtendArgs& g, uint32_t* err) {
-  const int64_t tiles = extend_tiles(g.a, kUnitRows, g.a.group, err);
-  if (tiles > g.tiles) raise_error(err, QQ_DEV_ERR_BOUNDS);  // entries share query rows
-  Units x;
-  x.tiles = (int)min(tiles, (int64_t)g.tiles);
-  const int all = x.tiles * g.a.c.kv_heads, rest = all % g.sms;
-  x.splits = rest == 0 ? 1 : min(g.most, g.sms / rest);
-  x.whole = x.splits == 1 ? all : all - rest;
-  return x;
-}
 
 // A unit or a stretch of one (all within 32 bits: at most 65535 tiles of 256
 // rows, and positions of a table of less than 2^31 tokens).
@@ -199,30 +189,68 @@ struct Unit {
   int tiles;
   const int32_t* table;    // the request's blocks
 };
-// Unit `index`, its stretch `split`; called by one whole warp.
-__device__ __forceinline__ Unit unit_of(const ExtendArgs& g, const Units& all_units, int index, int split) {
+// The unit that choose(units, index, split) names; called by one whole warp.  A
+// batch of up to 32 entries is read once.
+template <typename Choose>
+__device__ __forceinline__ Unit find_unit(const ExtendArgs& g, uint32_t* err, Choose choose) {
   const AttnArgs& a = g.a;
+  const int lane = threadIdx.x & 31;
+  int64_t row0 = 0, pre = 0;
+  auto tiles_of = [&](int e, int& n, uint32_t* report) {
+    n = (int)extend_entry(a, e, row0, pre, report);
+    return (n * a.group + kUnitRows - 1) / kUnitRows;
+  };
+  int n, mine = tiles_of(lane, n, err), all = mine;
+  for (int e = lane + 32; e < a.bs; e += 32) {
+    int other;
+    all += tiles_of(e, other, err);
+  }
+  all = __reduce_add_sync(0xffffffffu, all);
+  if (all > g.tiles) raise_error(err, QQ_DEV_ERR_BOUNDS);  // entries share query rows
+  Units units;
+  units.tiles = min(all, g.tiles);
+  const int total = units.tiles * a.c.kv_heads, rest = total % g.sms;
+  units.splits = rest == 0 ? 1 : min(g.most, g.sms / rest);
+  units.whole = units.splits == 1 ? total : total - rest;
+  int index = 0, split = 0;
+  choose(units, index, split);
   Unit u{};
   u.entry = -1;
-  const int tile = index / a.c.kv_heads;
-  if (tile >= all_units.tiles) return u;
-  const ExtendEntry x = extend_tile(a, all_units.tiles - 1 - tile, kUnitRows, a.group, nullptr);
-  if (x.entry < 0) return u;
-  u.kvh = index - tile * a.c.kv_heads;
-  u.q_row = (int)x.row0;
-  u.prefix = (int)x.prefix;
-  u.row0 = (int)x.tile * kUnitRows;
-  u.rows = min(kUnitRows, (int)x.n * a.group - u.row0);
-  u.table = a.table + a.reqs[x.entry] * a.table_stride;
-  const int keys = u.prefix + (u.row0 + u.rows - 1) / a.group + 1;  // what its last row sees
-  const int all = (keys + kN - 1) / kN;
-  const int cuts = index < all_units.whole ? 1 : min(all_units.splits, (all + 3) / 4), each = (all + cuts - 1) / cuts;
-  u.splits = (all + each - 1) / each;
-  if (split >= u.splits) return u;
-  u.entry = x.entry;
-  u.key_begin = split * each * kN;
-  u.key_end = min(keys, u.key_begin + each * kN);
-  u.tiles = (u.key_end - u.key_begin + kN - 1) / kN;
+  const int back = index / a.c.kv_heads, tile = units.tiles - 1 - back;
+  if (tile < 0) return u;
+  int before = 0;
+  for (int e0 = 0; e0 < a.bs; e0 += 32) {
+    if (a.bs > 32) mine = tiles_of(e0 + lane, n, nullptr);
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
+    }
+    const int excl = before + incl - mine;
+    const uint32_t m = __ballot_sync(0xffffffffu, tile >= excl && tile < excl + mine);
+    if (m == 0) {
+      before += __shfl_sync(0xffffffffu, incl, 31);
+      continue;
+    }
+    const int src = __ffs(m) - 1, entry = e0 + src;
+    u.kvh = index - back * a.c.kv_heads;
+    u.q_row = (int)__shfl_sync(0xffffffffu, row0, src);
+    u.prefix = (int)__shfl_sync(0xffffffffu, pre, src);
+    u.row0 = (tile - __shfl_sync(0xffffffffu, excl, src)) * kUnitRows;
+    u.rows = min(kUnitRows, __shfl_sync(0xffffffffu, n, src) * a.group - u.row0);
+    u.table = a.table + a.reqs[entry] * a.table_stride;
+    const int keys = u.prefix + (u.row0 + u.rows - 1) / a.group + 1;  // what its last row sees
+    const int key_tiles = (keys + kN - 1) / kN;
+    const int cuts = index < units.whole ? 1 : min(units.splits, (key_tiles + 3) / 4), each = (key_tiles + cuts - 1) / cuts;
+    u.splits = (key_tiles + each - 1) / each;
+    if (split >= u.splits) return u;
+    u.entry = entry;
+    u.key_begin = split * each * kN;
+    u.key_end = min(keys, u.key_begin + each * kN);
+    u.tiles = (u.key_end - u.key_begin + kN - 1) / kN;
+    return u;
+  }
   return u;
 }
 
@@ -250,9 +278,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
   allow_next_grid();
 
   if (warp == 0) {
-    const Units units = units_of(g, blockIdx.x == 0 ? a.err : nullptr);
-    const int id = blockIdx.x, cut = max(0, id - units.whole);
-    const Unit u = unit_of(g, units, min(id, units.whole) + cut / units.splits, cut % units.splits);
+    int cut = 0;
+    const Unit u = find_unit(g, blockIdx.x == 0 ? a.err : nullptr, [&](const Units& units, int& index, int& split) {
+      cut = max(0, (int)blockIdx.x - units.whole);
+      index = min((int)blockIdx.x, units.whole) + cut / units.splits;
+      split = cut % units.splits;
+    });
     if (lane == 0) s_unit = u, s_record = cut;
   }
   if (threadIdx.x == 32) {
@@ -279,15 +310,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
     mbar_init(bar(kBarLag + 1), 4);
     mbar_init_fence();
   }
-  __syncthreads();
-  const Unit& u = s_unit;
-  if (u.entry < 0) return;  // past the last unit, uniform
-  const int kvh = u.kvh;
   if (warp == kMmaWarp) tmem_alloc(smem_u32(&s_tmem), kTmemCols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  const Unit& u = s_unit;
+  const int kvh = u.kvh;
   const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
+  if (u.entry < 0) {  // past the last unit, uniform
+    if (warp == kMmaWarp) tmem_dealloc(tmem, kTmemCols);
+    return;
+  }
   const int tiles = __shfl_sync(0xffffffffu, u.tiles, 0);
 
   if (warp < kWidenWarp) {
@@ -295,51 +328,55 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
     // ================================================================ softmax (warps 0-7)
     const int h = warp >> 2, r = threadIdx.x;      // row of the CTA's 256
     const int token = (u.row0 + r) / a.group;
-    // ---- this warp's 32 query rows to fp16: four lanes per row, 32 channels each;
-    // the next eight rows are on their way meanwhile
-    uint4 ask[4];
-    auto query = [&](int r0) {
-      const int rr = warp * 32 + r0 + (lane >> 2);
-      const bool there = r0 < 32 && rr < u.rows;
+    // ---- this warp's 32 query rows to fp16: four lanes per row, 32 channels
+    // each, all of it asked for at once
+    uint4 ask[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int rr = warp * 32 + i * 8 + (lane >> 2);
       const int t = (u.row0 + rr) / a.group, hd = kvh * a.group + u.row0 + rr - t * a.group;
       const uint4* q = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) +
-                                                      (int64_t)(u.q_row + t) * a.q_stride + (int64_t)hd * kTcDim + (lane & 3) * 32);
+                                                      (int64_t)(u.q_row + t) * a.q_stride + (int64_t)hd * kTcDim +
+                                                      (lane & 3) * 32);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) ask[k] = load16_or_zero(q + k, there);
-    };
-    query(0);
-#pragma unroll 1
-    for (int r0 = 0; r0 < 32; r0 += 8) {
-      const int rr = warp * 32 + r0 + (lane >> 2);
-      float x[32];
+      for (int k = 0; k < 4; ++k) ask[i][k] = load16_or_zero(q + k, rr < u.rows);
+    }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t v[4] = {ask[k].x, ask[k].y, ask[k].z, ask[k].w};
+    for (int i = 0; i < 4; ++i) {
+      const int rr = warp * 32 + i * 8 + (lane >> 2);
+      uint32_t w[16];
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
-          x[8 * k + 2 * b] = __uint_as_float(v[b] << 16), x[8 * k + 2 * b + 1] = __uint_as_float(v[b] & 0xFFFF0000u);
+      for (int k = 0; k < 4; ++k) w[4 * k] = ask[i][k].x, w[4 * k + 1] = ask[i][k].y, w[4 * k + 2] = ask[i][k].z, w[4 * k + 3] = ask[i][k].w;
+      // magnitudes compare as integers
+      auto largest = [&]() {
+        uint32_t top = 0;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) top = __vmaxu2(top, w[k] & 0x7FFF7FFFu);
+        return max(top & 0xFFFF0000u, top << 16);
+      };
+      uint32_t most = largest();
+      if (most >= 0x7F800000u) {
+        // an infinite query has no scores either: NaN, and left out of the maximum
+        uint32_t top = 0;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          uint32_t fine = w[k] & 0x7FFF7FFFu;
+          if ((w[k] & 0x7F80u) == 0x7F80u) w[k] |= 0x7FFFu, fine &= 0xFFFF0000u;
+          if ((w[k] & 0x7F800000u) == 0x7F800000u) w[k] |= 0x7FFF0000u, fine &= 0xFFFFu;
+          top = __vmaxu2(top, fine);
+        }
+        most = max(top & 0xFFFF0000u, top << 16);
       }
-      query(r0 + 8);
-      float most = 0.f;
-#pragma unroll
-      for (int k = 0; k < 32; ++k) {
-        const bool finite = fabsf(x[k]) <= 3.402823466e38f;
-        if (finite) most = fmaxf(most, fabsf(x[k]));
-        else x[k] = __uint_as_float(0x7FFFFFFFu);  // an infinite query has no scores either
-      }
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-      const int k2 = max(-120, fit_exponent(most) - 1);  // at most 224
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      const int k2 = max(-120, fit_exponent(__uint_as_float(most)) - 1);  // at most 224
       const float up = a.scale_log2 < 0.f ? -exp2_int(k2) : exp2_int(k2);
       uint8_t* dst = smem + kOffQ + h * kTileBytes + (lane & 2) / 2 * kHalf + (rr & 127) * 128;
+      auto scaled = [&](uint32_t x) { return pack_f16(__uint_as_float(x << 16) * up, __uint_as_float(x & 0xFFFF0000u) * up); };
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int piece = (lane & 1) * 4 + k;
-        const float* y = x + 8 * k;
-        *reinterpret_cast<uint4*>(dst + ((piece ^ (rr & 7)) << 4)) =
-            make_uint4(pack_f16(y[0] * up, y[1] * up), pack_f16(y[2] * up, y[3] * up),
-                       pack_f16(y[4] * up, y[5] * up), pack_f16(y[6] * up, y[7] * up));
-      }
+      for (int k = 0; k < 4; ++k)
+        *reinterpret_cast<uint4*>(dst + ((((lane & 1) * 4 + k) ^ (rr & 7)) << 4)) =
+            make_uint4(scaled(w[4 * k]), scaled(w[4 * k + 1]), scaled(w[4 * k + 2]), scaled(w[4 * k + 3]));
       if ((lane & 3) == 0) s_up[rr] = fabsf(a.scale_log2) * exp2_int(-k2);
     }
     fence_async_shared();
@@ -528,6 +565,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
       }
       if (!record && part == 0) continue;
       __syncwarp();
+      const int first = u.row0 + warp * 32 + (lane >> 4);
+      int t = first / a.group, hd = first - t * a.group;  // of the row at hand
 #pragma unroll 4
       for (int k = 0; k < 16; ++k) {  // two rows at a time
         const int row = 2 * k + (lane >> 4), rr = warp * 32 + row;
@@ -536,9 +575,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
         if (record) {
           *reinterpret_cast<uint4*>(rec + 2 * kUnitRows + (int64_t)rr * kTcDim + part * 64 + (lane & 15) * 4) = w;
         } else {
-          const int t = (u.row0 + rr) / a.group, hd = kvh * a.group + u.row0 + rr - t * a.group;
           *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + (int64_t)(u.q_row + t) * a.out_stride +
-                                    (int64_t)hd * kTcDim + (lane & 15) * 8) = w;
+                                    (int64_t)(kvh * a.group + hd) * kTcDim + (lane & 15) * 8) = w;
+          for (hd += 2; hd >= a.group; hd -= a.group) ++t;
         }
       }
       __syncwarp();
@@ -710,11 +749,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv8_extend_join_kernel(Extend
   const AttnArgs& a = g.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 0) {
-    const Units units = units_of(g, nullptr);
-    Unit u{};
-    u.entry = -1;
-    if (units.splits > 1) u = unit_of(g, units, units.whole + blockIdx.x, 0);
-    if (lane == 0) s_unit = u, s_record = blockIdx.x * units.splits;
+    int record = 0;
+    const Unit u = find_unit(g, nullptr, [&](const Units& units, int& index, int&) {
+      record = blockIdx.x * units.splits;
+      index = units.whole + blockIdx.x;  // past the last one where none was cut
+    });
+    if (lane == 0) s_unit = u, s_record = record;
   }
   __syncthreads();
   wait_prior_grid();
