@@ -12,7 +12,7 @@
 // kernel joins.  One token per request is bound by the chain of a tile (table,
 // codes, scores, weights, product), so stretches go down to a tile and K and V
 // are asked for together (5 x up to 2500 keys of 2 heads of 64 for 8 query
-// heads: 17 us; 53 with 16 rows always, one tile in hand and stretches of four).
+// heads: 13.5 us; 53 with 16 rows always, one tile in hand and stretches of four).
 // An extend batch is bound by the fp32 FMAs and their shared-memory operands.
 
 #include <algorithm>

@@ -21,7 +21,7 @@
 // Tensor memory: per M tile S (128 fp32 columns, overlaid by P in fp16 once
 // read) and O (128).  The order per tile is S(j) P(j) O(j) S(j + 1): while
 // one tile's softmax runs the tensor cores work for the other.
-// The running maximum is raised only past a factor of 2^8; O is rescaled then.
+// The weights' reference is raised only past kRaiseAt; O is rescaled then.
 // Every wait is bounded; see the one-token kernel.
 
 #include <algorithm>
@@ -105,12 +105,6 @@ __device__ __forceinline__ void nan_of(uint32_t& acc, const uint4& h) {
       : "+r"(acc)
       : "r"(h.x), "r"(h.y), "r"(h.z), "r"(h.w), "r"(0));
 }
-__device__ __forceinline__ float max3(float x, float y, float z) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
-  return r;
-}
-
 // Loads under a predicate that leave their registers alone until they land (a
 // select behind a load would wait for it on the spot).
 __device__ __forceinline__ uint2 load8_or_zero(const void* p, bool there) {
@@ -170,7 +164,7 @@ __device__ __forceinline__ f32x2 add2(f32x2 x, f32x2 y) {
 // tiles from the last to the first, KV heads innermost.  SMs take a unit each at
 // a time, so the last units, which would leave SMs idle, are cut into `splits`
 // stretches of the keys, each of at least four key tiles (188 units of 35 to 47
-// key tiles on 148 SMs: 148 + 40 x 3 CTAs in 151 us; all whole 182, all cut in
+// key tiles on 148 SMs: 148 + 40 x 3 CTAs in 150 us; all whole 182, all cut in
 // two 175).  A batch with fewer units than SMs is cut throughout.
 struct Units {
   int tiles, whole, splits;
@@ -275,7 +269,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
   volatile int* abort_flag = &s_abort;
   auto wait = [&](int i, uint32_t parity) { return mbar_wait(bar(i), parity, abort_flag, a.err); };
   wait_prior_grid();
-  allow_next_grid();
 
   if (warp == 0) {
     int cut = 0;
@@ -314,6 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  allow_next_grid();  // not before the tensor memory is this CTA's
   const Unit& u = s_unit;
   const int kvh = u.kvh;
   const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
@@ -389,8 +383,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
     // The weights' reference m need not be the running maximum, only near
     // enough for fp16 (2^-24 to 2^16) and fp32: it starts as the maximum of the
     // first tile with a key, and is raised by log2 of a half tile's sum where
-    // that passes 2^kRaise, for the tiles to come.  So the scores are read
-    // once; a half whose sum passes 2^kMost (a weight might not fit fp16) is
+    // that passes kRaiseAt, for the tiles to come.  So the scores are read
+    // once; a half whose sum passes kMost (a weight might not fit fp16) is
     // made again from the tile's maximum.
     float m = -INFINITY, l = 0.f, alpha = 1.f;  // O still has to be multiplied by alpha
     bool ok = true;
@@ -403,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
       tc_fence_after();
       // columns c <= lim are seen by this row
       const int lim = max(-1, min(kN - 1, reach - j * kN));
-      const bool full = j * kN + kN - 1 <= sees;
+      const bool full = sees - j * kN >= kN - 1;
       uint32_t v[2][32];  // scores in chunks of 32 columns, the next one always on its way
       float part, sum;    // of the half in hand: what l takes, and the plain sum
       float most = 0.f;   // the larger of the halves' sums
