@@ -668,11 +668,11 @@ extern "C" int qq_block_plan(const qq_block_tables* tables, const int64_t* req_p
   const size_t smem = table_smem_bytes(bs);
   cudaStream_t s = as_stream(stream);
   if (num_slots <= kOneCtaSlots) {
-    if ((rc = one.ensure((const void*)block_plan_kernel<true, true>, smem)) != QQ_OK) return rc;
+    if ((rc = one.ensure((const void*)block_plan_kernel<true, true>, smem + kStaticSmem)) != QQ_OK) return rc;
     return launch_pdl(block_plan_kernel<true, true>, dim3(1), dim3(kTableThreads), smem, s, a);
   }
-  if ((rc = wide.ensure((const void*)block_plan_kernel<false, true>, smem)) != QQ_OK) return rc;
-  if ((rc = state.ensure((const void*)block_plan_kernel<true, false>, smem)) != QQ_OK) return rc;
+  if ((rc = wide.ensure((const void*)block_plan_kernel<false, true>, smem + kStaticSmem)) != QQ_OK) return rc;
+  if ((rc = state.ensure((const void*)block_plan_kernel<true, false>, smem + kStaticSmem)) != QQ_OK) return rc;
   const int64_t ctas = (num_slots + kTableThreads - 1) / kTableThreads;
   const int most = device_sm_count();
   rc = launch_pdl(block_plan_kernel<false, true>, dim3((unsigned)(ctas < most ? ctas : most)), dim3(kTableThreads), smem, s, a);
@@ -690,7 +690,7 @@ extern "C" int qq_block_trim(const qq_block_tables* tables, const int64_t* req_p
   a.seq = keep_lens;
   static SmemLimit limit;
   const size_t smem = table_smem_bytes(bs);
-  if ((rc = limit.ensure((const void*)block_trim_kernel, smem)) != QQ_OK) return rc;
+  if ((rc = limit.ensure((const void*)block_trim_kernel, smem + kStaticSmem)) != QQ_OK) return rc;
   return launch_pdl(block_trim_kernel, dim3(1), dim3(kTableThreads), smem, as_stream(stream), a);
 }
 

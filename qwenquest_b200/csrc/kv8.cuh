@@ -24,6 +24,10 @@ struct Cache {
   int shift;  // log2(block)
 };
 
+// The default limit of 48 KiB counts a kernel's own shared arrays too, so the
+// launches ask for this much more than their dynamic part.
+constexpr size_t kStaticSmem = 4096;
+
 inline Cache view(const qq_kv8_cache& c) {
   int shift = 0;
   while ((1 << shift) < c.block_size) ++shift;

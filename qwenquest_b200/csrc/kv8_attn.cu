@@ -381,7 +381,7 @@ template <typename T, int KEYS, int ROWS>
 int launch_any(const AnyArgs& g, int64_t tiles, cudaStream_t s) {
   static SmemLimit limit;
   const size_t smem = any_smem(g);
-  int rc = limit.ensure((const void*)kv8_attn_any_kernel<T, KEYS, ROWS>, smem);
+  int rc = limit.ensure((const void*)kv8_attn_any_kernel<T, KEYS, ROWS>, smem + kStaticSmem);
   if (rc != QQ_OK) return rc;
   const dim3 grid((unsigned)tiles, g.a.c.kv_heads * g.chunks, g.splits);
   rc = launch_pdl(kv8_attn_any_kernel<T, KEYS, ROWS>, grid, dim3(kAnyThreads), smem, s, g);

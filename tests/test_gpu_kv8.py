@@ -105,6 +105,18 @@ def test_plan_of_large_batches(bs):
         _assert_tables(tables, ref)
 
 
+@pytest.mark.parametrize("bs", [1735, 1745, 1754, 1755, 1760])
+def test_plan_and_trim_where_shared_memory_passes_48_kib(bs):
+    """The kernel's own shared arrays count towards the default limit as well."""
+    for new in (1, 3):
+        tables = BlockTables(bs, bs, 1, DEV, block_size=16)
+        slots, _ = tables.plan(torch.arange(bs), torch.full((bs,), new), torch.zeros(bs, dtype=torch.int64), bs * new)
+        assert slots.view(bs, new)[:, 0].tolist() == [16 * i for i in range(bs)]
+        tables.trim(torch.arange(bs))
+        tables.synchronize()
+        assert tables.available() == bs
+
+
 @pytest.mark.parametrize("big", [False, True])
 def test_plan_short_of_blocks_leaves_the_rest_as_it_was(big):
     """The entries behind the last free block get nothing, an entry that needs none is served."""
@@ -711,6 +723,22 @@ def test_results_do_not_depend_on_the_batch_or_the_call():
     first = b.cache.decode_attention(0, q, *args, b.scaling)
     again = b.cache.decode_attention(0, q, *args, b.scaling)
     assert torch.equal(first, again)
+
+
+@pytest.mark.parametrize("dim", [128, 136, 144])
+@pytest.mark.parametrize("heads", [3, 7, 12])
+def test_fp32_kernel_where_shared_memory_passes_48_kib(dim, heads):
+    seq, new = [70, 5], [20, 5]
+    b = _Batch(seq, 1, dim, 16, seed=dim + heads, heads=heads, dtype=torch.float32)
+    q = b.queries(25)
+    lens = _dev(b.reqs), _dev(seq)
+    out = b.cache.extend_attention(0, q.to(DEV), b.table_dev, *lens, _dev([50, 0]), _dev([0, 20]), b.scaling)
+    one = b.cache.decode_attention(0, q[:2].to(DEV), b.table_dev, *lens, b.scaling)
+    b.cache.synchronize()
+    b.check(out[19], q[19], b.slots(0, np.arange(70)), SMALL_EXTEND)
+    b.check(out[24], q[24], b.slots(1, np.arange(5)), SMALL_EXTEND)
+    for i in range(2):
+        b.check(one[i], q[i], b.slots(i, np.arange(seq[i])))
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
