@@ -19,12 +19,17 @@
 // Work: the tiles of all (request, KV head) pairs in a row, cut into equal
 // shares, one per CTA (two CTAs per SM); a pair cut by a share's edge leaves
 // (M, l, O) records that kv8_decode_join_kernel merges.
+// Few pairs of moderate length (a lone request, a selection) take the other
+// form: a cluster of 16, 8 or 4 CTAs to a pair, which joins its records through the
+// CTAs' shared memory and so needs no second launch.
 // Warps: 0-3 softmax, 4 TMA, 5 MMA issue, 6 queries, 7 scales.  The MMAs go
 // S(0) S(1) O(0) S(2) O(1) ...: the softmax of a tile runs while the next
 // tile's scores are made, and a tile's O is added in registers one tile later.
 // Every wait is bounded (kWaitLimitNs); on expiry the CTA reports
 // QQ_DEV_ERR_TIMEOUT, waits for its own copies and MMAs and returns.
 
+#include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cmath>
 
@@ -44,6 +49,7 @@ constexpr int kSoft = 128;                     // softmax threads
 constexpr int kThreads = 256;
 constexpr int kMeta = 4;                       // tiles of scales in flight
 constexpr int kMaxSlots = 12;
+constexpr int kClusterTiles = 4;              // tiles of each of them at most
 constexpr int kInv = 4;                        // pairs of which the softmax may not have seen the queries' scales
 constexpr uint32_t kMasked = 0xFFFFFFFFu;      // a V scale's bits where the token takes no part
 constexpr float kLo = 16.f;
@@ -206,7 +212,21 @@ __device__ __forceinline__ void write_query(const AttnArgs& a, int e, int h, int
   if (col == 0) qinv[r] = a.scale_log2 * exp2_int(-k2);
 }
 
-template <int KEYS, int HEADS>
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Word `addr` of the shared memory of the cluster's CTA `rank`.
+__device__ __forceinline__ float ld_cluster(uint32_t addr, int rank) {
+  float x;
+  asm volatile("{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}\n"
+               : "=f"(x)
+               : "r"(addr), "r"(rank)
+               : "memory");
+  return x;
+}
+
+// CLUSTER: a cluster of that many CTAs takes a pair and joins it itself.
+template <int KEYS, int HEADS, int CLUSTER>
 __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
     kv8_decode_kernel(const DecodeArgs g, const __grid_constant__ CUtensorMap map_k,
                       const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap row_k,
@@ -262,55 +282,72 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
   }
   if (warp == 5) tmem_alloc(smem_u32(&s_tmem), kTmemCols);
   wait_prior_grid();
-  const int per = (a.bs + kThreads - 1) / kThreads;
-  int64_t own, before, tiles;
-  sum_tiles<KEYS, kThreads>(a, per, own, before, tiles, blockIdx.x == 0 ? a.err : nullptr);
-  auto entry_tiles = [&](int j) {  // of this thread's entry j
-    return j == 0 ? own : (entry_keys<KEYS>(a, threadIdx.x * per + j, nullptr) + kTile - 1) / kTile;
-  };
-  const Shares shares(tiles * c.kv_heads, gridDim.x);
-  allow_next_grid();
-  if (blockIdx.x == 0) {
-    int64_t at = before;
-    for (int j = 0; j < per; ++j) {
-      const int e = threadIdx.x * per + j;
-      if (e >= a.bs) break;
-      g.before[e] = at;
-      at += entry_tiles(j);
-    }
-    if (threadIdx.x == 0) g.before[a.bs] = tiles;
-  }
-  const bool any = blockIdx.x < shares.ctas;
-  const int64_t lo = shares.lo(blockIdx.x);
-  {
-    int64_t at = before * c.kv_heads;
-    for (int j = 0; any && j < per; ++j) {
-      const int e = threadIdx.x * per + j;
-      if (e >= a.bs || at > lo) break;
-      const int T = (int)entry_tiles(j);
-      if (lo < at + (int64_t)T * c.kv_heads) {
-        int r = (int)(lo - at), h = 0;
-        if (r >= T) h = r / T, r -= h * T;
-        s_start[0] = e;
-        s_start[1] = h;
-        s_start[2] = r;
+  bool any = true;  // this CTA has tiles, `count` of them from s_start on
+  int count;
+  if constexpr (CLUSTER > 0) {
+    const int pair = blockIdx.x / CLUSTER, rank = blockIdx.x % CLUSTER, e = pair / c.kv_heads, h = pair - e * c.kv_heads;
+    const int64_t n = entry_keys<KEYS>(a, e, rank == 0 && h == 0 && threadIdx.x == 0 ? a.err : nullptr);
+    const int T = (int)((n + kTile - 1) / kTile), each = T / CLUSTER, more = T % CLUSTER;
+    count = each + (rank < more ? 1 : 0);
+    if (threadIdx.x == 0) s_start[0] = e, s_start[1] = h, s_start[2] = rank * each + min(rank, more);
+  } else {
+    const int per = (a.bs + kThreads - 1) / kThreads;
+    int64_t own, before, tiles;
+    sum_tiles<KEYS, kThreads>(a, per, own, before, tiles, blockIdx.x == 0 ? a.err : nullptr);
+    auto entry_tiles = [&](int j) {  // of this thread's entry j
+      return j == 0 ? own : (entry_keys<KEYS>(a, threadIdx.x * per + j, nullptr) + kTile - 1) / kTile;
+    };
+    const Shares shares(tiles * c.kv_heads, gridDim.x);
+    allow_next_grid();
+    if (blockIdx.x == 0) {
+      int64_t at = before;
+      for (int j = 0; j < per; ++j) {
+        const int e = threadIdx.x * per + j;
+        if (e >= a.bs) break;
+        g.before[e] = at;
+        at += entry_tiles(j);
       }
-      at += (int64_t)T * c.kv_heads;
+      if (threadIdx.x == 0) g.before[a.bs] = tiles;
+    }
+    any = blockIdx.x < shares.ctas;
+    const int64_t lo = shares.lo(blockIdx.x);
+    count = any ? (int)(shares.lo(blockIdx.x + 1) - lo) : 0;
+    {
+      int64_t at = before * c.kv_heads;
+      for (int j = 0; any && j < per; ++j) {
+        const int e = threadIdx.x * per + j;
+        if (e >= a.bs || at > lo) break;
+        const int T = (int)entry_tiles(j);
+        if (lo < at + (int64_t)T * c.kv_heads) {
+          int r = (int)(lo - at), h = 0;
+          if (r >= T) h = r / T, r -= h * T;
+          s_start[0] = e;
+          s_start[1] = h;
+          s_start[2] = r;
+        }
+        at += (int64_t)T * c.kv_heads;
+      }
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (CLUSTER > 0) allow_next_grid();
   if (!any) {  // uniform over the CTA
     if (warp == 5) tmem_dealloc(s_tmem, kTmemCols);
     return;
   }
   const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
-  const int count = (int)(shares.lo(blockIdx.x + 1) - lo);
+  count = __shfl_sync(0xffffffffu, count, 0);
   Walk<KEYS> w(a, s_start[0], s_start[1], s_start[2]);
   const int64_t pool_rows = (int64_t)c.num_blocks * c.kv_heads * c.block;
 
-  if (warp == 4) {
+  if (CLUSTER > 0 && count == 0) {
+    if (threadIdx.x < HEADS) {
+      reinterpret_cast<float*>(smem)[threadIdx.x] = -INFINITY;
+      reinterpret_cast<float*>(smem)[HEADS + threadIdx.x] = 0.f;
+    }
+  } else if (warp == 4) {
     // ================================================================ codes
     // the table entries or rows of a tile are loaded one tile ahead
     const int pages = kTile >> c.shift;
@@ -599,8 +636,10 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
       if (lane % (32 / HEADS) == 0) s_sum[lane / (32 / HEADS)][warp] = part;
       asm volatile("bar.sync 1, 128;" ::: "memory");
       if (ok) {
-        const bool whole = i >= w.t && first;  // all of the pair's tiles are this CTA's
-        float* rec = a.part + ((int64_t)blockIdx.x * 2 + (pair > 0)) * record_floats(HEADS);
+        const bool whole = CLUSTER == 0 && i >= w.t && first;  // all of the pair's tiles are this CTA's
+        // in a cluster over the first codes: all copies and products are done
+        float* rec = CLUSTER > 0 ? reinterpret_cast<float*>(smem)
+                             : a.part + ((int64_t)blockIdx.x * 2 + (pair > 0)) * record_floats(HEADS);
 #pragma unroll
         for (int r = 0; r < HEADS; ++r) {
           const float4 l4 = *reinterpret_cast<const float4*>(s_sum[r]);
@@ -624,6 +663,45 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
   if (warp == 5) {
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
+  }
+  if constexpr (CLUSTER > 0) {
+    // ---- the pair's outputs in equal parts, four threads per output, each with its part of the records
+    constexpr int kOuts = HEADS * kTcDim / CLUSTER, kRecords = CLUSTER / 4;
+    cluster_sync();
+    const int rank = blockIdx.x % CLUSTER, part = threadIdx.x & 3;
+#pragma unroll
+    for (int it = 0; it < kOuts / (kThreads / 4); ++it) {
+      const int i = rank * kOuts + it * (kThreads / 4) + (threadIdx.x >> 2), r = i / kTcDim, ch = i % kTcDim;
+      float m[kRecords], l[kRecords], o[kRecords];
+#pragma unroll
+      for (int k = 0; k < kRecords; ++k) {
+        m[k] = ld_cluster(base + r * 4, part * kRecords + k);
+        l[k] = ld_cluster(base + (HEADS + r) * 4, part * kRecords + k);
+        o[k] = ld_cluster(base + (2 * HEADS + r * kTcDim + ch) * 4, part * kRecords + k);
+      }
+      float mn = m[0];
+#pragma unroll
+      for (int k = 1; k < kRecords; ++k) mn = fmaxf(mn, m[k]);
+      mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 1));
+      mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 2));
+      const float ref = mn == -INFINITY ? 0.f : mn;
+      float sum = 0.f, x = 0.f;
+#pragma unroll
+      for (int k = 0; k < kRecords; ++k) {
+        const float f = ex2(m[k] - ref);
+        sum = fmaf(f, l[k], sum);
+        if (m[k] != -INFINITY) x = fmaf(f, o[k], x);  // a CTA without tiles left no outputs
+      }
+#pragma unroll
+      for (int d = 1; d < 4; d <<= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        x += __shfl_xor_sync(0xffffffffu, x, d);
+      }
+      if (part == 0 && r < a.group)
+        static_cast<__nv_bfloat16*>(a.out)[(int64_t)s_start[0] * a.out_stride + (int64_t)(s_start[1] * a.group + r) * kTcDim + ch] =
+            __float2bfloat16_rn(sum == 0.f ? 0.f : x / sum);
+    }
+    cluster_sync();  // the records stay until all have read them
   }
 }
 
@@ -717,32 +795,130 @@ __global__ void __launch_bounds__(32 * join_warps(SPLIT)) kv8_decode_join_kernel
 }
 
 template <int KEYS, int HEADS>
-int launch(DecodeArgs g, int64_t ctas, cudaStream_t s) {
-  constexpr int fixed = 1024 + 4 * 2 * HEADS * 128;
-  constexpr int slots = HEADS == 8 ? 6 : 10;  // two CTAs per SM of the 16-column kernel share its 228 KiB
-  static_assert(slots >= 4 && slots <= kMaxSlots, "ring");
-  g.slots = slots;
-  const size_t smem = fixed + slots * kSlotBytes;
-  static SmemLimit limit;
-  int rc = limit.ensure((const void*)kv8_decode_kernel<KEYS, HEADS>, smem);
-  if (rc != QQ_OK) return rc;
+constexpr int ring_slots() {
+  return HEADS == 8 ? 6 : 10;  // two CTAs per SM of the 16-column kernel share its 228 KiB
+}
+template <int KEYS, int HEADS>
+constexpr size_t decode_smem() {
+  return 1024 + 4 * 2 * HEADS * 128 + ring_slots<KEYS, HEADS>() * kSlotBytes;
+}
+
+struct Maps {
   CUtensorMap mk, mv, rk, rv;
-  const int64_t rows = (int64_t)g.a.c.num_blocks * g.a.c.kv_heads * g.a.c.block;
-  const int box = KEYS == kTable ? g.a.c.block : 16;
-  if ((rc = encode_rows(&mk, g.a.c.k, rows, box)) != QQ_OK) return rc;
-  if ((rc = encode_rows(&mv, g.a.c.v, rows, box)) != QQ_OK) return rc;
+};
+template <int KEYS>
+int encode_maps(const Cache& c, Maps& m) {
+  const int64_t rows = (int64_t)c.num_blocks * c.kv_heads * c.block;
+  const int box = KEYS == kTable ? c.block : 16;
+  int rc;
+  if ((rc = encode_rows(&m.mk, c.k, rows, box)) != QQ_OK) return rc;
+  if ((rc = encode_rows(&m.mv, c.v, rows, box)) != QQ_OK) return rc;
   if (KEYS == kRows) {
-    if ((rc = encode_rows(&rk, g.a.c.k, rows, 1)) != QQ_OK) return rc;
-    if ((rc = encode_rows(&rv, g.a.c.v, rows, 1)) != QQ_OK) return rc;
-  } else {
-    rk = mk, rv = mv;  // not read
+    if ((rc = encode_rows(&m.rk, c.k, rows, 1)) != QQ_OK) return rc;
+    return encode_rows(&m.rv, c.v, rows, 1);
   }
-  rc = launch_pdl(kv8_decode_kernel<KEYS, HEADS>, dim3((unsigned)ctas), dim3(kThreads), smem, s, g, mk, mv, rk, rv);
+  m.rk = m.mk, m.rv = m.mv;  // not read
+  return QQ_OK;
+}
+
+template <int KEYS, int HEADS>
+int launch(DecodeArgs g, int64_t ctas, cudaStream_t s) {
+  static_assert(ring_slots<KEYS, HEADS>() >= 4 && ring_slots<KEYS, HEADS>() <= kMaxSlots, "ring");
+  g.slots = ring_slots<KEYS, HEADS>();
+  constexpr size_t smem = decode_smem<KEYS, HEADS>();
+  static SmemLimit limit;
+  int rc = limit.ensure((const void*)kv8_decode_kernel<KEYS, HEADS, 0>, smem);
+  if (rc != QQ_OK) return rc;
+  Maps m;
+  if ((rc = encode_maps<KEYS>(g.a.c, m)) != QQ_OK) return rc;
+  rc = launch_pdl(kv8_decode_kernel<KEYS, HEADS, 0>, dim3((unsigned)ctas), dim3(kThreads), smem, s, g, m.mk, m.mv, m.rk,
+                  m.rv);
   if (rc != QQ_OK) return rc;
   const int pairs = g.a.bs * g.a.c.kv_heads;
   if (ctas >= 4 * (int64_t)pairs)
-    return launch_pdl(kv8_decode_join_kernel<HEADS, true>, dim3(g.a.bs, g.a.heads), dim3(32 * join_warps(true)), 0, s, g, ctas);
-  return launch_pdl(kv8_decode_join_kernel<HEADS, false>, dim3(g.a.bs, g.a.c.kv_heads), dim3(32 * join_warps(false)), 0, s, g, ctas);
+    return launch_pdl(kv8_decode_join_kernel<HEADS, true>, dim3(g.a.bs, g.a.heads), dim3(32 * join_warps(true)), 0, s, g,
+                      ctas);
+  return launch_pdl(kv8_decode_join_kernel<HEADS, false>, dim3(g.a.bs, g.a.c.kv_heads), dim3(32 * join_warps(false)), 0, s,
+                    g, ctas);
+}
+
+// The launch of `pairs` clusters.
+struct ClusterLaunch {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  ClusterLaunch(int pairs, int cluster, size_t smem, cudaStream_t s) {
+    cfg.gridDim = dim3(pairs * cluster);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  }
+};
+
+// How many clusters of the kernel the current device holds at a time (0: none), asked once per device.
+template <int KEYS, int HEADS, int CLUSTER>
+int resident_clusters() {
+  static std::atomic<int> known[kMaxDevices];  // one more than the number
+  const int d = current_device();
+  if (d < 0 || d >= kMaxDevices) return 0;
+  int n = known[d].load(std::memory_order_acquire);
+  if (n > 0) return n - 1;
+  constexpr size_t smem = decode_smem<KEYS, HEADS>();
+  const void* kernel = (const void*)kv8_decode_kernel<KEYS, HEADS, CLUSTER>;
+  n = 0;
+  ClusterLaunch l(1, CLUSTER, smem, nullptr);
+  l.cfg.numAttrs = 1;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kernel, &l.cfg) != cudaSuccess) {
+    cudaGetLastError();
+    n = 0;
+  }
+  known[d].store(n + 1, std::memory_order_release);
+  return n;
+}
+
+template <int KEYS, int HEADS, int CLUSTER>
+int launch_clusters(DecodeArgs g, cudaStream_t s) {
+  g.slots = ring_slots<KEYS, HEADS>();
+  Maps m;
+  const int rc = encode_maps<KEYS>(g.a.c, m);
+  if (rc != QQ_OK) return rc;
+  ClusterLaunch l(g.a.bs * g.a.c.kv_heads, CLUSTER, decode_smem<KEYS, HEADS>(), s);
+  return cudaLaunchKernelEx(&l.cfg, kv8_decode_kernel<KEYS, HEADS, CLUSTER>, g, m.mk, m.mv, m.rk, m.rv) == cudaSuccess
+             ? QQ_OK
+             : QQ_ERR_CUDA;
+}
+
+// The cluster a call goes by, 0: shares and a join.  All clusters run at a
+// time, and no CTA has more than kClusterTiles tiles.  On the device (group 8,
+// 4 KV heads) 1 x 2,048 keys take 7.7 us where shares and a join take 9.4, 1 x
+// 8,192 10.6 and 11.9, 3 x 2,048 9.1 and 11.0, 8 x 2,048 12.2 and 12.9; with
+// eight tiles to a CTA 2 x 8,192 would take 13.8 and 13.3.
+template <int CLUSTER>
+bool cluster_fits(int64_t pairs, int group, int64_t max_keys) {
+  if (max_keys > (int64_t)CLUSTER * kClusterTiles * kTile) return false;
+  return pairs <= (group <= 8 ? std::min(resident_clusters<kTable, 8, CLUSTER>(), resident_clusters<kRows, 8, CLUSTER>())
+                              : std::min(resident_clusters<kTable, 16, CLUSTER>(), resident_clusters<kRows, 16, CLUSTER>()));
+}
+int cluster_of(int bs, int kv_heads, int group, int64_t max_keys) {
+  const int64_t pairs = (int64_t)bs * kv_heads;
+  if (pairs > device_sm_count()) return 0;
+  return cluster_fits<16>(pairs, group, max_keys)  ? 16
+         : cluster_fits<8>(pairs, group, max_keys) ? 8
+         : cluster_fits<4>(pairs, group, max_keys) ? 4
+                                                   : 0;
+}
+template <int CLUSTER>
+int run_clusters(const DecodeArgs& g, int keys, cudaStream_t s) {
+  if (g.a.group <= 8) return keys == kTable ? launch_clusters<kTable, 8, CLUSTER>(g, s) : launch_clusters<kRows, 8, CLUSTER>(g, s);
+  return keys == kTable ? launch_clusters<kTable, 16, CLUSTER>(g, s) : launch_clusters<kRows, 16, CLUSTER>(g, s);
 }
 
 int64_t decode_ctas(int bs, int kv_heads, int group, int64_t max_keys) {
@@ -760,14 +936,17 @@ bool decode_tc_fits(const AttnArgs& a, int dtype) {
 }
 
 size_t decode_tc_workspace(int bs, int kv_heads, int group, int64_t max_keys) {
+  if (cluster_of(bs, kv_heads, group, max_keys) > 0) return 0;
   return sizeof(float) * (size_t)(decode_ctas(bs, kv_heads, group, max_keys) * 2 * record_floats(group <= 8 ? 8 : 16)) +
          sizeof(int64_t) * (size_t)(bs + 1);
 }
 
 int run_decode_tc(const AttnArgs& a, int keys, int64_t max_keys, size_t ws_bytes, cudaStream_t s) {
-  if (a.part == nullptr || ws_bytes < decode_tc_workspace(a.bs, a.c.kv_heads, a.group, max_keys)) return QQ_ERR_WORKSPACE;
   DecodeArgs g{};
   g.a = a;
+  const int cluster = cluster_of(a.bs, a.c.kv_heads, a.group, max_keys);
+  if (cluster > 0) return cluster == 16 ? run_clusters<16>(g, keys, s) : cluster == 8 ? run_clusters<8>(g, keys, s) : run_clusters<4>(g, keys, s);
+  if (a.part == nullptr || ws_bytes < decode_tc_workspace(a.bs, a.c.kv_heads, a.group, max_keys)) return QQ_ERR_WORKSPACE;
   const int64_t ctas = decode_ctas(a.bs, a.c.kv_heads, a.group, max_keys);
   g.before = reinterpret_cast<int64_t*>(a.part + ctas * 2 * record_floats(a.group <= 8 ? 8 : 16));
   if (a.group <= 8) return keys == kTable ? launch<kTable, 8>(g, ctas, s) : launch<kRows, 8>(g, ctas, s);
