@@ -9,7 +9,7 @@
 // `splits` equal stretches of their keys; tiles of 64 keys are dequantised to
 // fp32 in shared memory once for all rows.  The maximum m and the sum run along
 // with the tiles; split stretches leave (m, sum, O) records that a second
-// kernel joins.  One token per request is bound by the chain of a tile (table,
+// kernel joins, or are a cluster that joins them itself.  One token per request is bound by the chain of a tile (table,
 // codes, scores, weights, product), so stretches go down to a tile and K and V
 // are asked for together (5 x up to 2500 keys of 2 heads of 64 for 8 query
 // heads: 13.5 us; 53 with 16 rows always, one tile in hand and stretches of four).
@@ -42,6 +42,7 @@ struct AnyArgs {
   int tile_tokens;  // query tokens per CTA
   int key_groups;   // the product's threads: key groups x channels
   int splits;
+  int cluster;      // CTAs of a cluster that take a unit's splits and join them, 0: records and a join
 };
 
 // Records of a unit (row tile, KV head, head chunk) and split: rows x (m, l), then rows x dim.
@@ -63,7 +64,8 @@ __device__ __forceinline__ int64_t stretch_keys(int64_t keys, int splits) {
   return ((keys + kTileKeys - 1) / kTileKeys + splits - 1) / splits * kTileKeys;
 }
 
-template <typename T, int KEYS, int ROWS>
+// CLUSTER: the splits of a unit are a cluster, which joins them itself.
+template <typename T, int KEYS, int ROWS, bool CLUSTER>
 __global__ void __launch_bounds__(kAnyThreads) kv8_attn_any_kernel(AnyArgs g) {
   constexpr bool kBoth = any_both(ROWS);
   extern __shared__ __align__(16) float s_buf[];
@@ -104,7 +106,7 @@ __global__ void __launch_bounds__(kAnyThreads) kv8_attn_any_kernel(AnyArgs g) {
   const int64_t req = KEYS == kRows ? 0 : (L > 0 ? a.reqs[e] : 0);
   const int64_t stretch = stretch_keys(L, g.splits);
   const int64_t k0 = blockIdx.z * stretch, k1 = min(L, k0 + stretch);
-  if (k0 >= k1 && blockIdx.z > 0) return;  // nothing left for this one, uniform
+  if (!CLUSTER && k0 >= k1 && blockIdx.z > 0) return;  // nothing left for this one, uniform
 
   for (int i = tid; i < R * dim; i += kAnyThreads) {
     const int r = i / dim, d = i - r * dim;
@@ -244,26 +246,28 @@ __global__ void __launch_bounds__(kAnyThreads) kv8_attn_any_kernel(AnyArgs g) {
   }
   __syncthreads();
   float* rec = a.part + (((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * g.splits + blockIdx.z) * any_record(ROWS, dim);
-  const bool whole = stretch >= L;  // all keys are in this stretch
-  if (!whole && tid < R) rec[2 * tid] = s_m[tid], rec[2 * tid + 1] = s_l[tid];
+  const bool whole = !CLUSTER && stretch >= L;  // all keys are in this stretch
+  if (!CLUSTER && !whole && tid < R) rec[2 * tid] = s_m[tid], rec[2 * tid + 1] = s_l[tid];
   if (g.key_groups > 1) {  // the groups' sums meet in the first one's threads
     if (d0 < dim)
 #pragma unroll
       for (int r = 0; r < ROWS; ++r) s_k[(group * ROWS + r) * dim + d0] = acc[0][r];
     __syncthreads();
-    if (group > 0 || d0 >= dim) return;
+    if (!CLUSTER && (group > 0 || d0 >= dim)) return;
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r)
+    for (int r = 0; r < ROWS && d0 < dim; ++r)
       for (int k = 1; k < g.key_groups; ++k) acc[0][r] += s_k[(k * ROWS + r) * dim + d0];
   }
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int d = d0 + u * kAnyThreads;
-    if (d >= dim) break;
+    if (d >= dim || group > 0) break;
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
       if (r >= R) break;
-      if (whole) {
+      if (CLUSTER) {
+        s_q[r * dim + d] = acc[u][r];  // the queries have done their work
+      } else if (whole) {
         T* o = static_cast<T*>(a.out) + (row0 + r / nh) * a.out_stride + (int64_t)(h0 + r % nh) * dim;
         const float l = s_l[r];
         Elem<T>::store(o + d, l == 0.f ? 0.f : acc[u][r] / l);
@@ -271,6 +275,45 @@ __global__ void __launch_bounds__(kAnyThreads) kv8_attn_any_kernel(AnyArgs g) {
         rec[2 * ROWS + r * dim + d] = acc[u][r];
       }
     }
+  }
+  if constexpr (CLUSTER) {
+    // ---- four threads per output, each with its part of the records
+    __syncthreads();
+    cluster_sync();
+    const int outs = R * dim, part = tid & 3;
+    for (int i0 = blockIdx.z * (kAnyThreads / 4); i0 < outs; i0 += g.cluster * (kAnyThreads / 4)) {
+      const int i = min(i0 + (tid >> 2), outs - 1), r = i / dim;
+      float m[4], l[4], o[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int rank = part + 4 * k;
+        m[k] = -INFINITY, l[k] = 0.f, o[k] = 0.f;
+        if (rank >= g.cluster) continue;
+        m[k] = ld_cluster(smem_u32(s_m + r), rank);
+        l[k] = ld_cluster(smem_u32(s_l + r), rank);
+        o[k] = ld_cluster(smem_u32(s_q + i), rank);
+      }
+      float mn = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+      mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 1));
+      mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 2));
+      const float ref = mn == -INFINITY ? 0.f : mn;
+      float sum = 0.f, x = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float f = exp2f(m[k] - ref);
+        sum = fmaf(f, l[k], sum);
+        x = fmaf(f, o[k], x);
+      }
+#pragma unroll
+      for (int d = 1; d < 4; d <<= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        x += __shfl_xor_sync(0xffffffffu, x, d);
+      }
+      if (part == 0 && i0 + (tid >> 2) < outs)
+        Elem<T>::store(static_cast<T*>(a.out) + (row0 + r / nh) * a.out_stride + (int64_t)(h0 + r % nh) * dim + i - r * dim,
+                       sum == 0.f ? 0.f : x / sum);
+    }
+    cluster_sync();  // the records stay until all have read them
   }
 }
 
@@ -374,17 +417,23 @@ int any_splits(const AnyArgs& g, int64_t tiles, int kv_heads, int64_t max_keys) 
   return (int)(s < 1 ? 1 : (s > kMostSplits ? kMostSplits : s));
 }
 int64_t any_workspace(const AnyArgs& g, int64_t tiles) {
-  return g.splits == 1 ? 0 : (int64_t)sizeof(float) * tiles * g.a.c.kv_heads * g.chunks * g.splits * any_record(g.rows, g.a.c.dim);
+  return g.splits == 1 || g.cluster > 0 ? 0 : (int64_t)sizeof(float) * tiles * g.a.c.kv_heads * g.chunks * g.splits * any_record(g.rows, g.a.c.dim);
 }
 
 template <typename T, int KEYS, int ROWS>
 int launch_any(const AnyArgs& g, int64_t tiles, cudaStream_t s) {
-  static SmemLimit limit;
   const size_t smem = any_smem(g);
-  int rc = limit.ensure((const void*)kv8_attn_any_kernel<T, KEYS, ROWS>, smem + kStaticSmem);
-  if (rc != QQ_OK) return rc;
   const dim3 grid((unsigned)tiles, g.a.c.kv_heads * g.chunks, g.splits);
-  rc = launch_pdl(kv8_attn_any_kernel<T, KEYS, ROWS>, grid, dim3(kAnyThreads), smem, s, g);
+  if constexpr (KEYS != kExtend) {
+    if (g.cluster > 0) {
+      ClusterLaunch l(grid, dim3(1, 1, g.cluster), kAnyThreads, smem, s);
+      return cudaLaunchKernelEx(&l.cfg, kv8_attn_any_kernel<T, KEYS, ROWS, true>, g) == cudaSuccess ? QQ_OK : QQ_ERR_CUDA;
+    }
+  }
+  static SmemLimit limit;
+  int rc = limit.ensure((const void*)kv8_attn_any_kernel<T, KEYS, ROWS, false>, smem + kStaticSmem);
+  if (rc != QQ_OK) return rc;
+  rc = launch_pdl(kv8_attn_any_kernel<T, KEYS, ROWS, false>, grid, dim3(kAnyThreads), smem, s, g);
   if (rc != QQ_OK || g.splits == 1) return rc;
   const int64_t units = tiles * grid.y, per = 4 * (int64_t)device_sm_count() / units;  // CTAs to a unit
   const unsigned z = (unsigned)std::max<int64_t>(1, std::min<int64_t>(per, g.rows));
@@ -402,14 +451,59 @@ int launch_any(const AnyArgs& g, int keys, int64_t tiles, cudaStream_t s) {
                        : launch_any<T, kRows, 16>(g, tiles, s);
 }
 
+// Shared memory of `rows` rows of up to `dim` channels.
+size_t smem_up_to(int rows, int dim) {
+  AnyArgs g{};
+  g.a.c.dim = dim;
+  g.rows = rows;
+  g.key_groups = 1;
+  return any_smem(g);
+}
+template <typename T, int KEYS, int ROWS>
+int resident_any(int dim, int cluster) {
+  static ResidentClusters known[3][3];  // by cluster, by head_dim up to 64, 128 and 256
+  const int c = cluster == 16 ? 0 : cluster == 8 ? 1 : 2, d = dim <= 64 ? 0 : dim <= 128 ? 1 : 2;
+  return known[c][d].ask((const void*)kv8_attn_any_kernel<T, KEYS, ROWS, true>, dim3(1, 1, cluster), kAnyThreads,
+                         smem_up_to(ROWS, 64 << d), smem_up_to(ROWS, kMaxDim));
+}
+template <typename T, int KEYS>
+int resident_any(const AnyArgs& g, int cluster) {
+  return g.rows == 4   ? resident_any<T, KEYS, 4>(g.a.c.dim, cluster)
+         : g.rows == 8 ? resident_any<T, KEYS, 8>(g.a.c.dim, cluster)
+                       : resident_any<T, KEYS, 16>(g.a.c.dim, cluster);
+}
+// One token per entry: the cluster that takes a unit, 0 for records and a join.
+// All clusters run at a time, and no CTA has more than two tiles: 5 x 1,024 keys
+// of 2 heads of 64 (a tile to a CTA) take 9.3 us on the device where records and
+// a join take 11.5, 10 x 500 (two) 11.8 and 11.3 but 3 us less on the host; with
+// three to a CTA 1 x 2,500 would take 15.6 and 11.7.
+int any_cluster(const AnyArgs& g, int dtype, int64_t units, int64_t max_keys) {
+  if (max_keys <= kTileKeys || units > device_sm_count()) return 0;
+  for (int c = 16; c >= 4; c /= 2) {
+    if (max_keys > c * 2 * kTileKeys) return 0;
+    const int most = dtype == QQ_BF16
+                         ? std::min(resident_any<__nv_bfloat16, kTable>(g, c), resident_any<__nv_bfloat16, kRows>(g, c))
+                         : std::min(resident_any<float, kTable>(g, c), resident_any<float, kRows>(g, c));
+    if (units <= most) return c;
+  }
+  return 0;
+}
+// Splits and cluster of a call.
+void any_plan(AnyArgs& g, int keys, int dtype, int64_t tiles, int64_t max_keys) {
+  g.splits = any_splits(g, tiles, g.a.c.kv_heads, max_keys);
+  if (keys == kExtend || g.splits == 1) return;
+  g.cluster = any_cluster(g, dtype, tiles * g.a.c.kv_heads * g.chunks, max_keys);
+  if (g.cluster > 0) g.splits = g.cluster;
+}
+
 int run(const AttnArgs& a, int keys, int dtype, int64_t max_keys, size_t ws_bytes, cudaStream_t s) {
   if (keys != kExtend && decode_tc_fits(a, dtype)) return run_decode_tc(a, keys, max_keys, ws_bytes, s);
   if (keys == kExtend && extend_tc_fits(a, dtype)) return run_extend_tc(a, max_keys, ws_bytes, s);
   AnyArgs g = any_shape(a, keys);
   const int64_t tiles = any_tiles(g, keys, a.bs, a.tokens);
   if (tiles > INT32_MAX || (int64_t)a.c.kv_heads * g.chunks > 65535) return QQ_ERR_UNSUPPORTED;
-  g.splits = any_splits(g, tiles, a.c.kv_heads, max_keys);
-  if (g.splits > 1 && (a.part == nullptr || ws_bytes < (size_t)any_workspace(g, tiles))) return QQ_ERR_WORKSPACE;
+  any_plan(g, keys, dtype, tiles, max_keys);
+  if (any_workspace(g, tiles) > 0 && (a.part == nullptr || ws_bytes < (size_t)any_workspace(g, tiles))) return QQ_ERR_WORKSPACE;
   return dtype == QQ_BF16 ? launch_any<__nv_bfloat16>(g, keys, tiles, s) : launch_any<float>(g, keys, tiles, s);
 }
 
@@ -449,7 +543,7 @@ extern "C" size_t qq_kv8_workspace_bytes(const qq_kv8_cache* cache, int q_heads,
   const int keys = extend ? kExtend : kTable;
   AnyArgs g = any_shape(a, keys);
   const int64_t tiles = any_tiles(g, keys, bs, num_tokens);
-  g.splits = any_splits(g, tiles, a.c.kv_heads, max_keys);
+  any_plan(g, keys, dtype, tiles, max_keys);
   size_t need = (size_t)any_workspace(g, tiles);
   // enough for either kernel: which one runs depends on the pointers' alignment too
   if (keys != kExtend && decode_tc_fits(a, dtype)) {

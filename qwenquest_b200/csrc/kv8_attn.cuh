@@ -2,6 +2,8 @@
 // arguments, and how a key's place and a row's output are found.
 #pragma once
 
+#include <atomic>
+
 #include "kv8.cuh"
 
 namespace qq {
@@ -139,6 +141,67 @@ __device__ __forceinline__ int64_t key_slot(const AttnArgs& a, int e, int64_t re
   raise_error(err, QQ_DEV_ERR_BOUNDS);
   return -1;
 }
+
+// ---------------------------------------------------------------- clusters
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Word `addr` of the shared memory of the cluster's CTA `rank`.
+__device__ __forceinline__ float ld_cluster(uint32_t addr, int rank) {
+  float x;
+  asm volatile("{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}\n"
+               : "=f"(x)
+               : "r"(addr), "r"(rank)
+               : "memory");
+  return x;
+}
+
+// A launch by clusters of `cluster` CTAs.
+struct ClusterLaunch {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  ClusterLaunch(dim3 grid, dim3 cluster, int threads, size_t smem, cudaStream_t s) {
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster.x;
+    attr[0].val.clusterDim.y = cluster.y;
+    attr[0].val.clusterDim.z = cluster.z;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  }
+};
+
+// How many clusters of a kernel the current device holds at a time (0: none),
+// asked once per device, with `smem` bytes each; `most` is what any launch of it uses.
+class ResidentClusters {
+ public:
+  int ask(const void* kernel, dim3 cluster, int threads, size_t smem, size_t most) {
+    const int d = current_device();
+    if (d < 0 || d >= kMaxDevices) return 0;
+    int n = known_[d].load(std::memory_order_acquire);
+    if (n > 0) return n - 1;
+    n = 0;
+    ClusterLaunch l(cluster, cluster, threads, smem, nullptr);
+    l.cfg.numAttrs = 1;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) != cudaSuccess ||
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, kernel, &l.cfg) != cudaSuccess) {
+      cudaGetLastError();
+      n = 0;
+    }
+    known_[d].store(n + 1, std::memory_order_release);
+    return n;
+  }
+
+ private:
+  std::atomic<int> known_[kMaxDevices] = {};  // one more than the number
+};
 
 // The tensor-core kernel for one query token per entry (kTable, kRows): whether
 // it takes these arguments, the scratch it needs, and its launch.

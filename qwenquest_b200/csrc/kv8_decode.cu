@@ -212,19 +212,6 @@ __device__ __forceinline__ void write_query(const AttnArgs& a, int e, int h, int
   if (col == 0) qinv[r] = a.scale_log2 * exp2_int(-k2);
 }
 
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// Word `addr` of the shared memory of the cluster's CTA `rank`.
-__device__ __forceinline__ float ld_cluster(uint32_t addr, int rank) {
-  float x;
-  asm volatile("{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}\n"
-               : "=f"(x)
-               : "r"(addr), "r"(rank)
-               : "memory");
-  return x;
-}
-
 // CLUSTER: a cluster of that many CTAs takes a pair and joins it itself.
 template <int KEYS, int HEADS, int CLUSTER>
 __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
@@ -842,46 +829,11 @@ int launch(DecodeArgs g, int64_t ctas, cudaStream_t s) {
                     g, ctas);
 }
 
-// The launch of `pairs` clusters.
-struct ClusterLaunch {
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[2];
-  ClusterLaunch(int pairs, int cluster, size_t smem, cudaStream_t s) {
-    cfg.gridDim = dim3(pairs * cluster);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  }
-};
-
-// How many clusters of the kernel the current device holds at a time (0: none), asked once per device.
 template <int KEYS, int HEADS, int CLUSTER>
 int resident_clusters() {
-  static std::atomic<int> known[kMaxDevices];  // one more than the number
-  const int d = current_device();
-  if (d < 0 || d >= kMaxDevices) return 0;
-  int n = known[d].load(std::memory_order_acquire);
-  if (n > 0) return n - 1;
+  static ResidentClusters known;
   constexpr size_t smem = decode_smem<KEYS, HEADS>();
-  const void* kernel = (const void*)kv8_decode_kernel<KEYS, HEADS, CLUSTER>;
-  n = 0;
-  ClusterLaunch l(1, CLUSTER, smem, nullptr);
-  l.cfg.numAttrs = 1;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
-      cudaOccupancyMaxActiveClusters(&n, kernel, &l.cfg) != cudaSuccess) {
-    cudaGetLastError();
-    n = 0;
-  }
-  known[d].store(n + 1, std::memory_order_release);
-  return n;
+  return known.ask((const void*)kv8_decode_kernel<KEYS, HEADS, CLUSTER>, dim3(CLUSTER), kThreads, smem, smem);
 }
 
 template <int KEYS, int HEADS, int CLUSTER>
@@ -890,7 +842,7 @@ int launch_clusters(DecodeArgs g, cudaStream_t s) {
   Maps m;
   const int rc = encode_maps<KEYS>(g.a.c, m);
   if (rc != QQ_OK) return rc;
-  ClusterLaunch l(g.a.bs * g.a.c.kv_heads, CLUSTER, decode_smem<KEYS, HEADS>(), s);
+  ClusterLaunch l(dim3(g.a.bs * g.a.c.kv_heads * CLUSTER), dim3(CLUSTER), kThreads, decode_smem<KEYS, HEADS>(), s);
   return cudaLaunchKernelEx(&l.cfg, kv8_decode_kernel<KEYS, HEADS, CLUSTER>, g, m.mk, m.mv, m.rk, m.rv) == cudaSuccess
              ? QQ_OK
              : QQ_ERR_CUDA;

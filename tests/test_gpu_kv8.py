@@ -562,20 +562,22 @@ def test_extend_attention_matches_64_bits(kv, heads, dim, block, dtype, seq, new
             b.check(out[row], q[row], b.slots(i, np.arange(s - m + t + 1)), SMALL_EXTEND)
 
 
-@pytest.mark.parametrize("heads", [4, 32, 48])
+@pytest.mark.parametrize(("heads", "dim", "dtype"), [
+    (4, 128, torch.bfloat16), (32, 128, torch.bfloat16), (48, 128, torch.bfloat16), (8, 64, torch.float32),
+    (24, 40, torch.bfloat16), (64, 256, torch.float32)])
 @pytest.mark.parametrize("bs", [1, 2, 3, 6, 12])
 @pytest.mark.parametrize("width", [16, 100, 400])
-def test_decode_by_clusters_and_by_shares(heads, bs, width):
+def test_decode_by_clusters_and_by_shares(heads, dim, dtype, bs, width):
     """The table's width and the number of requests decide which form takes a call: a cluster of CTAs to a (request,
     KV head) pair, of three sizes, or equal shares of all tiles."""
     rng = np.random.default_rng(bs + width)
     seq = [1000, 0, 1, 129, 1024, 640, 128, 2, 900, 511, 512, 513][:bs]
-    b = _Batch(seq, 4, 128, 64, seed=heads + bs, heads=heads, dtype=torch.bfloat16, width=width)
+    b = _Batch(seq, 4, dim, 64, seed=heads + bs, heads=heads, dtype=dtype, width=width)
     q = b.queries(bs)
     reqs, lens = _dev(b.reqs), _dev(seq)
     out = b.cache.decode_attention(0, q.to(DEV), b.table_dev, reqs, lens, b.scaling)
     again = b.cache.decode_attention(0, q.to(DEV), b.table_dev, reqs, lens, b.scaling)
-    top = 64 * width // 4
+    top = 16 * width
     rows = np.full((bs, top), -1, dtype=np.int64)
     for i, s in enumerate(seq):
         rows[i, :min(s, top)] = b.slots(i, rng.permutation(s)[:top])
