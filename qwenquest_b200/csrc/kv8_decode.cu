@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
   volatile int* abort_flag = &s_abort;
-  auto wait = [&](int i, uint32_t parity) { return mbar_wait(bar(i), parity, abort_flag, a.err); };
+  auto wait = [&](int i, uint32_t parity) { return mbar_wait<8>(bar(i), parity, abort_flag, a.err); };
 
   // ---- barriers and tensor memory, then this CTA's share and where it begins
   if (threadIdx.x == kThreads - 1) {

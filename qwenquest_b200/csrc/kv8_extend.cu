@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
   volatile int* abort_flag = &s_abort;
-  auto wait = [&](int i, uint32_t parity) { return mbar_wait(bar(i), parity, abort_flag, a.err); };
+  auto wait = [&](int i, uint32_t parity) { return mbar_wait<8>(bar(i), parity, abort_flag, a.err); };
   wait_prior_grid();
 
   if (warp == 0) {

@@ -191,14 +191,17 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
 // CTA has given up (this wait ran out, or another thread's did).
 // With `drain` the wait ignores an earlier give-up (the last wait for the
 // CTA's own MMAs before its tensor memory is freed).
+// TRIES: tries between two looks at the clock (each waits a while in hardware;
+// the kernels of the 8-bit cache notice a phase sooner with eight, the others
+// with one).
+template <int TRIES = 1>
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t* err,
                                           bool drain = false) {
   if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = globaltimer_ns();
   for (;;) {
-    // each try waits a while in hardware; looking at the clock in between would notice the phase late
 #pragma unroll 1
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < TRIES; ++i)
       if (mbar_try_wait(bar, parity)) return true;
     if (*abort_flag && !drain) return false;
     if (globaltimer_ns() - t0 > kWaitLimitNs) {
