@@ -370,7 +370,10 @@ size_t qq_kv8_workspace_bytes(const qq_kv8_cache* cache, int q_heads, int dtype,
  * gives zeros (padding); a length past the table or a request out of range
  * gives zeros and QQ_DEV_ERR_BOUNDS; a block out of range takes no part and
  * is reported too.  bf16 with head_dim 128 and up to 16 query heads per KV
- * head runs on the tensor cores, anything else on the fp32 units. */
+ * head runs on the tensor cores, anything else on the fp32 units.  On the
+ * tensor cores a weight (times the scale of V) enters the product with 8 bits,
+ * or as a multiple of 2^-21 of the largest one among its 128 keys (or of 2^-12
+ * of the row's, where that is more). */
 int qq_kv8_decode_attention(const qq_kv8_cache* cache, const qq_batch* batch, const int32_t* block_table,
                             int64_t table_stride, int64_t table_rows, const void* q, int dtype, int q_heads,
                             int64_t q_stride, float scaling, void* out, int64_t out_stride, uint32_t* err,

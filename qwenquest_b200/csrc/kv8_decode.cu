@@ -5,16 +5,24 @@
 // Bound by the bytes of the codes (2 x 128 per token and KV head), so the
 // codes go from HBM to shared memory (TMA) to the tensor cores without a
 // conversion: both products have an operand of the other side in e4m3, held
-// to bf16's precision by a pair hi + lo / 16 in two columns of one MMA.
+// by a pair hi + lo / 16 (queries) or hi + lo / 32 (weights) in two columns of
+// one MMA: 8 significant bits, bf16's, down to a fixed part of the largest.
 //   S^T [128 tokens x NC] = K [128 x 128] . Q^T      NC = 2 x 8 (or 2 x 16)
 //   O^T [128 dims x NC]   = V^T [128 x 128] . P      columns: heads hi, heads lo
 // A tile of 128 tokens is a row per thread in both, so each thread has one
 // token's scores of all heads, and later one channel of all heads.
 //
 // Scales: a token's score is S ks q^-1 log2(e) scaling; its weight into the V
-// product is 2^(s - M) vs.  With vs = vm 2^ev the running maximum M is that of
-// s + ev, so what enters the product, vm 2^(s + ev - M), is at most 2 whatever
-// the blocks' scales are, and the sum l takes 2^(s + ev - M) 2^-ev.
+// product is 2^(s - R) vs.  With vs = vm 2^ev the reference R is a maximum of
+// s + ev, so what enters the product, vm 2^(s + ev - R), is at most 2 whatever
+// the blocks' scales are, and the sum l takes 2^(s + ev - R) 2^-ev.
+// R is the tile's own maximum, or 2^-kFall of the largest so far where that is
+// more: O and l are multiplied by 2^(R before - R), which may be above 1, when a
+// tile is added.  A weight in the product is a multiple of 2^-21 of 2^R, with 8
+// bits down to 2^-13 of it.  Against the running maximum the tail of a row
+// would lose those bits to one key with most of the mass, as attention sinks
+// have it, while l kept them: 131,072 equal keys behind one of 95 % of the mass
+// and a small value were off by 98 % of the result, and are by 0.1 %.
 //
 // Work: the tiles of all (request, KV head) pairs in a row, cut into equal
 // shares, one per CTA (two CTAs per SM); a pair cut by a share's edge leaves
@@ -52,8 +60,15 @@ constexpr int kMaxSlots = 12;
 constexpr int kClusterTiles = 4;              // tiles of each of them at most
 constexpr int kInv = 4;                        // pairs of which the softmax may not have seen the queries' scales
 constexpr uint32_t kMasked = 0xFFFFFFFFu;      // a V scale's bits where the token takes no part
-constexpr float kLo = 16.f;
+constexpr float kLo = 16.f;                    // queries: up to 448, whose rest is at most 16
 constexpr float kPScale = 128.f;               // weights (at most 2) times this are e4m3's upper binades
+constexpr float kPLo = 32.f;                   // their rest is at most 8
+constexpr float kNone = -3.402823466e38f;      // the maximum of no keys: finite, so that differences are numbers
+// How far the reference may lie below the largest score: keys that much lighter share steps of 2^-33 of the heaviest.
+// A key of a block of zeros (scale 2^-126) adds up to 2^-kLeastEv to l, 2^kFall more once the reference has fallen:
+// finite over 2^24 such keys.
+constexpr float kFall = 12.f;
+constexpr int kLeastEv = -90;
 
 // mbarriers
 enum : int {
@@ -512,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
     // the barrier they share, but touch no tensor memory and write nothing.
     const int tok = threadIdx.x;  // token of the tile, and channel of the output
     const uint32_t lane_base = tmem + ((uint32_t)(warp * 32) << 16);
-    float M[HEADS], l[HEADS], corr[HEADS], O[HEADS];
+    float M[HEADS], R[HEADS], l[HEADS], step[HEADS], O[HEADS];  // largest score, reference, sum, 2^(R before - R), output
     int pair = 0;
     bool first = true, ok = true;
     auto columns = [&](uint32_t col, uint32_t (&v)[NC]) {
@@ -528,7 +543,7 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
       columns(2 * NC + (i & 1) * NC, v);
 #pragma unroll
       for (int r = 0; r < HEADS; ++r)
-        O[r] = fmaf(O[r], by[r], fmaf(__uint_as_float(v[HEADS + r]), 1.f / kLo, __uint_as_float(v[r])));
+        O[r] = fmaf(O[r], by[r], fmaf(__uint_as_float(v[HEADS + r]), 1.f / kPLo, __uint_as_float(v[r])));
     };
     // the first queries by all four warps: nothing else can go on before them (1.8 us with one warp)
     constexpr int kCh = kTcDim * HEADS / kSoft;
@@ -543,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
       const int b = i & 1, m = i % kMeta;
       if (first) {
 #pragma unroll
-        for (int r = 0; r < HEADS; ++r) M[r] = -INFINITY, l[r] = 0.f, O[r] = 0.f, corr[r] = 0.f;
+        for (int r = 0; r < HEADS; ++r) M[r] = R[r] = kNone, l[r] = 0.f, O[r] = 0.f, step[r] = 0.f;
         // Q's own barrier may be two phases on by now: with a tile to a pair the
         // scores run two pairs ahead of this, and the queries two more.  The
         // scales of pair p + kInv are written after S(p + 2), so after P(p).
@@ -561,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
         columns(b * NC, v);
       }
       // vs = vm 2^ev; ev stays where 2^-ev and the sums of it are normal numbers
-      const int ev = seen ? min(126, max(-100, (int)((__float_as_uint(vs) >> 23) & 255) - 127)) : 0;
+      const int ev = seen ? min(126, max(kLeastEv, (int)((__float_as_uint(vs) >> 23) & 255) - 127)) : 0;
       const float back = seen ? exp2_int(-ev) : 0.f;
       const float vm = seen ? vs * back * kPScale : 0.f;
       float u[HEADS], most[HEADS];
@@ -574,7 +589,7 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
       const float top = reduce_lanes(most, lane, [](float x, float y) { return fmaxf(x, y); });
       if (lane % (32 / HEADS) == 0) s_max[b][lane / (32 / HEADS)][warp] = top;
       asm volatile("bar.sync 1, 128;" ::: "memory");
-      float before_corr[HEADS];
+      float before[HEADS];
       uint32_t hi8[HEADS / 2], lo8[HEADS / 2];
 #pragma unroll
       for (int r = 0; r < HEADS; r += 2) {
@@ -583,16 +598,17 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
         for (int k = 0; k < 2; ++k) {
           const int q = r + k;
           const float4 m4 = *reinterpret_cast<const float4*>(s_max[b][q]);
-          const float mn = fmaxf(fmaxf(fmaxf(m4.x, m4.y), fmaxf(m4.z, m4.w)), M[q]);
-          const float ref = mn == -INFINITY ? 0.f : mn;
-          before_corr[q] = corr[q];
-          corr[q] = ex2(M[q] - ref);
-          M[q] = mn;
+          const float m = fmaxf(fmaxf(m4.x, m4.y), fmaxf(m4.z, m4.w));
+          M[q] = fmaxf(m, M[q]);
+          const float ref = fmaxf(m, M[q] - kFall);
+          before[q] = step[q];
+          step[q] = ex2(R[q] - ref);
+          R[q] = ref;
           const float p = ex2(u[q] - ref);
-          l[q] = fmaf(l[q], corr[q], p * back);
+          l[q] = fmaf(l[q], step[q], p * back);
           wgt[k] = p * vm;
         }
-        split_e4m3x2(wgt[0], wgt[1], kLo, hi8[r / 2], lo8[r / 2]);
+        split_e4m3x2(wgt[0], wgt[1], kPLo, hi8[r / 2], lo8[r / 2]);
       }
       uint8_t* P = smem + off_p + b * kColBytes;
 #pragma unroll
@@ -613,12 +629,12 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
       fence_async_shared();
       tc_fence_before();
       mbar_arrive_warp(bar(kBarP + b));
-      if (!first) add_product(i - 1, before_corr);
+      if (!first) add_product(i - 1, before);
       first = w.last();
       if (!first && i + 1 < count) continue;
 
       // ---- the end of the pair, or of the share: the result, or a record of this part
-      add_product(i, corr);
+      add_product(i, step);
       const float part = reduce_lanes(l, lane, [](float x, float y) { return x + y; });
       if (lane % (32 / HEADS) == 0) s_sum[lane / (32 / HEADS)][warp] = part;
       asm volatile("bar.sync 1, 128;" ::: "memory");
@@ -637,7 +653,7 @@ __global__ void __launch_bounds__(kThreads, HEADS == 8 ? 2 : 1)
               static_cast<__nv_bfloat16*>(a.out)[w.e * a.out_stride + (int64_t)(w.h * a.group + r) * kTcDim + tok] =
                   __float2bfloat16_rn(sum == 0.f ? 0.f : o * __frcp_rn(sum));
           } else {
-            if (tok == 0) rec[r] = M[r], rec[HEADS + r] = sum;
+            if (tok == 0) rec[r] = R[r], rec[HEADS + r] = sum;
             rec[2 * HEADS + r * kTcDim + tok] = o;
           }
         }

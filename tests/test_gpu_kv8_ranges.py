@@ -1,0 +1,160 @@
+"""The 8-bit cache's attention over long rows and uneven weights, against 64 bits.
+
+What ``test_gpu_kv8.py`` says of the errors holds; here the sums and the floor of small weights are counted as the
+kernels make them, so that a bound is a small part of the result also where one key has most of a long row's mass:
+
+* sums: 128 products of a tile in one accumulator, then a multiply-add with a power (2^x itself is off by 2^-22) per
+  tile and per part that is joined, each off by 2^-23 at most (a sum that is cut off rather than rounded):
+  ``(128 + 3 tiles + 256) 2^-23`` of sum_j w_j |v_j|, for the row sum the same;
+* one-token kernel: a weight (times the scale of V) is two e4m3 numbers hi + lo / 32, taken times 128 against the largest
+  of its tile of 128 keys, or 2^-12 of the row's largest: off by 2^-8 of itself or by 2^-10 / 32 of 128, 2^-22 of that;
+* prefill kernel: a weight is an fp16 number, 2^-11, or 2^-25 where the row's largest is at least 2^5 (2^8 when the
+  reference is taken, at least 2^11 / 64 after it was raised): 2^-30 of the row's largest;
+* fp32 kernel: nothing of the kind, bf16 inputs or not.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv8 as oracle
+from qwenquest_b200.kv8 import KV8Cache
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+TILE = 128
+
+
+def _dev(x, dtype=torch.int64):
+    return torch.tensor(np.asarray(x), dtype=dtype, device=DEV)
+
+
+def _check(got, q, k, v, v_scale, scaling, form):
+    """One query ``q`` [heads, dim] against ``k``, ``v`` float64 [n, kv, dim]; ``form``: decode, extend or fp32."""
+    heads, dim = q.shape
+    n, kv, _ = k.shape
+    tiles = -(-n // TILE)
+    q64 = q.double().numpy()
+    got = got.double().cpu().numpy().reshape(heads, dim)
+    step = torch.finfo(q.dtype).eps / 2
+    for h in range(heads):
+        kh, vh, s = k[:, h // (heads // kv)], v[:, h // (heads // kv)], v_scale[:, h // (heads // kv)].astype(np.float64)
+        x = kh @ q64[h] * scaling
+        w = np.exp(x - x.max())
+        w /= w.sum()
+        out, size = w @ vh, w @ np.abs(vh)
+        spread = (np.abs(kh) @ np.abs(q64[h])).max() * scaling
+        rel = 2 * (dim + 8) * 2.0 ** -24 * spread + 2 * 2.0 ** -22 + 2 * (TILE + 3 * tiles + 256) * 2.0 ** -23
+        err = rel * size
+        codes = np.abs(vh) / s[:, None]
+        if form == "decode":
+            pad = tiles * TILE - n
+            top = np.maximum(np.pad(w * s, (0, pad)).reshape(tiles, TILE).max(1), 2.0 ** -12 * (w * s).max())
+            err = err + 2.0 ** -8 * size + 2.0 ** -22 * top @ np.pad(codes, ((0, pad), (0, 0))).reshape(tiles, TILE, dim).sum(1)
+        elif form == "extend":
+            err = err + 2.0 ** -11 * size + 2.0 ** -30 * (w * s).max() * codes.sum(0)
+        tol = step * np.abs(out) + (1 + step) * err + 1e-37
+        off = np.abs(got[h] - out)
+        assert (off <= tol).all(), (h, float((off / np.abs(out)).max()), float((off / tol).max()), float((tol / np.abs(out)).max()))
+
+
+class _Sinks:
+    """One request of ``n`` tokens over scattered blocks: keys of even scores but for a few positions that hold most of
+    a head's mass, 50 to 99.9 % of it, with small values; the other values are between 0.5 and 1.5, so that what the
+    tail loses is the result's."""
+
+    MASSES = (0.5, 0.9, 0.95, 0.98, 0.99, 0.995, 0.998, 0.999)
+
+    def __init__(self, n, sinks, seed, dim=128, block=64, spread=0.3, dtype=torch.bfloat16):
+        rng = np.random.default_rng(seed)
+        pages = -(-n // block)
+        shape = (pages + 1, 1, block, dim)
+        heads = len(self.MASSES)
+        scale = np.float32(2.0 ** -7)
+        self.order = rng.permutation(pages + 1)[:pages]
+        pos = np.arange(n)
+        self.slots = self.order[pos // block] * block + pos % block
+        at = (self.slots // block, 0, self.slots % block)
+        k = np.zeros(shape, dtype=np.uint8)
+        v = np.zeros(shape, dtype=np.uint8)
+        kx = rng.standard_normal((n, dim)) * 60
+        kx[:, 0] = 0
+        kx[sinks] = 0
+        kx[sinks, 0] = 448
+        vx = (0.5 + rng.random((n, dim))) * 128
+        vx[sinks] = 2.0 ** -3 * rng.random((len(sinks), dim))
+        k[at] = oracle.to_e4m3(kx)
+        v[at] = oracle.to_e4m3(vx)
+        self.scaling = dim ** -0.5
+        q = rng.standard_normal((heads, dim)) * spread
+        for h, m in enumerate(self.MASSES):  # the sinks' score against the mean weight of the tail, e^0.06 or so
+            q[h, 0] = np.log(n * m / (1 - m) / len(sinks)) / (self.scaling * 448 * scale)
+        self.q = torch.from_numpy(q[None]).to(dtype)
+        scales = np.full(shape[:2], scale, dtype=np.float32)
+        self.cache = KV8Cache.from_tensors(
+            [torch.from_numpy(k).to(DEV).view(torch.float8_e4m3fn)], [torch.from_numpy(v).to(DEV).view(torch.float8_e4m3fn)],
+            [torch.from_numpy(scales).to(DEV)], [torch.from_numpy(scales).to(DEV)])
+        self.n, self.block = n, block
+        self.k, self.v = oracle.rows(k, scales, self.slots), oracle.rows(v, scales, self.slots)
+        self.v_scale = np.full((n, 1), scale, dtype=np.float32)
+        self.table = _dev(self.order[None], torch.int32)
+
+    def check(self, got, form, seen=None, q=None):
+        seen = np.arange(self.n) if seen is None else seen
+        _check(got, self.q[0] if q is None else q, self.k[seen], self.v[seen], self.v_scale[seen], self.scaling, form)
+
+
+@pytest.mark.parametrize(("n", "sinks"), [
+    (32768, [0]), (131072, [0]), (131071, [70000]), (131072, [0, 1, 131071]), (8192, [0]), (2049, [2048]), (300, [5])])
+def test_decode_behind_a_key_with_most_of_the_mass(n, sinks):
+    """A lone request (a cluster, or all shares), and as many as fill the GPU, a whole one to each CTA."""
+    s = _Sinks(n, sinks, seed=n + len(sinks))
+    lone = s.cache.decode_attention(0, s.q.to(DEV), s.table, [0], [n], s.scaling)
+    many = 300
+    full = s.cache.decode_attention(0, s.q.to(DEV).expand(many, -1, -1), s.table, [0] * many, [n] * many, s.scaling)
+    s.cache.synchronize()
+    s.check(lone[0], "decode")
+    s.check(full[0], "decode")
+    s.check(full[many // 2 + 1], "decode")
+    s.check(full[many - 1], "decode")
+
+
+@pytest.mark.parametrize(("n", "top"), [(32768, 32768), (40000, 4096)])
+def test_selected_rows_behind_a_key_with_most_of_the_mass(n, top):
+    """All rows in another order, and a selection of pages, with the heavy key among them."""
+    s = _Sinks(n, [0], seed=n + top)
+    rng = np.random.default_rng(top)
+    pages = np.concatenate([[0], 1 + rng.permutation(n // s.block - 1)])[:top // s.block]
+    pos = (pages[:, None] * s.block + np.arange(s.block)).ravel()
+    rows = _dev(s.slots[pos], torch.int32)
+    lone = s.cache.sparse_decode_attention(0, s.q.to(DEV), rows[None], [top], s.scaling)
+    many = 300
+    full = s.cache.sparse_decode_attention(0, s.q.to(DEV).expand(many, -1, -1), rows.expand(many, -1).contiguous(),
+                                           [top] * many, s.scaling)
+    s.cache.synchronize()
+    for got in (lone[0], full[0], full[many - 1]):
+        s.check(got, "decode", seen=pos)
+
+
+@pytest.mark.parametrize(("heads", "kv"), [(8, 1), (32, 4), (16, 1)])
+def test_a_lone_request_of_131072_keys(heads, kv):
+    """A pair cut over all shares and joined from their records; keys and values of either sign, uneven scores."""
+    n, dim, block = 131072 + 77, 128, 64
+    rng = np.random.default_rng(heads)
+    pages = -(-n // block)
+    codes = [oracle.to_e4m3(rng.standard_normal((pages, kv, block, dim)) * 90 + 60) for _ in range(2)]
+    scales = [np.ldexp(1.0, rng.integers(-9, -5, (pages, kv))).astype(np.float32) for _ in range(2)]
+    order = rng.permutation(pages)
+    slots = order[np.arange(n) // block] * block + np.arange(n) % block
+    cache = KV8Cache.from_tensors(*([torch.from_numpy(c).to(DEV).view(torch.float8_e4m3fn)] for c in codes),
+                                  *([torch.from_numpy(x).to(DEV)] for x in scales))
+    q = torch.from_numpy(rng.standard_normal((1, heads, dim))).to(torch.bfloat16)
+    out = cache.decode_attention(0, q.to(DEV), _dev(order[None], torch.int32), [0], [n], dim ** -0.5)
+    rows = cache.sparse_decode_attention(0, q.to(DEV), _dev(slots, torch.int32)[None], [n], dim ** -0.5)
+    cache.synchronize()
+    k, v = (oracle.rows(c, x, slots) for c, x in zip(codes, scales))
+    for got in (out, rows):
+        _check(got[0], q[0], k, v, scales[1][slots // block], dim ** -0.5, "decode")
