@@ -8,8 +8,8 @@ kernels make them, so that a bound is a small part of the result also where one 
   ``(128 + 3 tiles + 256) 2^-23`` of sum_j w_j |v_j|, for the row sum the same;
 * one-token kernel: a weight (times the scale of V) is two e4m3 numbers hi + lo / 32, taken times 128 against the largest
   of its tile of 128 keys, or 2^-12 of the row's largest: off by 2^-8 of itself or by 2^-10 / 32 of 128, 2^-22 of that;
-* prefill kernel: a weight is an fp16 number, 2^-11, or 2^-25 where the row's largest is at least 2^5 (2^8 when the
-  reference is taken, at least 2^11 / 64 after it was raised): 2^-30 of the row's largest;
+* prefill kernel: a weight (times the scale of V) is an fp16 number, 2^-11, or 2^-25 where the weights of 64 keys sum to
+  2^7 at least (one of them 2^7 when the reference is taken, all of them after it was raised): 2^-32 of the row's sum;
 * fp32 kernel: nothing of the kind, bf16 inputs or not.
 """
 
@@ -55,7 +55,7 @@ def _check(got, q, k, v, v_scale, scaling, form):
             top = np.maximum(np.pad(w * s, (0, pad)).reshape(tiles, TILE).max(1), 2.0 ** -12 * (w * s).max())
             err = err + 2.0 ** -8 * size + 2.0 ** -22 * top @ np.pad(codes, ((0, pad), (0, 0))).reshape(tiles, TILE, dim).sum(1)
         elif form == "extend":
-            err = err + 2.0 ** -11 * size + 2.0 ** -30 * (w * s).max() * codes.sum(0)
+            err = err + 2.0 ** -11 * size + 2.0 ** -32 * (w * s).sum() * codes.sum(0)
         tol = step * np.abs(out) + (1 + step) * err + 1e-37
         off = np.abs(got[h] - out)
         assert (off <= tol).all(), (h, float((off / np.abs(out)).max()), float((off / tol).max()), float((tol / np.abs(out)).max()))
@@ -137,6 +137,19 @@ def test_selected_rows_behind_a_key_with_most_of_the_mass(n, top):
     s.cache.synchronize()
     for got in (lone[0], full[0], full[many - 1]):
         s.check(got, "decode", seen=pos)
+
+
+@pytest.mark.parametrize(("n", "new", "sinks"), [
+    (8192, 5000, [0]), (32768, 5000, [0]), (131072, 5000, [0]), (131072, 40, [0]), (32768, 5000, [20000]),
+    (8192, 8192, [0, 130])])
+def test_extend_behind_a_key_with_most_of_the_mass(n, new, sinks):
+    """Enough query rows that a thread block takes all keys of its own, and so few that they are cut."""
+    s = _Sinks(n, sinks, seed=n + new)
+    q = s.q.expand(new, -1, -1).contiguous()
+    out = s.cache.extend_attention(0, q.to(DEV), s.table, [0], [n], [n - new], [0], s.scaling)
+    s.cache.synchronize()
+    for t in (0, 31, new // 2, new - 1):
+        s.check(out[t], "extend", seen=np.arange(n - new + t + 1))
 
 
 @pytest.mark.parametrize(("heads", "kv"), [(8, 1), (32, 4), (16, 1)])
