@@ -303,7 +303,7 @@ typedef struct qq_block_tables {
  * for; more new tokens than that are QQ_DEV_ERR_BOUNDS).  req_to_token (null:
  * none; int32 [map_rows][map_stride]) gets the same slots by request and
  * position, the table the page selection translates through.  An entry of
- * seq_lens 0 is padding.  A request past the ring's free blocks (the sum in
+ * seq_lens 0 is padding, whatever request it names.  A request past the ring's free blocks (the sum in
  * batch order) gets none, slots of -1 and QQ_DEV_ERR_CAPACITY; a bad length, a
  * request out of range or named a second time likewise with
  * QQ_DEV_ERR_BOUNDS.  bs <= QQ_MAX_BS. */

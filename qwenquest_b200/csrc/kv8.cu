@@ -116,11 +116,12 @@ __device__ __forceinline__ int last_at_most(const V* sums, int n, V x) {
 }
 
 // A request that the batch names twice is served for its first entry only: the
-// claim word of a request takes the largest bs - i (0 between launches).
-__device__ __forceinline__ void claim_requests(const TableArgs& a) {
+// claim word of a request takes the largest bs - i (0 between launches).  An
+// entry whose `lens` is 0 is padding and claims nothing (null: none is).
+__device__ __forceinline__ void claim_requests(const TableArgs& a, const int64_t* lens) {
   for (int i = threadIdx.x; i < a.bs; i += kTableThreads) {
     const int64_t r = a.reqs[i];
-    if (r >= 0 && r < a.max_reqs) atomicMax(a.claim + r, a.bs - i);
+    if (r >= 0 && r < a.max_reqs && (lens == nullptr || lens[i] != 0)) atomicMax(a.claim + r, a.bs - i);
   }
   __syncthreads();
 }
@@ -145,7 +146,7 @@ __global__ void __launch_bounds__(kTableThreads) block_plan_kernel(TableArgs a) 
   if (tid == 0) s_taken = 0;
   wait_prior_grid();
   allow_next_grid();
-  claim_requests(a);
+  claim_requests(a, a.seq);
   const int64_t head = a.ring[0], free_count = a.ring[1] - head;
 
   // ---- this thread's entries: new tokens and blocks to take
@@ -255,7 +256,7 @@ __global__ void __launch_bounds__(kTableThreads) block_trim_kernel(TableArgs a) 
   const int block = 1 << a.shift;
   wait_prior_grid();
   allow_next_grid();
-  claim_requests(a);
+  claim_requests(a, nullptr);
   const int64_t tail = a.ring[1], room = a.capacity - (tail - a.ring[0]);
   int32_t back[kTablePer], my_back = 0;
   const int per = (a.bs + kTableThreads - 1) / kTableThreads;
