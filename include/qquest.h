@@ -323,10 +323,11 @@ int qq_block_trim(const qq_block_tables* tables, const int64_t* req_pool_indices
  * block and head.  block_size 16, 32, 64 or 128, head_dim a multiple of 8 up
  * to 256, codes 16-byte aligned, num_blocks * kv_heads * block_size < 2^31.
  * state (device [QQ_KV8_STATE_WORDS + 2 * kv_heads * num_blocks], 8-byte
- * aligned, zero-filled once) is needed by qq_kv8_append alone.  No reference
+ * aligned, zero-filled once; word 1 counts the calls, the words behind are 0
+ * between calls) is needed by qq_kv8_append alone.  No reference
  * counterpart: the reference keeps K and V in the model's dtype
  * (MHATokenToKVPool, memory.py:79-120). */
-#define QQ_KV8_STATE_WORDS 66
+#define QQ_KV8_STATE_WORDS 2
 typedef struct qq_kv8_cache {
   uint8_t* k;
   uint8_t* v;
@@ -347,9 +348,10 @@ typedef struct qq_kv8_cache {
  * block holds are requantised when it grows.  A token at offset 0 starts its
  * block anew.  Infinities are stored as +-448 s, NaN as NaN.  The tokens of a
  * block stand next to each other in ascending slots: a block met twice in one
- * call, like a slot out of range, is QQ_DEV_ERR_BOUNDS and one of the two
- * stretches is not written.  Calls of several streams may overlap where they
- * write different blocks (a block that two of them write at once is not found). */
+ * call, like a slot out of range, is QQ_DEV_ERR_BOUNDS, and only the first of
+ * the stretches is written.  Calls of several streams may overlap where they
+ * write different blocks (a block that two of them write at once is not found).
+ * num_tokens < 2^31. */
 int qq_kv8_append(const qq_kv8_cache* cache, const void* k, const void* v, int dtype, int64_t k_stride,
                   int64_t v_stride, const int64_t* slots, int64_t num_tokens, uint32_t* err, void* stream);
 

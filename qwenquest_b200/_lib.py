@@ -35,7 +35,7 @@ QQ_STEP_FINALIZE = 2
 QQ_MAX_LAYERS = 128
 QQ_MAX_BS = 4096
 QQ_NOALLOC_MAX_BS = 1024
-QQ_KV8_STATE_WORDS = 66
+QQ_KV8_STATE_WORDS = 2
 
 
 class QQQuestState(ctypes.Structure):

@@ -322,38 +322,38 @@ struct AppendArgs {
   const int64_t* slots;
   int64_t n;
   int window;  // tokens whose runs a CTA takes
+  bool claimed;  // kv8_claim_kernel has run
   uint32_t* err;
 };
 
 constexpr int kMaxWindow = 64;
 constexpr int kAppendThreads = 128;
-// The words of `state`: 64 bits that count calls in units of 2^-32, 32 such
-// counters for grids of many CTAs (one would be 8 us of atomics for 8192), the
-// claims.  Each CTA of a call adds its part when it is done, and the parts of a
-// call add up to one: the upper half advances when the last CTA leaves, and
-// stays right when calls on several streams overlap, whose parts mix.
-constexpr int kNumCounters = 32, kClaims = 2 + 2 * kNumCounters;
-constexpr uint32_t kFewCtas = 256;
-static_assert(kClaims == QQ_KV8_STATE_WORDS, "the header's size");
+// `state`: 64 bits whose upper half counts the calls, then a claim word per
+// block, K or V and head, 0 between calls.
+constexpr int kClaims = QQ_KV8_STATE_WORDS;
+// Up to this many tokens a window is one token and a run looks for its block
+// among the tokens before it; a call with more claims the blocks in a launch of
+// its own (64 tokens: 3.3 us by looking, 5.6 by claims; 256: 7.5 and 9.0; 512:
+// 12.6 and 13.4).
+constexpr int64_t kLookTokens = 512;
 
-__device__ __forceinline__ unsigned long long part_of_one(uint32_t shares, bool first) {
-  const unsigned long long each = (1ull << 32) / shares;
-  return first ? (1ull << 32) - each * (shares - 1) : each;
+__device__ __forceinline__ bool run_head(const Cache& c, int64_t slot, int64_t before) {
+  return slot >= 0 && ((slot & (c.block - 1)) == 0 || before != slot - 1);
 }
-__device__ __forceinline__ void count_cta(uint32_t* state) {
-  auto* words = reinterpret_cast<unsigned long long*>(state);
-  const uint32_t ctas = gridDim.x * gridDim.y, id = blockIdx.y * gridDim.x + blockIdx.x;
-  if (ctas < kFewCtas) {
-    atomicAdd(words, part_of_one(ctas, id == 0));
-    return;
-  }
-  const uint32_t mine = id % kNumCounters;
-  const unsigned long long part = part_of_one((ctas - mine + kNumCounters - 1) / kNumCounters, id < kNumCounters);
-  const unsigned long long was = atomicAdd(words + 1 + mine, part);
-  if (was >> 32 != (was + part) >> 32) atomicAdd(words, (1ull << 32) / kNumCounters);
+
+// The claims of a call: a block's word takes n - t for the first token t of a
+// run in it, the largest of them (so the first run has it).
+constexpr int kClaimThreads = 128;
+__global__ void __launch_bounds__(kClaimThreads) kv8_claim_kernel(Cache c, const int64_t* slots, int64_t n) {
+  wait_prior_grid();
+  allow_next_grid();
+  const int64_t t = (int64_t)blockIdx.x * kClaimThreads + threadIdx.x, total = (int64_t)c.num_blocks << c.shift;
+  if (t >= n) return;
+  const int64_t slot = slots[t];
+  if (slot >= total || !run_head(c, slot, t > 0 ? slots[t - 1] : -1)) return;
+  uint32_t* claims = c.state + kClaims + (slot >> c.shift) * 2 * c.kv_heads;
+  for (int i = 0; i < 2 * c.kv_heads; ++i) atomicMax(claims + i, (uint32_t)(n - t));
 }
-// What a call's claims are marked with: 0 is none.
-__device__ __forceinline__ uint32_t epoch_of(const uint32_t* state) { return ld_volatile_u32(state + 1) | 0x80000000u; }
 
 // A run is a stretch of tokens whose slots ascend by one inside a block; the
 // CTAs of its first token quantise it, one per K or V and head (blockIdx.y).
@@ -362,11 +362,12 @@ __device__ __forceinline__ uint32_t epoch_of(const uint32_t* state) { return ld_
 // is read once, and all of it at once (longer runs are read again, from L2).
 // Bound by the values' bytes for a prefill and by the chain slots -> values ->
 // maximum -> codes for a decode step.
-// Two runs of one call that meet in a block would race: a run claims its block
-// with the call's epoch, and the one that finds the epoch there is skipped and
-// reported.  The device counts the epochs, so a captured call gets a new one
-// with every replay.  (Calls that overlap may share an epoch or use two; they
-// write different blocks, so no claim is wrong.)
+// Two runs of one call that meet in a block would race: the first one is
+// written, the others are skipped and reported.  Which is the first is found
+// from the call's own slots, so calls of other streams, which write other
+// blocks, and captured calls have no part in it: either by looking at the tokens
+// before the run, or from the block's claim, which the run that made it takes
+// back (no other run of the call finds its own number there, before or after).
 template <typename T, int DIM>
 __global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 2 ? 8 : 4) kv8_append_kernel(AppendArgs a) {
   constexpr int kHeld = 8;
@@ -374,7 +375,6 @@ __global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 2 ? 8 : 4) kv8_ap
   __shared__ int64_t s_slots[kMaxWindow + kMaxBlock + 1];
   __shared__ uint32_t s_heads[kMaxWindow / 32];
   __shared__ float s_most[2][kAppendThreads / 32];
-  __shared__ int s_conflict[2];
   const Cache& c = a.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int dim = DIM > 0 ? DIM : c.dim;
@@ -386,7 +386,6 @@ __global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 2 ? 8 : 4) kv8_ap
   const int64_t total = (int64_t)c.num_blocks << c.shift;
   wait_prior_grid();
   allow_next_grid();
-  const uint32_t epoch = epoch_of(c.state);
   // s_slots[i] is the slot of token w0 - 1 + i (-1 outside the batch)
   for (int i = tid; i < a.window + c.block + 1; i += kAppendThreads) {
     const int64_t t = w0 - 1 + i;
@@ -398,7 +397,7 @@ __global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 2 ? 8 : 4) kv8_ap
     bool head = false;
     if (tid < a.window && w0 + tid < a.n) {
       const int64_t slot = s_slots[tid + 1];
-      head = slot >= 0 && ((slot & (c.block - 1)) == 0 || s_slots[tid] != slot - 1);
+      head = run_head(c, slot, s_slots[tid]);
       if (slot >= total) {
         raise_error(a.err, QQ_DEV_ERR_BOUNDS);
         head = false;
@@ -425,8 +424,22 @@ __global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 2 ? 8 : 4) kv8_ap
       }
       n = base + 32;
     }
-    if (tid == 0)
-      s_conflict[turn] = atomicExch(c.state + kClaims + (int64_t)b * 2 * c.kv_heads + blockIdx.y, epoch) == epoch;
+    // whether the block has an earlier run
+    auto look = [&]() {
+      bool met = false;
+      if (!a.claimed) {
+        for (int64_t i = tid; i < w0 + u; i += kAppendThreads) {
+          const int64_t other = a.slots[i];
+          met |= other >= 0 && other >> c.shift == b;
+        }
+      } else if (tid == 0) {
+        uint32_t* claim = c.state + kClaims + (int64_t)b * 2 * c.kv_heads + blockIdx.y;
+        met = ld_volatile_u32(claim) != (uint32_t)(a.n - (w0 + u));
+        if (!met) *claim = 0;
+      }
+      return met;
+    };
+    bool met;
     const T* src = static_cast<const T*>(is_v ? a.v : a.k) + (w0 + u) * stride + (int64_t)h * dim;
     const int64_t bh = (int64_t)b * c.kv_heads + h;
     uint8_t* codes = (is_v ? c.v : c.k) + bh * c.block * dim;
@@ -467,6 +480,7 @@ __global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 2 ? 8 : 4) kv8_ap
 #pragma unroll
         for (int w = 0; w < kWords; ++w) raw[k * kWords + w] = i < items ? __ldg(piece(i) + w) : make_uint4(0, 0, 0, 0);
       }
+      met = look();  // while the values are on their way
       // magnitudes compare as integers; only a run with an infinity or a NaN is looked at element by element
       uint32_t top = 0;
 #pragma unroll
@@ -490,6 +504,7 @@ __global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 2 ? 8 : 4) kv8_ap
         }
       }
     } else {
+      met = look();
 #pragma unroll 2
       for (int i = tid; i < items; i += kAppendThreads) {
         float x[8];
@@ -500,8 +515,7 @@ __global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 2 ? 8 : 4) kv8_ap
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
     if (lane == 0) s_most[turn][warp] = most;
-    __syncthreads();  // also: all have read the old scale
-    if (s_conflict[turn]) {
+    if (__syncthreads_or(met)) {  // also: all have read the old scale
       if (tid == 0) raise_error(a.err, QQ_DEV_ERR_BOUNDS);
       continue;
     }
@@ -556,7 +570,7 @@ __global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 2 ? 8 : 4) kv8_ap
     }
     if (tid == 0) *scale = now;
   }
-  if (tid == 0) count_cta(c.state);  // its epoch was read long ago
+  if (tid == 0 && blockIdx.x == 0 && blockIdx.y == 0) atomicAdd(c.state + 1, 1u);
 }
 
 // ------------------------------------------------------------------ gather
@@ -718,15 +732,21 @@ extern "C" int qq_kv8_append(const qq_kv8_cache* cache, const void* k, const voi
   a.n = num_tokens;
   a.err = err;
   // A token per CTA column while there are few (each may be its own run), wider
-  // windows for a prefill, whose runs are whole blocks: about 512 columns.
+  // windows for a prefill, whose runs are whole blocks: about kLookTokens columns.
   a.window = 1;
-  while (a.window < kMaxWindow && num_tokens > 512 * (int64_t)a.window) a.window *= 2;
+  while (a.window < kMaxWindow && num_tokens > kLookTokens * a.window) a.window *= 2;
+  a.claimed = num_tokens > kLookTokens;
   const int64_t ctas = (num_tokens + a.window - 1) / a.window;
   const int pairs = 2 * cache->kv_heads;
-  if (ctas * pairs > INT32_MAX || pairs > 65535) return QQ_ERR_UNSUPPORTED;
+  if (num_tokens > INT32_MAX || pairs > 65535) return QQ_ERR_UNSUPPORTED;
   const dim3 grid((unsigned)ctas, pairs);
   const bool d128 = cache->head_dim == 128;
   cudaStream_t s = as_stream(stream);
+  if (a.claimed) {
+    const dim3 claim_grid((unsigned)((num_tokens + kClaimThreads - 1) / kClaimThreads));
+    rc = launch_pdl(kv8_claim_kernel, claim_grid, dim3(kClaimThreads), 0, s, a.c, slots, num_tokens);
+    if (rc != QQ_OK) return rc;
+  }
   if (dtype == QQ_BF16)
     return d128 ? launch_pdl(kv8_append_kernel<__nv_bfloat16, 128>, dim3(grid), dim3(kAppendThreads), 0, s, a)
                 : launch_pdl(kv8_append_kernel<__nv_bfloat16, 0>, dim3(grid), dim3(kAppendThreads), 0, s, a);

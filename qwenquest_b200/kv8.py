@@ -299,7 +299,7 @@ class KV8Cache(_OnDevice):
 
         A slot of -1 skips its token.  The tokens of a block stand next to each other in ascending slots, as
         :meth:`BlockTables.plan` gives them; a block met twice in one call is an error, raised at the next
-        check.  A block's scale is a power of two that only grows until a token is written at its offset 0.
+        check, and only the first stretch is written.  A block's scale is a power of two that only grows until a token is written at its offset 0.
         """
         if self._err_word.value:
             self.check_errors()

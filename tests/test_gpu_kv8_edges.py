@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from oracle import kv8 as oracle
-from qwenquest_b200.kv8 import BlockTables
+from qwenquest_b200.kv8 import BlockTables, KV8Cache
 
 pytestmark = pytest.mark.gpu
 
@@ -36,3 +36,130 @@ def test_a_padding_entry_may_name_a_live_request(reqs, live, grow):
     assert slots.tolist() == w_slots.tolist() and offsets.tolist() == w_offsets.tolist()
     assert tables.block_table.tolist() == ref.table.tolist() and tables.held.tolist() == ref.held.tolist()
     assert not tables._claim.any()
+
+
+# ---------------------------------------------------------------- append
+
+
+class _Twin:
+    """An empty cache and its numpy twin."""
+
+    def __init__(self, blocks, kv, block, dim):
+        self.cache = KV8Cache(1, blocks, kv, dim, DEV, block_size=block)
+        self.codes = [np.zeros((blocks, kv, block, dim), dtype=np.uint8) for _ in range(2)]
+        self.scales = [np.zeros((blocks, kv), dtype=np.float32) for _ in range(2)]
+
+    def put(self, x, slots):
+        for c, s in zip(self.codes, self.scales):
+            oracle.append(c, s, x.double().cpu().numpy(), np.asarray(slots))
+
+    def check(self):
+        got = (self.cache.k[0], self.cache.v[0]), (self.cache.k_scale[0], self.cache.v_scale[0])
+        for g, want in zip(got[0], self.codes):
+            assert np.array_equal(g.view(torch.uint8).cpu().numpy(), want)
+        for g, want in zip(got[1], self.scales):
+            assert np.array_equal(g.cpu().numpy(), want)
+        assert not self.cache._state[0, 2:].any()  # no claim is left
+
+
+def test_appends_that_continue_their_blocks_beside_a_long_one():
+    """A call of slow thread blocks, more than fit at a time (64 tokens each, a block per token), and on another stream
+    calls of more blocks than the first one leaves room for: each continues the blocks of the one before it."""
+    block, kv, dim, long, mine, steps = 16, 1, 32, 1 << 16, 1024, 14
+    rng = np.random.default_rng(0)
+    twin = _Twin(long + mine, kv, block, dim)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+
+    def call(slots):
+        x = torch.from_numpy(rng.standard_normal((len(slots), kv, dim))).to(torch.bfloat16)
+        return x, slots, x.to(DEV), _dev(slots)
+
+    calls = [[call(mine * block + np.arange(long) * block)],
+             [call(rng.permutation(mine) * block + step) for step in range(steps)]]
+    graphs = []
+    for todo, stream in zip(calls, streams):
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=stream):
+            for _, _, x, slots in todo:
+                twin.cache.append(0, x, x, slots)
+    for _ in range(10):  # each replay starts its blocks anew
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    twin.cache.check_errors()
+    for x, slots, _, _ in calls[1]:
+        twin.put(x, slots)
+    x, slots, _, _ = calls[0][0]
+    for part in np.split(np.arange(long), 1 << 6)[::9]:
+        twin.put(x[torch.from_numpy(part)], slots[part])
+    seen = np.concatenate([np.arange(mine), mine + np.concatenate(np.split(np.arange(long), 1 << 6)[::9])])
+    for got, want in zip((twin.cache.k[0], twin.cache.v[0]), twin.codes):
+        assert np.array_equal(got.view(torch.uint8).cpu().numpy()[seen], want[seen])
+
+
+@pytest.mark.parametrize("n", [2, 511, 512, 513, 3000])
+def test_the_first_stretch_of_a_block_is_written(n):
+    """Blocks met again at every distance, in calls that look for them and in calls that claim them."""
+    block, kv, dim, blocks = 16, 2, 16, n + 4
+    rng = np.random.default_rng(n)
+    twin = _Twin(blocks, kv, block, dim)
+    slots = rng.permutation(blocks)[:n] * block + 3
+    again = np.sort(rng.permutation(n - 1)[:max(1, n // 20)]) + 1
+    for t in again:  # at another offset of a block met before, which may be that of a skipped token
+        slots[t] = slots[rng.integers(0, t)] // block * block + rng.integers(0, block)
+    kept, seen = [], set()
+    for t, s in enumerate(slots):
+        run_on = t > 0 and s % block and slots[t - 1] == s - 1
+        if run_on:
+            kept.append(kept[-1])
+            continue
+        kept.append(s // block not in seen)
+        seen.add(s // block)
+    kept = np.array(kept)
+    x = torch.from_numpy(rng.standard_normal((n, kv, dim))).to(torch.bfloat16)
+    for _ in range(2):
+        twin.cache.append(0, x.to(DEV), x.to(DEV), _dev(slots))
+        torch.cuda.synchronize()
+        if not kept.all():
+            with pytest.raises(RuntimeError):
+                twin.cache.check_errors()
+        twin.put(x[torch.from_numpy(kept)], slots[kept])
+        twin.check()
+
+
+def test_a_captured_append_replays_beside_eager_ones():
+    """Replays in which a block is met twice, or not, of few and of many tokens, with a call of another stream between."""
+    block, kv, dim, blocks = 16, 2, 16, 2000
+    rng = np.random.default_rng(3)
+    for n in (40, 900):
+        twin = _Twin(blocks, kv, block, dim)
+        x = torch.from_numpy(rng.standard_normal((n, kv, dim))).to(torch.bfloat16).to(DEV)
+        slots = torch.zeros(n, dtype=torch.int64, device=DEV)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            twin.cache.append(0, x, x, slots)
+        other = torch.cuda.Stream()
+        for step in range(5):
+            mine = rng.permutation(900)[:n] * block + step
+            if step == 2:
+                mine[n - 1] = mine[0] + 1 + block // 2
+            slots.copy_(_dev(mine))
+            theirs = (1000 + rng.permutation(900)[:n]) * block + step
+            y = torch.from_numpy(rng.standard_normal((n, kv, dim))).to(torch.bfloat16).to(DEV)
+            theirs_dev = _dev(theirs)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(other):
+                twin.cache.append(0, y, y, theirs_dev)
+            graph.replay()
+            torch.cuda.synchronize()
+            if step == 2:
+                with pytest.raises(RuntimeError):
+                    twin.cache.check_errors()
+                mine = mine[:-1]
+            twin.cache.check_errors()
+            twin.put(x[:len(mine)], mine)
+            twin.put(y, theirs)
+            twin.check()
