@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 2 ? 8 : 4) kv8_ap
     if (tid < a.window && w0 + tid < a.n) {
       const int64_t slot = s_slots[tid + 1];
       head = run_head(c, slot, s_slots[tid]);
-      if (slot >= total) {
+      if (slot >= total || slot < -1) {
         raise_error(a.err, QQ_DEV_ERR_BOUNDS);
         head = false;
       }

@@ -163,3 +163,19 @@ def test_a_captured_append_replays_beside_eager_ones():
             twin.put(x[:len(mine)], mine)
             twin.put(y, theirs)
             twin.check()
+
+
+@pytest.mark.parametrize("n", [4, 700])
+def test_append_reports_a_negative_slot_that_is_no_padding(n):
+    """-1 skips a token; -2 and below are out of range, the other tokens are written."""
+    for bad in (-2, -5, -(1 << 40)):
+        twin = _Twin(n, 1, 16, 16)
+        slots = np.arange(n) * 16
+        slots[1], slots[n - 1] = -1, bad
+        x = torch.randn(n, 1, 16, generator=torch.Generator().manual_seed(n))
+        twin.cache.append(0, x.to(DEV), x.to(DEV), _dev(slots))
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError):
+            twin.cache.check_errors()
+        twin.put(x[: n - 1], slots[: n - 1])
+        twin.check()
