@@ -301,8 +301,9 @@ typedef struct qq_block_tables {
  * new tokens, slots[token_offsets[i] + t] the slot of position prefix + t, and
  * slots behind the last new token -1 (num_slots is what the caller made room
  * for; more new tokens than that are QQ_DEV_ERR_BOUNDS).  req_to_token (null:
- * none; int32 [map_rows][map_stride]) gets the same slots by request and
- * position, the table the page selection translates through.  An entry of
+ * none; int32 [map_rows][map_stride], of which any column may be written) gets
+ * the same slots by request and position, the table the page selection
+ * translates through.  An entry of
  * seq_lens 0 is padding, whatever request it names.  A request past the ring's free blocks (the sum in
  * batch order) gets none, slots of -1 and QQ_DEV_ERR_CAPACITY; a bad length, a
  * request out of range or named a second time likewise with

@@ -176,8 +176,8 @@ class BlockTables(_OnDevice):
 
         Returns ``(slots, token_offsets)``: int64 ``[num_tokens]``, the slot of every new token in batch order
         (-1 behind the last one, and for an entry that is refused), and int64 ``[bs + 1]``, the first row of each
-        entry.  An entry of ``seq_lens`` 0 is padding.  ``req_to_token`` (int32 ``[rows, max_context]``) gets
-        the slots by request and position.  A batch that runs out of blocks raises ``RuntimeError`` at the next
+        entry.  An entry of ``seq_lens`` 0 is padding.  ``req_to_token`` (int32 ``[rows, max_context]``; columns
+        of a wider map where they hold ``max_blocks * block_size`` positions) gets the slots by request and position.  A batch that runs out of blocks raises ``RuntimeError`` at the next
         check; the entries that no longer fit are left as they were.
         """
         if self._err_word.value:
@@ -193,13 +193,21 @@ class BlockTables(_OnDevice):
         slots, offsets = made.split_with_sizes((num_tokens, bs + 1))
         mapped = (None, 0, 0)
         if req_to_token is not None:
-            if (req_to_token.dim() != 2 or req_to_token.dtype != torch.int32 or req_to_token.stride(1) != 1
-                    or req_to_token.device != self.device):
-                raise ValueError("req_to_token must be int32 [rows, max_context] with contiguous rows on the device")
-            mapped = (req_to_token.data_ptr(), req_to_token.stride(0), req_to_token.shape[0])
+            mapped = self._map(req_to_token)
         self._call(self.lib.qq_block_plan, self._tables, reqs.data_ptr(), seq.data_ptr(), prefix.data_ptr(), bs,
                    made.data_ptr(), num_tokens, made.data_ptr() + 8 * num_tokens, *mapped, self._err_ptr)
         return slots, offsets
+
+    def _map(self, t: torch.Tensor) -> tuple[int, int, int]:
+        """The map's address, the distance between its rows and their number.  The kernel takes the distance as a
+        row's length, so rows that are part of wider ones must hold every position the tables can."""
+        if t.dim() != 2 or t.dtype != torch.int32 or t.device != self.device or (t.shape[1] > 1 and t.stride(1) != 1):
+            raise ValueError("req_to_token must be int32 [rows, max_context] with contiguous rows on the device")
+        rows, width = t.shape
+        stride = t.stride(0) if rows > 1 else width
+        if stride < width or (stride > width and width < self.max_blocks * self.block_size):
+            raise ValueError(f"req_to_token must be contiguous, or at least {self.max_blocks * self.block_size} wide")
+        return t.data_ptr(), stride, rows
 
     def trim(self, req_pool_indices, keep_lens=None) -> None:
         """Requests keep the blocks of their first ``keep_lens[i]`` tokens (``None``: of none, they are finished);

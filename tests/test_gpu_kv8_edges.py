@@ -38,6 +38,43 @@ def test_a_padding_entry_may_name_a_live_request(reqs, live, grow):
     assert not tables._claim.any()
 
 
+def test_a_map_of_some_columns_keeps_the_others():
+    """Columns of a wider map: refused where a request may outgrow them, else filled without a word beside them."""
+    tables = BlockTables(20, 3, 4, DEV, block_size=16)
+    big = torch.full((4, 200), -9, dtype=torch.int32, device=DEV)
+    args = [0, 2], [40, 64], [0, 0], 104
+    for narrow in (big[:3, 8:48], big[:3, 150:], big[:, :63], big[:1].expand(3, -1), big[:, ::2]):
+        with pytest.raises(ValueError, match="req_to_token"):
+            tables.plan(*args, req_to_token=narrow)
+    assert (big == -9).all() and tables.available() == 20
+    slots, _ = tables.plan(*args, req_to_token=big[:3, 8:72])
+    tables.synchronize()
+    assert big[0, 8:48].tolist() == slots[:40].tolist() and big[2, 8:72].tolist() == slots[40:].tolist()
+    big[0, 8:48], big[2, 8:72] = -9, -9
+    assert (big == -9).all()
+    # a map of its own that is shorter than the tables: what fits is written, the rest reported
+    short = torch.full((3, 50), -9, dtype=torch.int32, device=DEV)
+    again, _ = tables.plan([2], [64], [30], 34, req_to_token=short)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError):
+        tables.check_errors()
+    assert again.tolist() == slots[70:].tolist() and short[2, 30:].tolist() == again[:20].tolist()
+    short[2, 30:] = -9
+    assert (short == -9).all()
+
+
+def test_a_map_of_one_row():
+    """The distance between the rows of one row is any number."""
+    big = torch.full((100,), -9, dtype=torch.int32, device=DEV)
+    for stride in (0, 1, 64, 1000):
+        tables = BlockTables(20, 1, 4, DEV, block_size=16)
+        one = big.as_strided((1, 64), (stride, 1))
+        slots, _ = tables.plan([0], [64], [0], 64, req_to_token=one)
+        tables.synchronize()
+        assert one[0].tolist() == slots.tolist()
+    assert (big[64:] == -9).all()
+
+
 # ---------------------------------------------------------------- append
 
 
