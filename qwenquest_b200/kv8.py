@@ -142,9 +142,13 @@ class BlockTables(_OnDevice):
     def _setup(self, block_table, held, free_blocks, ring, block_size) -> None:
         if block_size not in BLOCK_SIZES:
             raise ValueError(f"block_size must be one of {BLOCK_SIZES}, got {block_size}")
-        if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1:
+        if block_table.dim() != 2 or block_table.dtype != torch.int32:
             raise ValueError("block_table must be int32 [max_reqs, max_blocks] with contiguous rows")
         reqs, width = block_table.shape
+        # what stride() says of a dimension of size 1 is any number
+        stride = block_table.stride(0) if reqs > 1 else width
+        if (width > 1 and block_table.stride(1) != 1) or stride < width:
+            raise ValueError("block_table must be int32 [max_reqs, max_blocks] with contiguous rows")
         for name, t, dtype, shape in (("held", held, torch.int32, (reqs,)), ("ring", ring, torch.int64, (2,)),
                                       ("free_blocks", free_blocks, torch.int32, (free_blocks.numel(),))):
             if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.device != block_table.device:
@@ -154,7 +158,7 @@ class BlockTables(_OnDevice):
         self.block_size, self.max_reqs, self.max_blocks = block_size, reqs, width
         self._claim = torch.zeros(reqs, dtype=torch.int32, device=self.device)
         self._tables = _lib.QQBlockTables(
-            block_table.data_ptr(), block_table.stride(0), held.data_ptr(), self._claim.data_ptr(),
+            block_table.data_ptr(), stride, held.data_ptr(), self._claim.data_ptr(),
             free_blocks.data_ptr(), ring.data_ptr(), free_blocks.numel(), reqs, width, block_size)
 
     def check_errors(self) -> None:
@@ -420,7 +424,7 @@ class KV8Cache(_OnDevice):
         top = rows.shape[1]
         size = self._workspace(heads, code, bs, bs, top, 0)
         self._call_with_scratch(size, self.lib.qq_kv8_sparse_attention, self._layers[layer], bs, rows.data_ptr(),
-                                rows.stride(0), top, lens.data_ptr(), q_ptr, code, heads, q_stride, float(scaling),
+                                max(rows.stride(0), top), top, lens.data_ptr(), q_ptr, code, heads, q_stride, float(scaling),
                                 out.data_ptr(), out_stride, self._err_ptr)
         return out
 

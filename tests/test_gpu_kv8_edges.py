@@ -75,6 +75,45 @@ def test_a_map_of_one_row():
     assert (big[64:] == -9).all()
 
 
+@pytest.mark.parametrize("stride", [0, 1, 7])
+def test_tables_of_one_row_or_one_column(stride):
+    """What a tensor says of the stride of a dimension of size 1 is any number."""
+    for shape, strides, grow in (((1, 4), (stride, 1), 60), ((3, 1), (1, stride), 10)):
+        table = torch.full((9,), -1, dtype=torch.int32, device=DEV)
+        held = torch.zeros(shape[0], dtype=torch.int32, device=DEV)
+        tables = BlockTables.from_tensors(table.as_strided(shape, strides), held, torch.arange(8, dtype=torch.int32, device=DEV),
+                                          torch.tensor([0, 8], device=DEV), 16)
+        n = shape[0]
+        slots, _ = tables.plan(list(range(n)), [grow] * n, [0] * n, n * grow)
+        tables.synchronize()
+        pages = -(-grow // 16)
+        assert table[:n * pages].tolist() == list(range(n * pages)) and (table[n * pages:] == -1).all()
+        assert slots.tolist() == [i * pages * 16 + t for i in range(n) for t in range(grow)]
+        tables.trim(list(range(n)))
+        tables.synchronize()
+        assert (table == -1).all() and tables.available() == 8
+    wide = torch.zeros(1, 4, dtype=torch.int32, device=DEV).expand(3, -1)
+    with pytest.raises(ValueError, match="block_table"):
+        BlockTables.from_tensors(wide, held, torch.arange(8, dtype=torch.int32, device=DEV), torch.tensor([0, 8], device=DEV), 16)
+
+
+@pytest.mark.parametrize("stride", [0, 1, 1000])
+def test_selected_rows_of_one_request(stride):
+    """The same of the rows of one request, and of one row of each."""
+    cache = KV8Cache(1, 8, 2, 128, DEV, block_size=16)
+    x = torch.randn(100, 2, 128, device=DEV).to(torch.bfloat16)
+    cache.append(0, x, x, torch.arange(100, device=DEV))
+    q = torch.randn(3, 8, 128, device=DEV).to(torch.bfloat16)
+    rows = torch.arange(100, dtype=torch.int32, device=DEV)
+    want = cache.sparse_decode_attention(0, q[:1], rows.view(1, 100), [90], 0.1)
+    got = cache.sparse_decode_attention(0, q[:1], rows.as_strided((1, 100), (stride, 1)), [90], 0.1)
+    assert torch.equal(got, want)
+    want = cache.sparse_decode_attention(0, q, rows[:3].view(3, 1).clone(), [1] * 3, 0.1)
+    got = cache.sparse_decode_attention(0, q, rows.as_strided((3, 1), (1, stride)), [1] * 3, 0.1)
+    assert torch.equal(got, want)
+    cache.synchronize()
+
+
 # ---------------------------------------------------------------- append
 
 
