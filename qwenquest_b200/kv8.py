@@ -40,6 +40,16 @@ __all__ = ["BlockTables", "KV8Cache"]
 BLOCK_SIZES = (16, 32, 64, 128)
 
 
+def _as_int(t: torch.Tensor, dtype: torch.dtype, name: str, device: torch.device) -> torch.Tensor:
+    """Integers of another type or place.  Narrowed to 32 bits, those past them become the nearest, which the kernels
+    find out of range; cut off they might be numbers in range."""
+    if t.numel() and (t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool):
+        raise ValueError(f"{name}: integers are wanted, got {t.dtype}")
+    if dtype == torch.int32 and t.dtype.itemsize >= 4 and t.dtype != torch.int32:
+        t = t.to(device=device, dtype=torch.int64).clamp(-2 ** 31, 2 ** 31 - 1)
+    return t.to(device=device, dtype=dtype)
+
+
 def _cuda_device(device) -> torch.device:
     device = torch.device(device)
     if device.type != "cuda":
@@ -106,9 +116,7 @@ class _OnDevice:
         if not isinstance(t, torch.Tensor):
             t = torch.as_tensor(t)
         if t.dtype != dtype or t.get_device() != self._index:
-            if t.numel() and (t.dtype.is_floating_point or t.dtype == torch.bool):
-                raise ValueError(f"{name}: integers are wanted, got {t.dtype}")
-            t = t.to(device=self.device, dtype=dtype)
+            t = _as_int(t, dtype, name, self.device)
         if t.dim() != 1 or (n is not None and t.shape[0] != n):
             raise ValueError(f"{name} must be [{'n' if n is None else n}], got {tuple(t.shape)}")
         return t if t.is_contiguous() else t.contiguous()
@@ -418,8 +426,10 @@ class KV8Cache(_OnDevice):
         code = dtype_code(q.dtype)
         if rows.dim() != 2 or rows.shape[0] != bs or rows.shape[1] == 0 or rows.get_device() != self._index:
             raise ValueError(f"rows must be int32 [{bs}, top_k] on {self.device}, got {tuple(rows.shape)}")
-        if rows.dtype != torch.int32 or rows.stride(1) != 1 or rows.stride(0) < rows.shape[1]:
-            rows = rows.to(torch.int32).contiguous()
+        if rows.dtype != torch.int32:
+            rows = _as_int(rows, torch.int32, "rows", self.device)
+        if rows.stride(1) != 1 or rows.stride(0) < rows.shape[1]:
+            rows = rows.contiguous()
         lens = self._ints(lens, torch.int32, "lens", bs)
         top = rows.shape[1]
         size = self._workspace(heads, code, bs, bs, top, 0)

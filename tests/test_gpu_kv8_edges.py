@@ -114,6 +114,34 @@ def test_selected_rows_of_one_request(stride):
     cache.synchronize()
 
 
+def test_selected_rows_past_32_bits_are_reported():
+    """int64 rows and lengths: what lies past 32 bits takes no part and is reported, and is not cut off to a valid row."""
+    cache = KV8Cache(1, 8, 2, 128, DEV, block_size=16)
+    x = torch.randn(100, 2, 128, device=DEV).to(torch.bfloat16)
+    cache.append(0, x, x, torch.arange(100, device=DEV))
+    q = torch.randn(2, 8, 128, device=DEV).to(torch.bfloat16)
+    rows = torch.arange(60, device=DEV).view(2, 30)
+    want = cache.sparse_decode_attention(0, q, rows.to(torch.int32), [30, 30], 0.1)
+    assert torch.equal(cache.sparse_decode_attention(0, q, rows, _dev([30, 30]), 0.1), want)
+    cache.synchronize()
+    few = torch.cat([rows[:, :5], torch.full((2, 1), -1, device=DEV), rows[:, 6:]], 1)
+    want = cache.sparse_decode_attention(0, q, few, [30, 30], 0.1)
+    far = rows.clone()
+    far[:, 5] = 2 ** 32 + 99
+    got = cache.sparse_decode_attention(0, q, far, [30, 30], 0.1)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError):
+        cache.check_errors()
+    assert torch.equal(got, want)
+    got = cache.sparse_decode_attention(0, q, rows, _dev([30, 2 ** 32 + 3]), 0.1)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError):
+        cache.check_errors()
+    assert not got[1].any()
+    with pytest.raises(ValueError, match="integers are wanted"):
+        cache.sparse_decode_attention(0, q, rows.float(), [30, 30], 0.1)
+
+
 # ---------------------------------------------------------------- append
 
 
