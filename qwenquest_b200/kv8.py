@@ -171,10 +171,14 @@ class BlockTables(_OnDevice):
 
     def check_errors(self) -> None:
         """Raise for device errors of earlier calls (no synchronisation)."""
-        if self._err_word.value & _lib.QQ_DEV_ERR_CAPACITY:
-            self._err.take()
-            raise RuntimeError("no free block left: some requests of an earlier plan got none")
-        super().check_errors()
+        if not self._err_word.value & _lib.QQ_DEV_ERR_CAPACITY:
+            return super().check_errors()
+        others = self._err.take() & ~_lib.QQ_DEV_ERR_CAPACITY
+        try:
+            _lib.raise_device_error(others, self._what)
+        except RuntimeError as other:
+            raise RuntimeError(f"no free block left: some requests of an earlier plan got none; and {other}") from other
+        raise RuntimeError("no free block left: some requests of an earlier plan got none")
 
     def available(self) -> int:
         """Free blocks (reads the device, so it waits)."""

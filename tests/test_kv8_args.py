@@ -2,12 +2,14 @@
 
 from __future__ import annotations
 
+import ctypes
 from types import SimpleNamespace
 
 import pytest
 import torch
 
-from qwenquest_b200 import kv8
+from qwenquest_b200 import _lib, kv8
+from qwenquest_b200._device import DeviceError
 
 HOST = SimpleNamespace(device=torch.device("cpu"), _index=-1)
 
@@ -36,3 +38,19 @@ def test_what_is_no_integer_is_refused(other):
     for dtype in (torch.int32, torch.int64):
         with pytest.raises(ValueError, match="integers are wanted"):
             kv8._OnDevice._ints(HOST, torch.ones(2, dtype=other), dtype, "lens")
+
+
+def test_errors_beside_a_full_ring_are_named_too():
+    """One batch may run out of blocks and name a bad request: both are raised, once."""
+    tables = kv8.BlockTables.__new__(kv8.BlockTables)
+    tables._err = DeviceError(torch.zeros(1, dtype=torch.int32))
+    tables._err_word = ctypes.c_int32.from_address(tables._err.word.data_ptr())
+    tables._what = "(block tables)"
+    full, bounds = _lib.QQ_DEV_ERR_CAPACITY, _lib.QQ_DEV_ERR_BOUNDS
+    for bits, said in ((full, ["no free block"]), (full | bounds, ["no free block", "out of range"]), (bounds, ["out of range"])):
+        tables._err.word[0] = bits
+        with pytest.raises(RuntimeError) as raised:
+            tables.check_errors()
+        assert all(text in str(raised.value) for text in said)
+        assert ("no free block" in str(raised.value)) == bool(bits & full)
+        tables.check_errors()
