@@ -71,7 +71,12 @@ __device__ inline TableSmem table_smem(void* p, int bs) {
   return s;
 }
 
-// Exclusive sums over the block of one (int64, int32) pair per thread; totals to all threads.
+// Counts of blocks, which stop at INT_MAX: 4,096 entries may ask for more than 2^31 between them.
+__device__ __forceinline__ int32_t add_counts(int32_t x, int32_t y) {
+  return (int32_t)min((uint32_t)x + (uint32_t)y, (uint32_t)INT_MAX);
+}
+
+// Exclusive sums over the block of one (int64, count of blocks) pair per thread; totals to all threads.
 __device__ void block_scan(int64_t& a, int32_t& b, int64_t& a_total, int32_t& b_total) {
   __shared__ int64_t sa[32];
   __shared__ int32_t sb[32];
@@ -82,9 +87,10 @@ __device__ void block_scan(int64_t& a, int32_t& b, int64_t& a_total, int32_t& b_
   for (int o = 1; o < 32; o <<= 1) {
     const int64_t ua = __shfl_up_sync(0xffffffffu, ia, o);
     const int32_t ub = __shfl_up_sync(0xffffffffu, ib, o);
-    if (lane >= o) ia += ua, ib += ub;
+    if (lane >= o) ia += ua, ib = add_counts(ib, ub);
   }
   if (lane == 31) sa[warp] = ia, sb[warp] = ib;
+  const int32_t before = __shfl_up_sync(0xffffffffu, ib, 1);
   __syncthreads();
   if (warp == 0) {
     int64_t wa = sa[lane];
@@ -93,14 +99,14 @@ __device__ void block_scan(int64_t& a, int32_t& b, int64_t& a_total, int32_t& b_
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t ua = __shfl_up_sync(0xffffffffu, wa, o);
       const int32_t ub = __shfl_up_sync(0xffffffffu, wb, o);
-      if (lane >= o) wa += ua, wb += ub;
+      if (lane >= o) wa += ua, wb = add_counts(wb, ub);
     }
     sa[lane] = wa, sb[lane] = wb;
   }
   __syncthreads();
   a_total = sa[31], b_total = sb[31];
   a = ia - a + (warp ? sa[warp - 1] : 0);
-  b = ib - b + (warp ? sb[warp - 1] : 0);
+  b = add_counts(lane ? before : 0, warp ? sb[warp - 1] : 0);
 }
 
 // The last i in [0, n) with sums[i] <= x (sums ascending, sums[0] <= x).
@@ -147,7 +153,7 @@ __global__ void __launch_bounds__(kTableThreads) block_plan_kernel(TableArgs a) 
   wait_prior_grid();
   allow_next_grid();
   claim_requests(a, a.seq);
-  const int64_t head = a.ring[0], free_count = a.ring[1] - head;
+  const int64_t head = a.ring[0], free_count = min(a.ring[1] - head, (int64_t)INT_MAX - 1);
 
   // ---- this thread's entries: new tokens and blocks to take
   int64_t toks[kTablePer], my_toks = 0;
@@ -178,7 +184,7 @@ __global__ void __launch_bounds__(kTableThreads) block_plan_kernel(TableArgs a) 
     s.held[i] = held;
     s.pre[i] = pre;
     my_toks += toks[j];
-    my_need += need[j];
+    my_need = add_counts(my_need, need[j]);
   }
   int64_t tok_at = my_toks, tok_total;
   int32_t need_at = my_need, need_total;
@@ -190,7 +196,7 @@ __global__ void __launch_bounds__(kTableThreads) block_plan_kernel(TableArgs a) 
     s.off[i] = tok_at;
     s.sum[i] = need_at;
     tok_at += toks[j];
-    need_at += need[j];
+    need_at = add_counts(need_at, need[j]);
     if (need[j] > 0) {
       if (need_at <= free_count) {
         atomicMax(&s_taken, need_at);
@@ -257,7 +263,7 @@ __global__ void __launch_bounds__(kTableThreads) block_trim_kernel(TableArgs a) 
   wait_prior_grid();
   allow_next_grid();
   claim_requests(a, nullptr);
-  const int64_t tail = a.ring[1], room = a.capacity - (tail - a.ring[0]);
+  const int64_t tail = a.ring[1], room = min(a.capacity - (tail - a.ring[0]), (int64_t)INT_MAX - 1);
   int32_t back[kTablePer], my_back = 0;
   const int per = (a.bs + kTableThreads - 1) / kTableThreads;
 #pragma unroll
@@ -280,7 +286,7 @@ __global__ void __launch_bounds__(kTableThreads) block_trim_kernel(TableArgs a) 
     }
     s.req[i] = req;
     s.held[i] = held;
-    my_back += back[j];
+    my_back = add_counts(my_back, back[j]);
   }
   int64_t none = 0, none_total;
   int32_t at = my_back, total;
@@ -290,7 +296,7 @@ __global__ void __launch_bounds__(kTableThreads) block_trim_kernel(TableArgs a) 
     const int i = tid * per + j;
     if (j >= per || i >= a.bs) continue;
     s.sum[i] = at;
-    at += back[j];
+    at = add_counts(at, back[j]);
   }
   if (tid == 0) s.sum[a.bs] = total;
   __syncthreads();

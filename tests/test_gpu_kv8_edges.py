@@ -114,6 +114,37 @@ def test_selected_rows_of_one_request(stride):
     cache.synchronize()
 
 
+def test_a_plan_that_asks_for_more_than_31_bits_of_blocks():
+    """Each request may hold 2^29 blocks; five of them want 2^31 and more between them, and the ring has 20."""
+    width = 1 << 29
+    i32 = dict(dtype=torch.int32, device=DEV)
+    table, held, free = torch.empty(6, width, **i32), torch.zeros(6, **i32), torch.arange(100, 120, **i32)
+    tables = BlockTables.from_tensors(table, held, free, torch.tensor([0, 20], device=DEV), 16)
+    for first in (0, 5000):  # the slots by one thread block, and by a grid
+        reqs, seq = [5, 0, 1, 2, 3, 4], [first + 20] + [width * 16] * 5
+        prefix = [0] + [width * 16 - 1] * 5
+        if first:
+            seq[0], prefix[0] = 40, 20
+        n = first + 25
+        slots, offsets = tables.plan(reqs, seq, prefix, n)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="no free block"):
+            tables.check_errors()
+        at = prefix[0]
+        assert slots[:20].tolist() == [(100 + p // 16) * 16 + p % 16 for p in range(at, at + 20)]
+        assert (slots[20:] == -1).all() and offsets.tolist() == [0, 20, 21, 22, 23, 24, 25]
+        pages = -(-seq[0] // 16)
+        assert held.tolist() == [0, 0, 0, 0, 0, pages] and tables.ring.tolist() == [pages, 20]
+        assert table[5, :pages].tolist() == list(range(100, 100 + pages))
+    # lengths the table never had: nothing goes back to the ring
+    held[:5] = width
+    tables.trim([5, 0, 1, 2, 3, 4])
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError):
+        tables.check_errors()
+    assert held.tolist() == [width] * 5 + [3] and tables.ring.tolist() == [3, 20] and free.tolist() == list(range(100, 120))
+
+
 def test_selected_rows_past_32_bits_are_reported():
     """int64 rows and lengths: what lies past 32 bits takes no part and is reported, and is not cut off to a valid row."""
     cache = KV8Cache(1, 8, 2, 128, DEV, block_size=16)
