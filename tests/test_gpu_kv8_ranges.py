@@ -21,6 +21,7 @@ import torch
 
 from oracle import kv8 as oracle
 from qwenquest_b200.kv8 import KV8Cache
+from tests.test_gpu_kv8 import GEOMETRIES, _Batch
 
 pytestmark = pytest.mark.gpu
 
@@ -171,3 +172,47 @@ def test_a_lone_request_of_131072_keys(heads, kv):
     k, v = (oracle.rows(c, x, slots) for c, x in zip(codes, scales))
     for got in (out, rows):
         _check(got[0], q[0], k, v, scales[1][slots // block], dim ** -0.5, "decode")
+
+
+@pytest.mark.parametrize(("kv", "heads", "dim", "block", "dtype"), GEOMETRIES)
+@pytest.mark.parametrize("seq", [[1, 63, 129, 700], [2600, 30]])
+def test_each_kernel_within_its_own_bound(kv, heads, dim, block, dtype, seq):
+    """Ordinary values, values of one sign (what is lost shows) and scales far apart, against the bound of the kernel
+    that runs: bf16 with head_dim 128 on the tensor cores, up to 16 heads to a KV head for one token; the rest in fp32."""
+    tc = dtype == torch.bfloat16 and dim == 128
+    one = "decode" if tc and heads // kv <= 16 else "fp32"
+    for kind in ("both signs", "one sign", "scales"):
+        def scales(rng, shape):
+            return (np.exp2(rng.integers(-20, 6, shape)) * (1 + rng.random(shape))).astype(np.float32)
+
+        b = _Batch(seq, kv, dim, block, seed=sum(seq) + dim + heads, heads=heads, dtype=dtype,
+                   scales=scales if kind == "scales" else None)
+        if kind == "scales":
+            b.ks[0] = np.where(np.isnan(b.ks[0]), b.ks[0], np.float32(2.0 ** -8))
+            b.cache.k_scale[0].copy_(torch.from_numpy(b.ks[0]))
+        if kind == "one sign":
+            b.v[0] &= 0x7F
+            b.cache.v[0].view(torch.uint8).copy_(torch.from_numpy(b.v[0]))
+        q = b.queries(len(seq))
+        args = b.table_dev, _dev(b.reqs), _dev(seq)
+        out = b.cache.decode_attention(0, q.to(DEV), *args, b.scaling)
+        rows = np.full((len(seq), max(seq)), -1, dtype=np.int64)
+        for i, s in enumerate(seq):
+            rows[i, :s] = b.slots(i, b.rng.permutation(s))
+        picked = b.cache.sparse_decode_attention(0, q.to(DEV), _dev(rows, torch.int32), _dev(seq, torch.int32), b.scaling)
+        new = [min(s, n) for s, n in zip(seq, (40, 30, 129, 300))]
+        offsets = np.concatenate([[0], np.cumsum(new)])
+        many = b.queries(int(offsets[-1]))
+        ext = b.cache.extend_attention(0, many.to(DEV), *args, _dev(np.subtract(seq, new)), _dev(offsets), b.scaling)
+        b.cache.synchronize()
+        for i, s in enumerate(seq):
+            at = b.slots(i, np.arange(s))
+            k, v = (oracle.rows(c, x, at) for c, x in ((b.k[0], b.ks[0]), (b.v[0], b.vs[0])))
+            v_scale = b.vs[0][at // block]
+            _check(out[i], q[i], k, v, v_scale, b.scaling, one)
+            order = np.argsort(at)[np.searchsorted(np.sort(at), rows[i, :s])]
+            _check(picked[i], q[i], k[order], v[order], v_scale[order], b.scaling, one)
+            for t in {0, new[i] // 2, new[i] - 1}:
+                n = s - new[i] + t + 1
+                row = offsets[i] + t
+                _check(ext[row], many[row], k[:n], v[:n], v_scale[:n], b.scaling, "extend" if tc else "fp32")
