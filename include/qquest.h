@@ -397,7 +397,7 @@ int qq_kv8_sparse_attention(const qq_kv8_cache* cache, int bs, const int32_t* ro
  * last sequence are left as they were, like those of an entry whose lengths,
  * offset or request do not fit (QQ_DEV_ERR_BOUNDS).  Entries share no query
  * rows: those that do leave them undefined, and more of it than num_tokens
- * and bs allow for is QQ_DEV_ERR_BOUNDS. */
+ * and bs allow for is QQ_DEV_ERR_BOUNDS.  table_stride * block_size <= 2^31 - 2^17. */
 int qq_kv8_extend_attention(const qq_kv8_cache* cache, const qq_extend_batch* batch, const int32_t* block_table,
                             int64_t table_stride, int64_t table_rows, const void* q, int dtype, int q_heads,
                             int64_t q_stride, float scaling, void* out, int64_t out_stride, uint32_t* err,

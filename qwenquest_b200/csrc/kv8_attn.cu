@@ -33,6 +33,7 @@ constexpr int kMostRows = 16;
 constexpr int kTileKeys = 64;
 constexpr int kAnyThreads = 128;
 constexpr int kMostSplits = 256;
+constexpr int64_t kSparePositions = 1 << 17;  // of an extend batch: 128 for each stretch of a row and the two tiles ahead
 
 struct AnyArgs {
   AttnArgs a;
@@ -618,7 +619,10 @@ extern "C" int qq_kv8_extend_attention(const qq_kv8_cache* cache, const qq_exten
   if (batch->req_pool_indices == nullptr || batch->seq_lens == nullptr || batch->prefix_lens == nullptr ||
       batch->token_offsets == nullptr || block_table == nullptr || table_stride <= 0 || table_rows <= 0)
     return QQ_ERR_INVALID;
-  if (batch->bs > QQ_MAX_BS || table_stride > INT32_MAX / kv8::kMaxBlock) return QQ_ERR_UNSUPPORTED;
+  // positions, and those of the key tiles asked for ahead or cut off behind the last one, are held in 32 bits
+  if (batch->bs > QQ_MAX_BS || table_stride > INT32_MAX / kv8::kMaxBlock ||
+      table_stride << a.c.shift > INT32_MAX - kSparePositions)
+    return QQ_ERR_UNSUPPORTED;
   a.bs = batch->bs;
   a.reqs = batch->req_pool_indices;
   a.seq = batch->seq_lens;

@@ -54,3 +54,27 @@ def test_errors_beside_a_full_ring_are_named_too():
         assert all(text in str(raised.value) for text in said)
         assert ("no free block" in str(raised.value)) == bool(bits & full)
         tables.check_errors()
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not _lib.LIB_PATH.exists():
+        import __graft_entry__
+
+        __graft_entry__.build()
+    return _lib.load()
+
+
+def test_extend_refuses_a_table_whose_positions_near_31_bits(lib):
+    """The kernel holds the positions of key tiles behind the last one in 32 bits too: 2^31 - 2^17 tokens at most."""
+    cache = _lib.QQKv8Cache(0x10000, 0x20000, 0x30000, 0x40000, 0x50000, 100, 4, 128, 128)
+    batch = _lib.QQExtendBatch(0x100, 0x200, 0x300, 0x400, None, 10, 1, 0)
+
+    def extend(stride, workspace=None):
+        return lib.qq_kv8_extend_attention(cache, batch, 0x300, stride, 2, 0x10000, _lib.QQ_BF16, 32, 4096, 0.1, 0x20000, 4096,
+                                           None, workspace, 0, None)
+
+    most = (2 ** 31 - 2 ** 17) // 128
+    for stride in (2 ** 24 - 1, 2 ** 24 - 2, most + 1):
+        assert extend(stride) == _lib.QQ_ERR_UNSUPPORTED
+    assert extend(most - 1) == _lib.QQ_ERR_WORKSPACE  # within the limit: the next check refuses
