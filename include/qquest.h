@@ -376,7 +376,8 @@ size_t qq_kv8_workspace_bytes(const qq_kv8_cache* cache, int q_heads, int dtype,
  * head runs on the tensor cores, anything else on the fp32 units.  On the
  * tensor cores a weight (times the scale of V) enters the product with 8 bits,
  * or as a multiple of 2^-21 of the largest one among its 128 keys (or of 2^-12
- * of the row's, where that is more). */
+ * of the row's, where that is more); kv_heads times the tiles of 128 keys that
+ * a request's row of the table (or of the list) has is below 2^31 there. */
 int qq_kv8_decode_attention(const qq_kv8_cache* cache, const qq_batch* batch, const int32_t* block_table,
                             int64_t table_stride, int64_t table_rows, const void* q, int dtype, int q_heads,
                             int64_t q_stride, float scaling, void* out, int64_t out_stride, uint32_t* err,

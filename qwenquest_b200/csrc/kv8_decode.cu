@@ -910,6 +910,8 @@ size_t decode_tc_workspace(int bs, int kv_heads, int group, int64_t max_keys) {
 }
 
 int run_decode_tc(const AttnArgs& a, int keys, int64_t max_keys, size_t ws_bytes, cudaStream_t s) {
+  // a share's place among the tiles of its entry's heads is held in 32 bits
+  if ((max_keys + kTile - 1) / kTile * a.c.kv_heads > INT32_MAX) return QQ_ERR_UNSUPPORTED;
   DecodeArgs g{};
   g.a = a;
   const int cluster = cluster_of(a.bs, a.c.kv_heads, a.group, max_keys);

@@ -78,3 +78,15 @@ def test_extend_refuses_a_table_whose_positions_near_31_bits(lib):
     for stride in (2 ** 24 - 1, 2 ** 24 - 2, most + 1):
         assert extend(stride) == _lib.QQ_ERR_UNSUPPORTED
     assert extend(most - 1) == _lib.QQ_ERR_WORKSPACE  # within the limit: the next check refuses
+
+
+def test_decode_refuses_more_tiles_than_31_bits_count(lib):
+    """All heads of one request's row: 2^24 tiles of 128 keys times 128 heads."""
+    def calls(kv, block, stride, top):
+        cache = _lib.QQKv8Cache(0x10000, 0x20000, 0x30000, 0x40000, 0x50000, 100, kv, 128, block)
+        tail = (0x10000, _lib.QQ_BF16, kv, kv * 128, 0.1, 0x20000, kv * 128, None, None, 0, None)
+        return (lib.qq_kv8_decode_attention(cache, _lib.QQBatch(0x100, 0x200, 1), 0x300, stride, 2, *tail),
+                lib.qq_kv8_sparse_attention(cache, 1, 0x300, top, top, 0x400, *tail))
+
+    assert calls(129, 128, 2 ** 24 - 1, 2 ** 31 - 1) == (_lib.QQ_ERR_UNSUPPORTED,) * 2
+    assert calls(127, 128, 2 ** 24 - 1, 2 ** 31 - 1) == (_lib.QQ_ERR_WORKSPACE,) * 2
