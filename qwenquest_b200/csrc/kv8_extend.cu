@@ -15,7 +15,7 @@
 // stretches whose (M, l, O) records kv8_extend_join_kernel merges.
 // Scales: as in the one-token kernel a score is S ks / up, the weight into
 // the V product 2^(s + lg - M) with lg = log2(vs), and the sum takes that
-// times 2^-lg: constants of a group of 16 keys (no block is shorter).
+// times 2^(-lg - kTop): constants of a group of 16 keys (no block is shorter).
 // Warps: 0-7 softmax (thread = row = TMEM lane; 0-3 tile 0, 4-7 tile 1),
 // 8-11 widen K and V, 12-13 MMA issue (one per M tile), 14 scales.
 // Tensor memory: per M tile S (128 fp32 columns, overlaid by P in fp16 once
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
   __shared__ Unit s_unit;
   __shared__ int s_record;  // of a stretch
   __shared__ float s_up[kUnitRows];                                   // scale_log2 / up of each row
-  __shared__ __align__(16) float4 s_scale[kMeta][kGroups];        // ks, lg, 2^-lg of 16 keys
+  __shared__ __align__(16) float4 s_scale[kMeta][kGroups];        // ks, lg, 2^(-lg - kTop) of 16 keys
   const AttnArgs& a = g.a;
   const Cache& c = a.c;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -533,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
     ok = __all_sync(0xffffffffu, ok && (tiles == 0 || wait(kBarDone + h, 0)));
     tc_fence_after();
     const bool record = u.splits > 1;
-    const float f = record ? alpha : (l == 0.f ? 0.f : alpha / l);
+    const float to_l = alpha * exp2f(-kTop), f = record ? to_l : (l == 0.f ? 0.f : to_l / l);
     float* rec = a.part + (int64_t)s_record * kRecord;
     if (record && ok && r < u.rows) rec[2 * r] = m, rec[2 * r + 1] = l;
     const int rows = ok ? u.rows : 0;
@@ -674,10 +674,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_extend_kernel(ExtendArgs g) {
         if (b >= 0 && b < c.num_blocks) {
           const int bh = b * c.kv_heads + kvh;
           f.x = c.k_scale[bh];
-          // 2^-lg stays a normal number
+          // 2^-lg stays a normal number; times 2^-kTop, or l of 2^20 keys of blocks of zeros would not be finite
           f.y = fminf(fmaxf(log2f(c.v_scale[bh]), -100.f), 126.f);
           if (isnan(c.v_scale[bh])) f.y = c.v_scale[bh];
-          f.z = exp2f(-f.y);
+          f.z = exp2f(-f.y - kTop);
         }
       }
       if (j >= kMeta && !__all_sync(0xffffffffu, wait(kBarMetaFree + m, ((j / kMeta) - 1) & 1))) break;

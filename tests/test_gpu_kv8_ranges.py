@@ -216,3 +216,32 @@ def test_each_kernel_within_its_own_bound(kv, heads, dim, block, dtype, seq):
                 n = s - new[i] + t + 1
                 row = offsets[i] + t
                 _check(ext[row], many[row], k[:n], v[:n], v_scale[:n], b.scaling, "extend" if tc else "fp32")
+
+
+@pytest.mark.parametrize("zeros", [1 << 12, 1 << 21])
+def test_keys_of_zero_values_before_the_first_others(zeros):
+    """Blocks of zeros have the smallest scale, 2^-126, and so the largest share of a row's sum for the reference that
+    they set: the sum stays finite over 2^21 of them, and the keys behind them get their part of the mass."""
+    kv, heads, dim, block, real, new = 1, 8, 128, 64, 128, 4800
+    n = zeros + new
+    cache = KV8Cache(1, 2 + new // block, kv, dim, DEV, block_size=block)
+    x = torch.zeros(block + new, kv, dim, device=DEV, dtype=torch.bfloat16)
+    v = torch.zeros_like(x)
+    v[block:block + real] = 1.0  # the first of the new tokens
+    cache.append(0, x, v, torch.arange(block + new, device=DEV))
+    assert cache.v_scale[0][0].item() == 2.0 ** -126
+    table = torch.cat([torch.zeros(zeros // block, dtype=torch.int32, device=DEV),
+                       torch.arange(1, 1 + new // block, dtype=torch.int32, device=DEV)])[None]
+    q = torch.ones(new, heads, dim, device=DEV, dtype=torch.bfloat16)  # all scores are 0: even weights
+    ext = cache.extend_attention(0, q, table, [0], [n], [zeros], [0], 0.1)
+    many = 300
+    lens = [zeros + real + 5] * many
+    full = cache.decode_attention(0, q[:many], table, [0] * many, lens, 0.1)
+    lone = cache.decode_attention(0, q[:1], table, [0], lens[:1], 0.1)
+    cache.synchronize()
+    seen = torch.arange(1, new + 1, device=DEV, dtype=torch.float64)
+    for got, want in ((ext, seen.clamp(max=real) / (zeros + seen)), (full, torch.full((many,), real / lens[0], device=DEV)),
+                      (lone, torch.full((1,), real / lens[0], device=DEV))):
+        want = want[:, None].double()
+        off = float(((got.double() - want).abs() / want).max())
+        assert off <= 2.0 ** -8 + 2.0 ** -9
